@@ -1,0 +1,520 @@
+// Decode attention over a paged 8-bit cache (layout and scales: kv_q8.cuh): one query token per sequence,
+//
+//   o_h = sum_t p_t v_t,  p = softmax_t(scale q_h . k_t),  k_t = s_K(block of t) K[t],  v_t = s_V(block of t) V[t],  t < len.
+//
+// Bound by HBM: a cached token and KV head is 256 bytes and 4 * 128 multiply-adds per query head. What has to fit beside the
+// loads is the conversion of every byte, so numbers go to f16 pairs (exact for both types, one instruction for two e4m3) and
+// both products run on warp-level m16n8k16 tensor-core tiles with the cache as the 16-row operand:
+//   S^T (16 tokens x 8 heads) = K (16 x 128) Q^T,   O^T (128 x 8 heads) += V^T (128 x 16) P^T.
+// Both sums run in an order of our choice, and so do the rows of O^T: a lane takes 16 consecutive bytes of a row wherever the
+// tile layout asks for some of its columns, with the query's columns permuted alike, so that cached bytes go from global
+// memory to the lane that multiplies them without a transposition (V^T pairs two tokens' bytes with a byte permutation).
+//
+// The scales stay out of the products: s_K multiplies a token's scores, and s_V enters the exponent, w_t = p_t s_V(t) =
+// 2^15 exp2(x_t + log2 s_V(t) - M) with M the running maximum of that sum: whatever the scales, the weights that are rounded to
+// f16 are at most 2^15, and those down to 2^-29 of the largest are exact to 2^-11, smaller ones to 2^-40 of the largest. The
+// softmax's own sum is sum_t w_t / s_V(t), in fp32.
+// The query is brought to f16 by a power of two per head that puts its largest element into [2^7, 2^8): exact for elements down
+// to 2^-22 of the largest, whose bf16 significands f16 holds whole.
+//
+// A warp takes every fourth tile of 16 tokens of its CTA's run and keeps a ring of them in flight with asynchronous 16-byte copies;
+// a lane reads back only what it copied itself, so no barrier stands in the loop.
+#include <float.h>
+
+#include "../common/host.h"
+#include "../common/ptx.cuh"
+#include "../common/rope.cuh"
+#include "../mlf_api.h"
+#include "kv_q8.cuh"
+
+namespace mlf {
+
+constexpr int DQ_WARPS = 4;
+constexpr int DQ_THREADS = DQ_WARPS * 32;
+constexpr int DQ_TILE = 16;                                  // tokens
+constexpr int DQ_STAGES = 4;                                 // tiles in flight per warp
+constexpr int DQ_STAGE_BYTES = 2 * DQ_TILE * Q8_D + 128;     // keys, values, 16 + 16 scales
+constexpr int DQ_SMEM = DQ_WARPS * DQ_STAGES * DQ_STAGE_BYTES;
+constexpr float DQ_UP = 15.f;                                // log2 of the largest weight
+constexpr int DQ_RED = Q8_D + 2;                             // floats of a partial result: maximum, sum, output
+
+struct DecodeQ8Params {
+  const __nv_bfloat16* q;         // [B, Hq, 128], row pitch ldq elements
+  long long ldq;
+  uint8_t* cache;
+  float* scale;
+  const int* block_table;         // [B, max_blocks]
+  const int* seq_lens;            // [B]
+  __nv_bfloat16* out;             // [B, Hq, 128]
+  float* ws;                      // [B, Hkv, splits, G, 130] (m, l, o[128]) when splits > 1
+  int B, Hq, Hkv, G, block_size, max_blocks, num_blocks, splits, unit;   // unit: tokens that a split is a multiple of
+  float scale_log2;
+  int* err;
+  // packed form: unrotated heads of packed QKV rows; the newest token goes to slots[b]
+  const __nv_bfloat16* k_new;
+  const __nv_bfloat16* v_new;
+  const long long* slots;
+  float theta;
+  int early;
+};
+
+__device__ __forceinline__ void dq_copy16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void dq_copy4(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void dq_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void dq_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+// D(16x8, fp32) += A(16x16, f16, row) B(16x8, f16, col)
+__device__ __forceinline__ void dq_mma(float (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ unsigned dq_transpose(unsigned a) {    // an 8 x 8 matrix of f16, a row's pair per lane
+  unsigned d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+__device__ __forceinline__ unsigned dq_half2(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const unsigned*>(&h);
+}
+
+// The newest token's key (side 0: rotated) or value, in 8 bits: a warp, four elements a lane. Its block's scale is settled as a
+// cache write would (a block's first row starts it anew; a larger scale rounds the held rows again), and the row is written;
+// a row without a slot has a scale of its own. Returns the four bytes and the scale that they stand in.
+template <int FMT>
+__device__ __forceinline__ unsigned q8_append_row(const DecodeQ8Params& p, float (&x)[4], int hkv, int side, long long slot, float& now) {
+  const int lane = threadIdx.x & 31;
+  float amax = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  now = q8_scale_for<FMT>(amax);
+  uint8_t* dst = nullptr;
+  if (slot >= 0) {
+    const long long blk = slot / p.block_size;
+    if (blk >= p.num_blocks) {
+      if (lane == 0) atomicCAS(p.err, 0, ERR_BAD_INDEX);
+    } else {
+      const int off = (int)(slot - blk * p.block_size);
+      const long long pitch = (long long)p.Hkv * Q8_D;
+      uint8_t* rows = p.cache + ((blk * 2 + side) * p.block_size * p.Hkv + hkv) * Q8_D + lane * 4;
+      float* sc = p.scale + (blk * 2 + side) * p.Hkv + hkv;
+      dst = rows + off * pitch;
+      if (off > 0) {
+        const float before = *sc;
+        if (before < now) {
+          const float ratio = before * __frcp_rn(now);
+          for (int r = 0; r < p.block_size; ++r) {
+            if (r == off) continue;
+            unsigned* w = reinterpret_cast<unsigned*>(rows + r * pitch);
+            *w = q8_shrink4<FMT>(*w, ratio);
+          }
+        }
+        now = fmaxf(before, now);
+      }
+      __syncwarp();                // every lane has read the old scale
+      if (lane == 0) *sc = now;
+    }
+  }
+  const float inv = __frcp_rn(now);
+  const unsigned w = q8_pack4<FMT>(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+  if (dst != nullptr) *reinterpret_cast<unsigned*>(dst) = w;
+  return w;
+}
+
+// NT: tiles of eight query heads (the group's heads, zero-padded).
+template <int FMT, int NT, bool ROPE>
+__global__ void __launch_bounds__(DQ_THREADS)
+paged_decode_q8_kernel(const DecodeQ8Params p) {
+  extern __shared__ __align__(128) uint8_t dq_smem[];
+  __shared__ __align__(16) uint8_t s_new[2][Q8_D];
+  __shared__ float s_new_scale[2];
+  __shared__ float2 s_cs[ROPE ? Q8_D / 2 : 1];
+  const int b = blockIdx.x, hkv = blockIdx.y, sp = blockIdx.z;
+  pdl_trigger();
+  // Lengths, table and cached rows may be read ahead of the kernels before this one where those do not write them.
+  const bool early = ROPE && p.early != 0;
+  if (!early) pdl_wait();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int g = lane >> 2, c = lane & 3;
+  int len = p.seq_lens[b];
+  const long long cap = (long long)p.max_blocks * p.block_size;
+  if (len < 0 || len > cap) {                  // beyond what the table's row can describe: clamped and reported
+    if (tid == 0) atomicCAS(p.err, 0, ERR_BAD_INDEX);
+    len = len < 0 ? 0 : (int)cap;
+  }
+  // a split is a whole number of blocks, so that a block whose scale grows with its newest row is read by one CTA alone
+  const int per = ((len + p.splits - 1) / p.splits + p.unit - 1) / p.unit * p.unit;
+  const int t_lo = min(len, sp * per), t_hi = min(len, t_lo + per);
+  float* ws = p.ws ? p.ws + (((long long)b * p.Hkv + hkv) * p.splits + sp) * p.G * DQ_RED : nullptr;
+  if (t_lo >= t_hi) {
+    if (early) pdl_wait();
+    if (ws) {
+      for (int i = tid; i < p.G * DQ_RED; i += DQ_THREADS) ws[i] = i % DQ_RED == 0 ? -INFINITY : 0.f;
+    } else {
+      for (int i = tid; i < p.G * Q8_D; i += DQ_THREADS) p.out[((long long)b * p.Hq + hkv * p.G) * Q8_D + i] = __float2bfloat16(0.f);
+    }
+    return;
+  }
+  const int* bt = p.block_table + (long long)b * p.max_blocks;
+  const long long v_off = (long long)p.block_size * p.Hkv * Q8_D, blk_bytes = 2 * v_off;
+  const int tiles = (t_hi - t_lo + DQ_TILE - 1) / DQ_TILE;
+  const int mine = tiles > warp ? (tiles - warp + DQ_WARPS - 1) / DQ_WARPS : 0;      // tiles warp, warp + 4, ...
+  const uint32_t ring = smem_u32(dq_smem) + warp * DQ_STAGES * DQ_STAGE_BYTES;
+  uint8_t* ring_p = dq_smem + warp * DQ_STAGES * DQ_STAGE_BYTES;
+  const bool has_new = ROPE && t_hi == len;
+  // tiles that reach into the newest token's block wait until that token is written
+  const int held_back = has_new ? (len - 1) / p.block_size * p.block_size : 0x7fffffff;
+
+  auto issue = [&](int i) {                    // this warp's i-th tile
+    const int t0 = t_lo + (warp + i * DQ_WARPS) * DQ_TILE;
+    const uint32_t st = ring + (i % DQ_STAGES) * DQ_STAGE_BYTES;
+    const int t = t0 + (lane & 15);
+    const bool there = t < t_hi;
+    int page = (there ? t : t0) / p.block_size;
+    const int row = (there ? t : t0) - page * p.block_size;
+    page = bt[page];
+    if (page < 0 || page >= p.num_blocks) { atomicCAS(p.err, 0, ERR_BAD_INDEX); page = 0; }
+    const int at = there ? row : -1;
+    dq_copy4(st + 2 * DQ_TILE * Q8_D + lane * 4, p.scale + ((long long)page * 2 + (lane >> 4)) * p.Hkv + hkv, there ? 4 : 0);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {              // rows g and g + 8 of the keys, 16-byte columns c and c + 4
+      const int pg = __shfl_sync(0xffffffffu, page, g + 8 * j), r = __shfl_sync(0xffffffffu, at, g + 8 * j);
+      const uint8_t* src = p.cache + pg * blk_bytes + ((long long)max(r, 0) * p.Hkv + hkv) * Q8_D + c * 16;
+      dq_copy16(st + (j * 2) * 512 + lane * 16, src, r >= 0 ? 16 : 0);
+      dq_copy16(st + (j * 2 + 1) * 512 + lane * 16, src + 64, r >= 0 ? 16 : 0);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {              // rows 2c, 2c + 1, 2c + 8, 2c + 9 of the values, column g
+      const int tr = 2 * c + (j & 1) + 8 * (j >> 1);
+      const int pg = __shfl_sync(0xffffffffu, page, tr), r = __shfl_sync(0xffffffffu, at, tr);
+      dq_copy16(st + DQ_TILE * Q8_D + j * 512 + lane * 16, p.cache + pg * blk_bytes + v_off + ((long long)max(r, 0) * p.Hkv + hkv) * Q8_D + g * 16,
+                r >= 0 ? 16 : 0);
+    }
+  };
+  auto late = [&](int i) { return has_new && t_lo + (warp + i * DQ_WARPS) * DQ_TILE + DQ_TILE > held_back; };
+#pragma unroll
+  for (int i = 0; i < DQ_STAGES; ++i) {
+    if (i < mine && !late(i)) issue(i);
+    dq_commit();
+  }
+  if (ROPE) {
+    if (tid < Q8_D / 2) s_cs[tid] = rope_cos_sin((float)(len - 1), __logf(p.theta), rope_exponent<Q8_D>(tid));
+    __syncthreads();
+  }
+  if (early) pdl_wait();
+  long long slot = -1;
+  if (has_new) {
+    slot = p.slots[b];
+    if (warp < 2) {
+      const __nv_bfloat16* src = (warp ? p.v_new : p.k_new) + (long long)b * p.ldq + (long long)hkv * Q8_D + lane * 4;
+      const uint2 own = *reinterpret_cast<const uint2*>(src);
+      float2 u = unpack_bf16x2(own.x), v = unpack_bf16x2(own.y);
+      float x[4] = {u.x, u.y, v.x, v.y};
+      if (warp == 0) {                         // rotated and rounded to bf16, as a cache write takes it
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float other = __shfl_xor_sync(0xffffffffu, x[j], 16);
+          float lo = lane < 16 ? x[j] : other, hi = lane < 16 ? other : x[j];
+          rope_rotate(lo, hi, s_cs[(lane & 15) * 4 + j]);
+          x[j] = __bfloat162float(__float2bfloat16(lane < 16 ? lo : hi));
+        }
+      }
+      float now;
+      const unsigned w = q8_append_row<FMT>(p, x, hkv, warp, slot, now);
+      *reinterpret_cast<unsigned*>(&s_new[warp][lane * 4]) = w;
+      if (lane == 0) s_new_scale[warp] = now;
+      __threadfence();                         // the copies below read past the L1
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < DQ_STAGES; ++i)
+      if (i < mine && late(i)) issue(i);
+    dq_commit();
+  }
+
+  // Q^T as the B operand: head n = g of each tile of eight, the 32 elements that this lane's pieces of a key row hold
+  unsigned qb[NT][8][2];
+  float qf[NT][2];                             // of heads 2c and 2c + 1: power of two taken out, softmax scale, log2 e
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int head = n * 8 + g;
+    float x[32];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        // rows are 4-byte aligned at least
+        float2 a = make_float2(0.f, 0.f), e = a;
+        if (head < p.G) {
+          const uint32_t* src = reinterpret_cast<const uint32_t*>(p.q + (long long)b * p.ldq + (long long)(hkv * p.G + head) * Q8_D + h * 64 + c * 16 + j * 4);
+          a = unpack_bf16x2(src[0]);
+          e = unpack_bf16x2(src[1]);
+        }
+        x[h * 16 + j * 4] = a.x; x[h * 16 + j * 4 + 1] = a.y; x[h * 16 + j * 4 + 2] = e.x; x[h * 16 + j * 4 + 3] = e.y;
+      }
+    if (ROPE) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        rope_rotate(x[j], x[16 + j], s_cs[c * 16 + j]);
+        x[j] = __bfloat162float(__float2bfloat16(x[j]));
+        x[16 + j] = __bfloat162float(__float2bfloat16(x[16 + j]));
+      }
+    }
+    float amax = 0.f;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) amax = fmaxf(amax, fabsf(x[j]));
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+    int e = (int)(__float_as_uint(amax) >> 23) - 127;          // largest element in [2^e, 2^(e+1))
+    e = max(-100, min(120, e));
+    const float up = __uint_as_float((unsigned)(127 + 7 - e) << 23), down = __uint_as_float((unsigned)(127 - 7 + e) << 23);
+#pragma unroll
+    for (int ks = 0; ks < 8; ++ks) {
+      qb[n][ks][0] = dq_half2(x[ks * 4] * up, x[ks * 4 + 1] * up);
+      qb[n][ks][1] = dq_half2(x[ks * 4 + 2] * up, x[ks * 4 + 3] * up);
+    }
+    qf[n][0] = __shfl_sync(0xffffffffu, down, 8 * c) * p.scale_log2;         // the lane of head 2c, then of 2c + 1
+    qf[n][1] = __shfl_sync(0xffffffffu, down, 8 * c + 4) * p.scale_log2;
+  }
+
+  float o[NT][8][4];
+  float m_run[NT][2], l_run[NT][2];            // of heads 2c, 2c + 1 (l: this lane's tokens only)
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+#pragma unroll
+    for (int mt = 0; mt < 8; ++mt) o[n][mt][0] = o[n][mt][1] = o[n][mt][2] = o[n][mt][3] = 0.f;
+    m_run[n][0] = m_run[n][1] = -INFINITY;
+    l_run[n][0] = l_run[n][1] = 0.f;
+  }
+
+  for (int i = 0; i < mine; ++i) {
+    if (has_new && late(i)) dq_wait<0>();      // its group is not the i-th one
+    else dq_wait<DQ_STAGES - 1>();
+    __syncwarp();                              // the scales are other lanes' copies
+    uint8_t* st = ring_p + (i % DQ_STAGES) * DQ_STAGE_BYTES;
+    const int t0 = t_lo + (warp + i * DQ_WARPS) * DQ_TILE;
+    const float* sc = reinterpret_cast<const float*>(st + 2 * DQ_TILE * Q8_D);
+    float ks0 = sc[g], ks1 = sc[g + 8], vs0 = sc[16 + g], vs1 = sc[16 + g + 8];
+    if (ROPE && slot < 0 && has_new && len - 1 >= t0 && len - 1 < t0 + DQ_TILE) {   // a newest token that is nowhere in the cache
+      const int r = len - 1 - t0;
+      if ((r & 7) == g) {
+        uint8_t* kd = st + (r >> 3) * 1024 + lane * 16;
+        *reinterpret_cast<uint4*>(kd) = *reinterpret_cast<const uint4*>(&s_new[0][c * 16]);
+        *reinterpret_cast<uint4*>(kd + 512) = *reinterpret_cast<const uint4*>(&s_new[0][64 + c * 16]);
+        if (r < 8) { ks0 = s_new_scale[0]; vs0 = s_new_scale[1]; }
+        else { ks1 = s_new_scale[0]; vs1 = s_new_scale[1]; }
+      }
+      if (((r & 7) >> 1) == c)
+        *reinterpret_cast<uint4*>(st + DQ_TILE * Q8_D + ((r & 1) + 2 * (r >> 3)) * 512 + lane * 16) = *reinterpret_cast<const uint4*>(&s_new[1][g * 16]);
+    }
+    const bool in0 = t0 + g < t_hi, in1 = t0 + g + 8 < t_hi;
+    // a block of zeros (or one that was never written) may have any scale: 2^-60 stands for what is smaller
+    vs0 = fminf(fmaxf(vs0, 8.6736174e-19f), 1.1529215e18f);
+    vs1 = fminf(fmaxf(vs1, 8.6736174e-19f), 1.1529215e18f);
+    const float lv0 = __log2f(vs0), lv1 = __log2f(vs1), iv0 = __frcp_rn(vs0), iv1 = __frcp_rn(vs1);
+    float s[NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {              // 64 of the key's 128 columns
+      const uint4 a = *reinterpret_cast<const uint4*>(st + h * 512 + lane * 16), e = *reinterpret_cast<const uint4*>(st + (2 + h) * 512 + lane * 16);
+      const unsigned aw[4] = {a.x, a.y, a.z, a.w}, ew[4] = {e.x, e.y, e.z, e.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        unsigned a0, a2, a1, a3;
+        q8_unpack4<FMT>(aw[j], a0, a2);
+        q8_unpack4<FMT>(ew[j], a1, a3);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) dq_mma(s[n], a0, a1, a2, a3, qb[n][h * 4 + j][0], qb[n][h * 4 + j][1]);
+      }
+    }
+    unsigned pb[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      // s: tokens g (0, 1) and g + 8 (2, 3), heads 2c and 2c + 1
+      s[n][0] = in0 ? fmaf(s[n][0] * qf[n][0], ks0, lv0) : -INFINITY;
+      s[n][1] = in0 ? fmaf(s[n][1] * qf[n][1], ks0, lv0) : -INFINITY;
+      s[n][2] = in1 ? fmaf(s[n][2] * qf[n][0], ks1, lv1) : -INFINITY;
+      s[n][3] = in1 ? fmaf(s[n][3] * qf[n][1], ks1, lv1) : -INFINITY;
+      float alpha[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float mx = fmaxf(s[n][e], s[n][2 + e]);
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+        const float m_new = fmaxf(m_run[n][e], mx);
+        const float m_use = m_new == -INFINITY ? 0.f : m_new - DQ_UP;
+        alpha[e] = exp2f(m_run[n][e] - DQ_UP - m_use);
+        m_run[n][e] = m_new;
+        s[n][e] = exp2f(s[n][e] - m_use);
+        s[n][2 + e] = exp2f(s[n][2 + e] - m_use);
+        l_run[n][e] = l_run[n][e] * alpha[e] + s[n][e] * iv0 + s[n][2 + e] * iv1;
+      }
+#pragma unroll
+      for (int mt = 0; mt < 8; ++mt) {
+        o[n][mt][0] *= alpha[0]; o[n][mt][1] *= alpha[1];
+        o[n][mt][2] *= alpha[0]; o[n][mt][3] *= alpha[1];
+      }
+      // rows are tokens here and columns in the next product
+      pb[n][0] = dq_transpose(dq_half2(s[n][0], s[n][1]));
+      pb[n][1] = dq_transpose(dq_half2(s[n][2], s[n][3]));
+    }
+    uint4 v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const uint4*>(st + DQ_TILE * Q8_D + j * 512 + lane * 16);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {              // rows 16 g + 4 j .. + 3 of O^T
+      const unsigned t0w = (&v[0].x)[j], t1w = (&v[1].x)[j], t8w = (&v[2].x)[j], t9w = (&v[3].x)[j];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {            // two tokens' bytes side by side: rows 4 j + 2 h, 4 j + 2 h + 1
+        unsigned a0, a1, a2, a3;
+        q8_unpack4<FMT>(__byte_perm(t0w, t1w, h ? 0x7362 : 0x5140), a0, a1);
+        q8_unpack4<FMT>(__byte_perm(t8w, t9w, h ? 0x7362 : 0x5140), a2, a3);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) dq_mma(o[n][j * 2 + h], a0, a1, a2, a3, pb[n][0], pb[n][1]);
+      }
+    }
+    __syncwarp();                              // the scales of this stage have been read
+    if (i + DQ_STAGES < mine) issue(i + DQ_STAGES);
+    dq_commit();
+  }
+  dq_wait<0>();
+  __syncthreads();                             // the rings are free
+  // ---- merge the four warps: red[warp][head][m, l, o[128]]
+  float* red = reinterpret_cast<float*>(dq_smem);
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float l = l_run[n][e];
+      l += __shfl_xor_sync(0xffffffffu, l, 4);
+      l += __shfl_xor_sync(0xffffffffu, l, 8);
+      l += __shfl_xor_sync(0xffffffffu, l, 16);
+      const int head = n * 8 + 2 * c + e;
+      if (head < p.G) {
+        float* r = red + ((long long)warp * p.G + head) * DQ_RED;
+        if (g == 0) { r[0] = m_run[n][e]; r[1] = l; }
+#pragma unroll
+        for (int mt = 0; mt < 8; ++mt) {
+          r[2 + g * 16 + 2 * mt] = o[n][mt][e];
+          r[2 + g * 16 + 2 * mt + 1] = o[n][mt][2 + e];
+        }
+      }
+    }
+  __syncthreads();
+  for (int i = tid; i < p.G * Q8_D; i += DQ_THREADS) {
+    const int h = i / Q8_D, d = i % Q8_D;
+    float M = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < DQ_WARPS; ++w) M = fmaxf(M, red[(w * p.G + h) * DQ_RED]);
+    const float M_use = M == -INFINITY ? 0.f : M;
+    float acc = 0.f, l = 0.f;
+#pragma unroll
+    for (int w = 0; w < DQ_WARPS; ++w) {
+      const float* r = red + (w * p.G + h) * DQ_RED;
+      const float f = exp2f(r[0] - M_use);     // a warp without tokens has m = -inf, l = 0, o = 0
+      acc += f * r[2 + d];
+      l += f * r[1];
+    }
+    if (ws) {
+      ws[h * DQ_RED + 2 + d] = acc;
+      if (d == 0) { ws[h * DQ_RED] = M; ws[h * DQ_RED + 1] = l; }
+    } else {
+      p.out[((long long)b * p.Hq + hkv * p.G + h) * Q8_D + d] = __float2bfloat16(l > 0.f ? acc / l : 0.f);
+    }
+  }
+}
+
+// out = sum_s exp2(m_s - M) o_s / sum_s exp2(m_s - M) l_s over the splits of a sequence and head
+__global__ void __launch_bounds__(Q8_D)
+paged_decode_q8_merge_kernel(const float* ws, __nv_bfloat16* out, int Hq, int Hkv, int G, int splits) {
+  pdl_trigger();
+  pdl_wait();
+  const int b = blockIdx.x / Hq, h = blockIdx.x % Hq, d = threadIdx.x;
+  const float* base = ws + (((long long)b * Hkv + h / G) * splits * G + h % G) * DQ_RED;
+  const long long sstride = (long long)G * DQ_RED;
+  float M = -INFINITY;
+  for (int s = 0; s < splits; ++s) M = fmaxf(M, base[s * sstride]);
+  float L = 0.f, o = 0.f;
+  for (int s = 0; s < splits; ++s) {
+    const float m = base[s * sstride];
+    if (m == -INFINITY) continue;
+    const float w = exp2f(m - M);
+    L += w * base[s * sstride + 1];
+    o += w * base[s * sstride + 2 + d];
+  }
+  out[(long long)blockIdx.x * Q8_D + d] = __float2bfloat16(L > 0.f ? o / L : 0.f);
+}
+
+}  // namespace mlf
+
+using namespace mlf;
+
+MLF_API long long mlf_paged_decode_q8_ws_elems(int B, int Hq, int splits) { return (long long)B * Hq * splits * DQ_RED; }
+
+// One query token per sequence over an 8-bit cache. Without slots: q [B, Hq, 128], row pitch ldq. With slots (the packed form): q is
+// the QKV product [B, (Hq + 2 Hkv) * 128], not yet rotated; the newest token of a sequence, the last of its seq_lens, is rotated at
+// position seq_lens - 1, written to its slot (< 0: not written) as mlf_kv_write_q8 would and attended to like the cached ones.
+// fmt: 0 e4m3, 1 int8. splits > 1 needs ws. inputs_static: as for mlf_paged_decode_rope.
+MLF_API int mlf_paged_decode_q8(const void* q, long long ldq, void* cache, float* scale, int fmt, const int* block_table, const int* seq_lens,
+                                const long long* slots, void* out, float* ws, int B, int Hq, int Hkv, int block_size, int max_blocks, int num_blocks,
+                                int splits, float softmax_scale, float theta, int inputs_static, uint64_t stream) {
+  if (B <= 0) return 0;
+  MLF_REQUIRE(fmt == Q8_E4M3 || fmt == Q8_INT8, "paged_decode_q8: format %d", fmt);
+  MLF_REQUIRE(Hkv > 0 && Hq > 0 && Hq % Hkv == 0, "paged_decode_q8: bad head counts %d, %d", Hq, Hkv);
+  const int G = Hq / Hkv;
+  MLF_REQUIRE(G <= 16, "paged_decode_q8: group size %d not supported (1 to 16)", G);
+  MLF_REQUIRE(block_size > 0 && max_blocks > 0 && num_blocks > 0 && splits > 0, "paged_decode_q8: bad sizes");
+  MLF_REQUIRE((long long)max_blocks * block_size < (1LL << 31) - (1 << 20), "paged_decode_q8: block table of %d x %d tokens", max_blocks, block_size);
+  MLF_REQUIRE(Hkv <= 65535 && splits <= 65535, "paged_decode_q8: grid");
+  MLF_REQUIRE(splits == 1 || ws != nullptr, "paged_decode_q8: workspace required for %d splits", splits);
+  MLF_REQUIRE((reinterpret_cast<uintptr_t>(cache) & 15) == 0, "paged_decode_q8: the cache must be 16-byte aligned");
+  const bool rope = slots != nullptr;
+  MLF_REQUIRE(rope ? ldq % 4 == 0 && (reinterpret_cast<uintptr_t>(q) & 7) == 0 && theta > 0.f : ldq % 2 == 0 && (reinterpret_cast<uintptr_t>(q) & 3) == 0,
+              "paged_decode_q8: query rows must be %d-byte aligned", rope ? 8 : 4);
+  DecodeQ8Params p;
+  p.q = static_cast<const __nv_bfloat16*>(q);
+  p.ldq = ldq;
+  p.cache = static_cast<uint8_t*>(cache);
+  p.scale = scale;
+  p.block_table = block_table; p.seq_lens = seq_lens;
+  p.out = static_cast<__nv_bfloat16*>(out);
+  p.ws = splits > 1 ? ws : nullptr;
+  p.B = B; p.Hq = Hq; p.Hkv = Hkv; p.G = G; p.block_size = block_size; p.max_blocks = max_blocks; p.num_blocks = num_blocks;
+  p.splits = splits;
+  p.unit = block_size * ((DQ_WARPS * DQ_TILE + block_size - 1) / block_size);
+  p.scale_log2 = softmax_scale * 1.4426950408889634f;
+  p.err = device_status_word();
+  p.k_new = rope ? p.q + (long long)Hq * Q8_D : nullptr;
+  p.v_new = rope ? p.k_new + (long long)Hkv * Q8_D : nullptr;
+  p.slots = slots;
+  p.theta = theta;
+  p.early = inputs_static;
+  void (*const kernels[2][2][2])(DecodeQ8Params) = {
+      {{paged_decode_q8_kernel<Q8_E4M3, 1, false>, paged_decode_q8_kernel<Q8_E4M3, 1, true>},
+       {paged_decode_q8_kernel<Q8_E4M3, 2, false>, paged_decode_q8_kernel<Q8_E4M3, 2, true>}},
+      {{paged_decode_q8_kernel<Q8_INT8, 1, false>, paged_decode_q8_kernel<Q8_INT8, 1, true>},
+       {paged_decode_q8_kernel<Q8_INT8, 2, false>, paged_decode_q8_kernel<Q8_INT8, 2, true>}}};
+  const auto kernel = kernels[fmt][G > 8 ? 1 : 0][rope ? 1 : 0];
+  static bool attr_set[64][8] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  bool& set = attr_set[dev & 63][fmt * 4 + (G > 8 ? 2 : 0) + (rope ? 1 : 0)];
+  if (!set) {
+    MLF_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, DQ_SMEM));
+    set = true;
+  }
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  MLF_CHECK_CUDA(launch_pdl(kernel, dim3(B, Hkv, splits), dim3(DQ_THREADS), DQ_SMEM, st, p));
+  count_launch();
+  if (splits > 1) {
+    MLF_CHECK_CUDA(launch_pdl(paged_decode_q8_merge_kernel, dim3((unsigned)(B * Hq)), dim3(Q8_D), 0, st, (const float*)ws, p.out, Hq, Hkv, G, splits));
+    count_launch();
+  }
+  return 0;
+}

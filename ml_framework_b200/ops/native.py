@@ -8,8 +8,10 @@ The PyTorch statements of the same math, used on CPU tensors and as test oracles
 from __future__ import annotations
 
 import ctypes as C
+from array import array
 from functools import lru_cache
-from typing import Optional
+from itertools import chain
+from typing import Optional, Sequence, Tuple
 
 import torch
 
@@ -393,6 +395,49 @@ def flash_bwd(q, k, v, o, dout, lse, B: int, S: int, *, causal: bool = True, sca
 
 
 # ------------------------------------------------------------------ paged attention / KV cache
+_Q8 = {torch.float8_e4m3fn: 0, torch.int8: 1}
+
+
+def _on_current_device(what: str, *tensors: Optional[torch.Tensor]):
+    """Launches go to the current device's stream: tensors of another device, or of the host, are refused."""
+    for t in tensors:
+        if t is not None and not (t.is_cuda and t.device.index == torch._C._cuda_getDevice()):
+            raise ValueError(f"{what}: a tensor is on {t.device}, the kernel runs on the current CUDA device")
+
+
+def _q8_format(what: str, kv_cache: torch.Tensor, kv_scale: Optional[torch.Tensor]) -> int:
+    """Format of an 8-bit cache [num_blocks, 2, block_size, Hkv, 128] with its scales [num_blocks, 2, Hkv]."""
+    fmt = _Q8.get(kv_cache.dtype)
+    if fmt is None:
+        raise TypeError(f"{what}: scales belong to a cache of torch.float8_e4m3fn or torch.int8, not {kv_cache.dtype}")
+    if kv_cache.dim() != 5 or kv_cache.shape[1] != 2 or kv_cache.shape[4] != 128 or not kv_cache.is_contiguous():
+        raise ValueError(f"{what}: the cache must be contiguous [num_blocks, 2, block_size, kv_heads, 128], got {tuple(kv_cache.shape)}")
+    if kv_scale is None:
+        raise ValueError(f"{what}: a cache of {kv_cache.dtype} needs kv_scale")
+    want = (kv_cache.shape[0], 2, kv_cache.shape[3])
+    if tuple(kv_scale.shape) != want or kv_scale.dtype != torch.float32 or not kv_scale.is_contiguous():
+        raise ValueError(f"{what}: kv_scale must be contiguous float32 {want}, got {kv_scale.dtype} {tuple(kv_scale.shape)}")
+    return fmt
+
+
+def _index(what: str, name: str, t: torch.Tensor, dtype, shape) -> torch.Tensor:
+    if t.dtype != dtype or tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{what}: {name} must be {dtype} {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
+    return t.contiguous()
+
+
+def _heads(what: str, name: str, t: torch.Tensor, H: Optional[int] = None) -> torch.Tensor:
+    """bf16 [T, H, 128] whose tokens are whole rows at any pitch."""
+    if t.dim() != 3 or t.shape[2] != 128 or (H is not None and t.shape[1] != H) or t.dtype != torch.bfloat16:
+        raise ValueError(f"{what}: {name} must be bfloat16 [tokens, {'heads' if H is None else H}, 128], got {t.dtype} {tuple(t.shape)}")
+    return t if t.stride(2) == 1 and (t.stride(1) == 128 or t.shape[1] == 1) else t.contiguous()
+
+
+def _aligned_rows(t: torch.Tensor) -> torch.Tensor:
+    """``t`` with rows that start on 16 bytes: itself where they do."""
+    return t if t.data_ptr() % 16 == 0 and t.stride(0) % 8 == 0 else t.contiguous()
+
+
 @lru_cache(maxsize=None)
 def _sm_count(device_index: int) -> int:
     """SMs of the current device, whose index the caller passes."""
@@ -422,8 +467,40 @@ def _decode_split(pairs: int, max_seq_len: int, sms: int) -> int:
     return -(-max_seq_len // splits)
 
 
+def _decode_q8(what: str, q: torch.Tensor, ldq: int, Hq: int, kv_cache, kv_scale, block_table, seq_lens, slots, max_seq_len: int, scale, split_tokens: int,
+               theta: float, inputs_static: bool) -> torch.Tensor:
+    """Attention of :func:`paged_decode` (``slots`` None) and :func:`paged_decode_rope` over an 8-bit cache."""
+    fmt = _q8_format(what, kv_cache, kv_scale)
+    B, Hkv = q.shape[0], kv_cache.shape[3]
+    if Hq % Hkv or Hq // Hkv > 16:
+        raise ValueError(f"{what}: {Hq} query heads over {Hkv} KV heads (groups of 1 to 16)")
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != B:
+        raise ValueError(f"{what}: block_table must be int32 [{B}, max_blocks], got {block_table.dtype} {tuple(block_table.shape)}")
+    table, lens = block_table.contiguous(), _index(what, "seq_lens", seq_lens, torch.int32, (B,))
+    slots = _index(what, "slots", slots, torch.int64, (B,)) if slots is not None else None
+    _on_current_device(what, q, kv_cache, kv_scale, table, lens, slots)
+    out = torch.empty(B, Hq, 128, dtype=q.dtype, device=q.device)
+    if B == 0 or Hq == 0:
+        return out
+    if table.shape[1] == 0:
+        return out.zero_()
+    L = _L()
+    L.mlf_paged_decode_q8_ws_elems.restype = C.c_longlong
+    if split_tokens <= 0:
+        split_tokens = _decode_split(B * Hkv, max_seq_len, _sm_count(torch._C._cuda_getDevice()))
+    st = (max(split_tokens, 128) + 127) // 128 * 128
+    splits = max(1, (max_seq_len + st - 1) // st)
+    ws = torch.empty(int(L.mlf_paged_decode_q8_ws_elems(B, Hq, splits)), dtype=torch.float32, device=q.device) if splits > 1 else None
+    rc = L.mlf_paged_decode_q8(_p(q), C.c_longlong(ldq), _p(kv_cache), _p(kv_scale), fmt, _p(table), _p(lens), _p(slots), _p(out), _p(ws), B, Hq, Hkv,
+                               kv_cache.shape[2], table.shape[1], kv_cache.shape[0], splits, C.c_float(scale if scale is not None else 128 ** -0.5),
+                               C.c_float(theta), int(inputs_static), _st())
+    _lib.check(rc, "mlf_paged_decode_q8")
+    return out
+
+
 def paged_decode(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
-                 max_seq_len: int, *, scale: Optional[float] = None, split_tokens: int = 512, fused_merge: bool = False) -> torch.Tensor:
+                 max_seq_len: int, *, scale: Optional[float] = None, split_tokens: int = 512, fused_merge: bool = False,
+                 kv_scale: Optional[torch.Tensor] = None) -> torch.Tensor:
     """One query token per sequence against its paged KV cache.
 
     q [B, Hq, 128]; kv_cache [num_blocks, 2, block_size, Hkv, 128]; block_table int32 [B, max_blocks];
@@ -432,7 +509,16 @@ def paged_decode(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Ten
     ``split_tokens`` <= 0 picks the split count from the batch size (enough CTAs to fill the GPU).
     ``fused_merge`` lets the last split of each (sequence, kv head) merge the splits inside the same launch instead of
     a second small kernel; it measured slower (57 us against 48 us at batch 64, 576 cached tokens), hence off.
+
+    An 8-bit cache (float8_e4m3fn or int8) comes with ``kv_scale``, float32 [num_blocks, 2, Hkv]: a value is its number times the
+    scale of its block, side (K, V) and head. Any positive scales; groups of 1 to 16 query heads per KV head; the splits
+    (a whole number of blocks each) are merged by a second kernel. A sequence of length 0 gives zeros.
     """
+    if kv_scale is not None or kv_cache.dtype in _Q8:
+        q = _heads("paged_decode", "q", q)
+        if q.data_ptr() % 4 or q.stride(0) % 2:
+            q = q.contiguous()
+        return _decode_q8("paged_decode", q, q.stride(0), q.shape[1], kv_cache, kv_scale, block_table, seq_lens, None, max_seq_len, scale, split_tokens, 0.0, False)
     B, Hq, D = q.shape
     nb, two, bs, Hkv, D2 = kv_cache.shape
     assert D == 128 and D2 == 128 and two == 2 and kv_cache.is_contiguous()
@@ -460,13 +546,26 @@ def paged_decode(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Ten
 
 
 def paged_decode_rope(qkv: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor, slots: torch.Tensor,
-                      Hq: int, Hkv: int, max_seq_len: int, theta: float, *, scale: Optional[float] = None, split_tokens: int = 0, inputs_static: bool = False) -> torch.Tensor:
+                      Hq: int, Hkv: int, max_seq_len: int, theta: float, *, scale: Optional[float] = None, split_tokens: int = 0, inputs_static: bool = False,
+                      kv_scale: Optional[torch.Tensor] = None) -> torch.Tensor:
     """:func:`rope_kv_write_` at positions ``seq_lens - 1`` followed by :func:`paged_decode` in one launch: ``qkv``
     [B, (Hq + 2 Hkv) * 128] holds the unrotated projection of each sequence's newest token, which ``seq_lens`` counts;
     its key and value go to cache slot ``slots`` (int64, < 0 skips the write). ``qkv`` is left as it is. ``inputs_static``:
     neither the last launch without programmatic overlap nor any launch after it writes ``block_table``, ``seq_lens`` or the
-    cached rows of earlier tokens, which may then be read ahead of the kernels before this one."""
+    cached rows of earlier tokens, which may then be read ahead of the kernels before this one.
+
+    With ``kv_scale`` (an 8-bit cache, see :func:`paged_decode`) the new rows are rounded to 8 bits as :func:`kv_cache_write` does
+    and attended to as they are then held; ``inputs_static`` speaks of the scales too."""
     B = qkv.shape[0]
+    if kv_scale is not None or kv_cache.dtype in _Q8:
+        what = "paged_decode_rope"
+        if qkv.dim() != 2 or qkv.dtype != torch.bfloat16 or qkv.shape[1] != (Hq + 2 * Hkv) * 128 or qkv.stride(1) != 1 or kv_cache.shape[3] != Hkv:
+            raise ValueError(f"{what}: qkv must be bfloat16 [B, ({Hq} + 2 * {Hkv}) * 128] beside a cache of {Hkv} heads, got {qkv.dtype} {tuple(qkv.shape)}")
+        if qkv.data_ptr() % 8 or qkv.stride(0) % 4 or not theta > 0:
+            raise ValueError(f"{what}: rows must be 8-byte aligned and theta positive")
+        if inputs_static and not (seq_lens.is_contiguous() and block_table.is_contiguous() and slots.is_contiguous()):
+            raise ValueError(f"{what}: inputs_static needs contiguous block_table, seq_lens and slots")      # a copy here would write them
+        return _decode_q8(what, qkv, qkv.stride(0), Hq, kv_cache, kv_scale, block_table, seq_lens, slots, max_seq_len, scale, split_tokens, theta, inputs_static)
     nb, two, bs, Hc, D = kv_cache.shape
     assert D == 128 and two == 2 and Hc == Hkv and kv_cache.is_contiguous() and qkv.shape[1] == (Hq + 2 * Hkv) * D
     assert qkv.stride(1) == 1 and qkv.dtype == torch.bfloat16 and kv_cache.dtype == torch.bfloat16 and slots.dtype == torch.int64
@@ -487,8 +586,32 @@ def paged_decode_rope(qkv: torch.Tensor, kv_cache: torch.Tensor, block_table: to
     return out
 
 
-def kv_cache_write(kv_cache: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor):
-    """Scatter k, v [T, Hkv, 128] into cache slots (slot = block * block_size + offset; < 0 skips)."""
+def kv_cache_write(kv_cache: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, kv_scale: Optional[torch.Tensor] = None):
+    """Scatter k, v [T, Hkv, 128] into cache slots (slot = block * block_size + offset; < 0 skips).
+
+    With ``kv_scale`` (an 8-bit cache, see :func:`paged_decode`) rows are rounded to numbers of 8 bits, ties to even, under one scale for
+    each block, side and head: the smallest power of two, from 2^-40 to 2^40, under which the largest magnitude fits (448 for e4m3,
+    127 for int8; larger values than 2^40 allows become the largest number). A call that writes a block's first row starts
+    the block anew: rows of it that the call does not write lose their meaning. A call that writes later rows only keeps the
+    larger of the block's scale and their own, and rounds the rows that the block holds to it. Rows of one block may
+    stand anywhere in the list; a slot given twice keeps one of its rows. NaN stays NaN in e4m3 and becomes 0 in int8."""
+    if kv_scale is not None or kv_cache.dtype in _Q8:
+        what = "kv_cache_write"
+        fmt = _q8_format(what, kv_cache, kv_scale)
+        k, v = _aligned_rows(_heads(what, "k", k, kv_cache.shape[3])), _aligned_rows(_heads(what, "v", v, kv_cache.shape[3]))
+        T = k.shape[0]
+        if v.shape[0] != T:
+            raise ValueError(f"{what}: {T} keys and {v.shape[0]} values")
+        slots = _index(what, "slots", slots, torch.int64, (T,))
+        _on_current_device(what, kv_cache, kv_scale, k, v, slots)
+        if T == 0 or kv_cache.numel() == 0:
+            return
+        nb, _, bs, Hkv, _ = kv_cache.shape
+        where = torch.empty(nb * bs, dtype=torch.int32, device=k.device)
+        rc = _L().mlf_kv_write_q8(_p(kv_cache), _p(kv_scale), fmt, _p(k), _p(v), _p(slots), _p(where), C.c_longlong(T), Hkv, bs, nb,
+                                  C.c_longlong(k.stride(0)), C.c_longlong(v.stride(0)), _st())
+        _lib.check(rc, "mlf_kv_write_q8")
+        return
     nb, _, bs, Hkv, D = kv_cache.shape
     T = k.shape[0]
     assert k.stride(2) == 1 and k.stride(1) == D and v.stride(2) == 1 and v.stride(1) == D
@@ -498,9 +621,26 @@ def kv_cache_write(kv_cache: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slo
     _lib.check(rc, "mlf_kv_cache_write")
 
 
-def rope_kv_write_(qkv: torch.Tensor, pos: torch.Tensor, slots: torch.Tensor, kv_cache: torch.Tensor, Hq: int, Hkv: int, theta: float):
+def rope_kv_write_(qkv: torch.Tensor, pos: torch.Tensor, slots: torch.Tensor, kv_cache: torch.Tensor, Hq: int, Hkv: int, theta: float,
+                   kv_scale: Optional[torch.Tensor] = None):
     """In place on packed ``qkv`` [T, (Hq + 2 Hkv) * 128]: rotary embedding of the query and key heads; the rotated
-    keys and the values are also written to their cache slots (one launch)."""
+    keys and the values are also written to their cache slots (one launch). With ``kv_scale`` (an 8-bit cache) the write is
+    :func:`kv_cache_write`'s, in launches of its own, and rows must be 16-byte aligned."""
+    if kv_scale is not None or kv_cache.dtype in _Q8:
+        what = "rope_kv_write_"
+        _q8_format(what, kv_cache, kv_scale)
+        T = qkv.shape[0]
+        if qkv.dim() != 2 or qkv.dtype != torch.bfloat16 or qkv.shape[1] != (Hq + 2 * Hkv) * 128 or qkv.stride(1) != 1 or kv_cache.shape[3] != Hkv:
+            raise ValueError(f"{what}: qkv must be bfloat16 [T, ({Hq} + 2 * {Hkv}) * 128] beside a cache of {Hkv} heads, got {qkv.dtype} {tuple(qkv.shape)}")
+        if qkv.data_ptr() % 16 or qkv.stride(0) % 8:
+            raise ValueError(f"{what}: rows must be 16-byte aligned")
+        pos, slots = _index(what, "pos", pos, torch.int64, (T,)), _index(what, "slots", slots, torch.int64, (T,))
+        _on_current_device(what, qkv, pos, slots, kv_cache, kv_scale)
+        if T == 0:
+            return qkv
+        rope_qkv(qkv, pos, Hq, Hkv, theta, out=qkv)
+        kv_cache_write(kv_cache, qkv[:, Hq * 128:(Hq + Hkv) * 128].view(T, Hkv, 128), qkv[:, (Hq + Hkv) * 128:].view(T, Hkv, 128), slots, kv_scale)
+        return qkv
     nb, _, bs, Hc, D = kv_cache.shape
     assert D == 128 and Hc == Hkv and qkv.dim() == 2 and qkv.stride(1) == 1 and qkv.shape[1] == (Hq + 2 * Hkv) * 128
     assert qkv.dtype == torch.bfloat16 and pos.dtype == torch.int64 and slots.dtype == torch.int64
@@ -511,8 +651,22 @@ def rope_kv_write_(qkv: torch.Tensor, pos: torch.Tensor, slots: torch.Tensor, kv
     return qkv
 
 
-def kv_gather(kv_cache: torch.Tensor, block_table_row: torch.Tensor, length: int):
-    """Contiguous (k, v) [length, Hkv, 128] of one sequence from its pages."""
+def kv_gather(kv_cache: torch.Tensor, block_table_row: torch.Tensor, length: int, kv_scale: Optional[torch.Tensor] = None):
+    """Contiguous (k, v) [length, Hkv, 128] of one sequence from its pages; in bf16 the values of an 8-bit cache (``kv_scale``)."""
+    if kv_scale is not None or kv_cache.dtype in _Q8:
+        what = "kv_gather"
+        fmt = _q8_format(what, kv_cache, kv_scale)
+        nb, _, bs, Hkv, _ = kv_cache.shape
+        row = _index(what, "block_table_row", block_table_row, torch.int32, (block_table_row.numel(),))
+        if not 0 <= length <= row.numel() * bs:
+            raise ValueError(f"{what}: {length} tokens, {row.numel()} block-table entries of {bs}")
+        _on_current_device(what, kv_cache, kv_scale, row)
+        k = torch.empty(length, Hkv, 128, dtype=torch.bfloat16, device=kv_cache.device)
+        v = torch.empty_like(k)
+        if length:
+            rc = _L().mlf_kv_gather_q8(_p(kv_cache), _p(kv_scale), fmt, _p(row), int(row.numel()), int(length), Hkv, bs, nb, _p(k), _p(v), _st())
+            _lib.check(rc, "mlf_kv_gather_q8")
+        return k, v
     nb, _, bs, Hkv, D = kv_cache.shape
     k = torch.empty(length, Hkv, D, dtype=kv_cache.dtype, device=kv_cache.device)
     v = torch.empty_like(k)
@@ -520,6 +674,28 @@ def kv_gather(kv_cache: torch.Tensor, block_table_row: torch.Tensor, length: int
     rc = _L().mlf_kv_gather(_p(kv_cache), _p(row), int(row.numel()), int(length), Hkv, bs, nb, _p(k), _p(v), _st())
     _lib.check(rc, "mlf_kv_gather")
     return k, v
+
+
+def kv_copy_blocks_(tensors: Sequence[torch.Tensor], pairs: Sequence[Tuple[int, int]]):
+    """``t[dst] = t[src]`` for every tensor (a layer's cache, or its scales; any type, ``[num_blocks, ...]`` alike) and every
+    (src, dst) of ``pairs``, in one launch for up to 64 tensors and 384 pairs. The pairs are host numbers. A block is written once
+    at most and none is both read and written, so that no order of the copies matters; anything else is refused."""
+    tensors = list(tensors)
+    flat = array("i", chain.from_iterable(pairs))
+    if len(flat) != 2 * len(pairs):
+        raise ValueError("kv_copy_blocks_: pairs must be (source, destination) block numbers")
+    if not tensors or not flat:
+        return
+    nb = tensors[0].shape[0] if tensors[0].dim() else 0
+    for t in tensors:
+        if t.numel() == 0 or t.shape[0] != nb or not t.is_contiguous():
+            raise ValueError(f"kv_copy_blocks_: tensors must be contiguous with the same number of blocks, got {tuple(t.shape)} beside {nb}")
+    _on_current_device("kv_copy_blocks_", *tensors)
+    bases = array("Q", [t.data_ptr() for t in tensors])
+    sizes = array("q", [t.numel() // nb * t.element_size() for t in tensors])
+    p = C.c_void_p
+    rc = _L().mlf_kv_copy_blocks(p(bases.buffer_info()[0]), p(sizes.buffer_info()[0]), len(tensors), p(flat.buffer_info()[0]), len(pairs), nb, _st())
+    _lib.check(rc, "mlf_kv_copy_blocks")
 
 
 def argmax_rows(logits: torch.Tensor, vocab: int) -> torch.Tensor:

@@ -96,6 +96,54 @@ def paged_attention_ref(q, kv_cache, block_table, seq_lens, *, scale=None):
     return torch.stack(outs)
 
 
+# ------------------------------------------------------------------ paged cache in 8 bits
+def q8_scale_ref(amax: torch.Tensor, dtype) -> torch.Tensor:
+    """The smallest power of two, 2^-40 to 2^40, under which magnitudes up to ``amax`` fit ``dtype`` (448 or 127)."""
+    frac, e = torch.frexp(amax.float())
+    top, bits = (448 / 512, 9) if dtype == torch.float8_e4m3fn else (127 / 128, 7)
+    e = torch.where(frac <= top, e - bits, e - bits + 1)
+    e = torch.where(amax == 0, torch.full_like(e, -40), torch.where(torch.isinf(amax), torch.full_like(e, 40), e)).clamp(-40, 40)
+    return torch.ldexp(torch.ones_like(amax, dtype=torch.float32), e)
+
+
+def q8_round_ref(x: torch.Tensor, dtype) -> torch.Tensor:
+    """Numbers in units of their scale rounded to 8 bits, ties to even; NaN stays in e4m3 and becomes 0 in int8."""
+    if dtype == torch.float8_e4m3fn:
+        return x.clamp(-448.0, 448.0).to(dtype)
+    return torch.nan_to_num(x, nan=0.0).round().clamp(-127.0, 127.0).to(dtype)
+
+
+def kv_values_ref(cache: torch.Tensor, scale: Optional[torch.Tensor]) -> torch.Tensor:
+    """The values of cache blocks [n, 2, block_size, Hkv, D] (all of a cache, or some blocks with their scales) in fp32."""
+    return cache.float() if scale is None else cache.float() * scale[:, :, None, :, None]
+
+
+def kv_write_ref(cache: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, scale: Optional[torch.Tensor] = None):
+    """k, v [T, Hkv, D] into cache slots (< 0 skips), in place. With ``scale`` (an 8-bit cache) the blocks' scales are settled first:
+    a block whose first row is written takes the new rows' own, another one the larger of that and its old scale, to which
+    the rows that it holds are rounded."""
+    bs = cache.shape[2]
+    ok = slots >= 0
+    blk, off = slots[ok] // bs, slots[ok] % bs
+    new = torch.stack((k[ok], v[ok]), 1)
+    if scale is None:
+        cache[blk, :, off] = new.to(cache.dtype)
+        return
+    new = new.float()
+    for b in torch.unique(blk).tolist():
+        at = blk == b
+        amax = torch.nan_to_num(new[at].abs(), nan=0.0, posinf=float("inf")).amax((0, 3))
+        now = q8_scale_ref(amax, cache.dtype)
+        if not bool((off[at] == 0).any()):
+            before = scale[b].clone()
+            now = torch.maximum(now, before)
+            grown = (before < now)[:, None, :, None]
+            held = cache[b].float()
+            cache[b] = q8_round_ref(torch.where(grown, held * (before / now)[:, None, :, None], held), cache.dtype)
+        scale[b] = now
+        cache[b][:, off[at]] = q8_round_ref(new[at] / now[None, :, :, None], cache.dtype).transpose(0, 1)
+
+
 def adamw_ref(p, m, v, g, *, lr, beta1, beta2, eps, weight_decay, step, vmax=None):
     """One AdamW step in fp32, decay first then the Adam update
     (src/MLFramework/Optimizers/Adam.cs:167-213). Returns new (p, m, v[, vmax])."""
