@@ -705,3 +705,34 @@ def argmax_rows(logits: torch.Tensor, vocab: int) -> torch.Tensor:
     rc = _L().mlf_argmax_rows(_p(logits), C.c_longlong(logits.shape[0]), C.c_longlong(logits.stride(0)), int(vocab), _p(out), _st())
     _lib.check(rc, "mlf_argmax_rows")
     return out
+
+
+def sample_rows(logits: torch.Tensor, vocab: int, u: torch.Tensor, temperature: torch.Tensor, top_k: Optional[torch.Tensor] = None,
+                top_p: Optional[torch.Tensor] = None, min_p: Optional[torch.Tensor] = None, want_logprobs: bool = False):
+    """Next tokens (int64 [rows]) from the first ``vocab`` columns of ``logits`` [rows, ld], bf16 or fp32, each row with settings of its own:
+    ``temperature`` (float32; 0 or less: the largest logit), ``top_k`` (int32; 0 or less: no limit), ``top_p`` (1 or more: no limit) and
+    ``min_p`` (0 or less: no limit; float32 each). ``u``: a random number of [0, 1) per row, float32.
+
+    With w_i = exp((x_i - max x) / temperature), in the order of x (of equal ones the lower index first): the first top_k tokens
+    are kept; of these the shortest prefix whose weights reach top_p of theirs; of these those with w_i >= min_p; the first one in any
+    case. The token is the first one, by index, at which the running sum of the kept weights exceeds u times their total. A row gives the same token
+    whatever stands in the other rows. NaN counts as -inf; a row without any other logit gives token 0. With
+    ``want_logprobs``: (tokens, logprobs), float32 [rows], the logarithm of the token's probability among the kept ones (0 for
+    temperature 0, -inf for a row of -inf)."""
+    what = "sample_rows"
+    if logits.dim() != 2 or logits.dtype not in (torch.bfloat16, torch.float32) or not 0 < vocab <= logits.shape[1]:
+        raise ValueError(f"{what}: logits must be bfloat16 or float32 [rows, at least {vocab}], got {logits.dtype} {tuple(logits.shape)}")
+    rows = logits.shape[0]
+    if logits.stride(1) != 1:
+        logits = logits.contiguous()
+    u, temperature = _index(what, "u", u, torch.float32, (rows,)), _index(what, "temperature", temperature, torch.float32, (rows,))
+    top_k = _index(what, "top_k", top_k, torch.int32, (rows,)) if top_k is not None else None
+    top_p = _index(what, "top_p", top_p, torch.float32, (rows,)) if top_p is not None else None
+    min_p = _index(what, "min_p", min_p, torch.float32, (rows,)) if min_p is not None else None
+    _on_current_device(what, logits, u, temperature, top_k, top_p, min_p)
+    tokens = torch.empty(rows, dtype=torch.int64, device=logits.device)
+    logprobs = torch.empty(rows, dtype=torch.float32, device=logits.device) if want_logprobs else None
+    rc = _L().mlf_sample_rows(_p(logits), int(logits.dtype == torch.float32), C.c_longlong(rows), C.c_longlong(logits.stride(0)), int(vocab), _p(u),
+                              _p(temperature), _p(top_k), _p(top_p), _p(min_p), _p(tokens), _p(logprobs), _st())
+    _lib.check(rc, "mlf_sample_rows")
+    return (tokens, logprobs) if want_logprobs else tokens

@@ -144,6 +144,41 @@ def kv_write_ref(cache: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slots: t
         cache[b][:, off[at]] = q8_round_ref(new[at] / now[None, :, :, None], cache.dtype).transpose(0, 1)
 
 
+# ------------------------------------------------------------------ sampling
+def sample_ref(logits: torch.Tensor, vocab: int, u: torch.Tensor, temperature: torch.Tensor, top_k: Optional[torch.Tensor] = None,
+               top_p: Optional[torch.Tensor] = None, min_p: Optional[torch.Tensor] = None):
+    """(tokens, logprobs) of ``native.sample_rows`` in 64 bits, by its definition."""
+    x = logits[:, :vocab].double()
+    x = torch.where(torch.isnan(x), torch.full_like(x, float("-inf")), x)
+    rows, dev = x.shape[0], x.device
+    t = temperature.double()[:, None]
+    greedy = ~(t > 0)
+    top = x.amax(1, keepdim=True)
+    first = (x == top).to(torch.int8).argmax(1)                     # of equal ones the lowest index
+    w = torch.where(x == top, 1.0, torch.exp((x - top) / torch.where(greedy, 1.0, t)))
+    w = torch.where(torch.isinf(x) & (x < 0), 0.0, w)
+    _, order = torch.sort(x, dim=1, descending=True, stable=True)
+    ws = w.gather(1, order)
+    rank = torch.arange(vocab, device=dev)[None, :]
+    k = torch.full((rows, 1), vocab, device=dev) if top_k is None else torch.where(top_k <= 0, vocab, top_k.long())[:, None]
+    ws = torch.where(rank < k, ws, 0.0)
+    keep = ws > 0
+    if top_p is not None:
+        p = top_p.double()[:, None]
+        keep &= (p >= 1) | (torch.cumsum(ws, 1) - ws < p * ws.sum(1, keepdim=True)) | (rank == 0)
+    if min_p is not None:
+        keep &= (ws >= min_p.double()[:, None]) | (rank == 0)
+    kept = torch.zeros_like(x).scatter_(1, order, torch.where(keep, ws, 0.0))
+    run = torch.cumsum(kept, 1)
+    last = torch.where(kept > 0, rank, 0).amax(1)
+    token = torch.minimum((run <= u.double()[:, None] * run[:, -1:]).sum(1), last)
+    logprob = torch.log(kept.gather(1, token[:, None])[:, 0] / run[:, -1])
+    none = torch.isinf(top[:, 0]) & (top[:, 0] < 0)
+    token = torch.where(greedy[:, 0], first, token)
+    logprob = torch.where(greedy[:, 0], torch.zeros_like(logprob), logprob)
+    return torch.where(none, torch.zeros_like(token), token), torch.where(none, torch.full_like(logprob, float("-inf")), logprob).float()
+
+
 def adamw_ref(p, m, v, g, *, lr, beta1, beta2, eps, weight_decay, step, vmax=None):
     """One AdamW step in fp32, decay first then the Adam update
     (src/MLFramework/Optimizers/Adam.cs:167-213). Returns new (p, m, v[, vmax])."""
