@@ -16,6 +16,7 @@
 
 #include <deque>
 #include <mutex>
+#include <new>
 #include <unordered_map>
 #include <vector>
 
@@ -257,6 +258,40 @@ MLF_API int mlf_bm_fork(void* h, long long src, long long dst, int prefix_tokens
   }
   m->seqs[dst] = d;
   return nb;
+}
+
+// Moves the blocks in use to the lowest numbers: pairs (up to total_blocks of them) receives the (source, destination) copies that
+// the caller must perform on the device, sources above every destination; tables and reference counts name the new places
+// afterwards and the free blocks are those behind them, in order. Returns the number of copies.
+MLF_API int mlf_bm_compact(void* h, int* pairs) {
+  auto* m = static_cast<BlockManager*>(h);
+  std::lock_guard<std::mutex> lk(m->mu);
+  try {
+    const int live = m->total_blocks - (int)m->free_list.size();
+    std::vector<int> to(m->total_blocks, -1);
+    std::deque<int> free_list;
+    for (int b = live; b < m->total_blocks; ++b) free_list.push_back(b);
+    int n = 0, hole = 0;
+    for (int b = live; b < m->total_blocks; ++b) {
+      if (m->refcount[b] <= 0) continue;
+      while (m->refcount[hole] > 0) ++hole;
+      pairs[2 * n] = b;
+      pairs[2 * n + 1] = to[b] = hole++;
+      ++n;
+    }
+    for (int i = 0; i < n; ++i) {
+      m->refcount[pairs[2 * i + 1]] = m->refcount[pairs[2 * i]];
+      m->refcount[pairs[2 * i]] = 0;
+    }
+    for (auto& kv : m->seqs)
+      for (int& b : kv.second.blocks)
+        if (to[b] >= 0) b = to[b];
+    m->free_list.swap(free_list);
+    return n;
+  } catch (const std::bad_alloc&) {
+    set_error("block manager: out of host memory while compacting");
+    return -1;
+  }
 }
 
 MLF_API int mlf_bm_ref_count(void* h, int block) {

@@ -16,6 +16,7 @@ import argparse
 import json
 import random
 import time
+from typing import Optional
 
 import torch
 
@@ -32,16 +33,17 @@ def _max_len(spec) -> int:
 
 def run(model_name: str = "llama-tiny", n_requests: int = 32, rate: float = 0.0, prompt_len=64, max_tokens=16,
         max_batch: int = 32, block_size: int = 16, device: str = "cpu", seed: int = 0, kv_fraction: float = 0.5, pg=None, fused: bool = True,
-        torch_ops: bool = False):
+        torch_ops: bool = False, kv_dtype: Optional[str] = None, temperature: float = 0.0):
     """``torch_ops``: the comparison arm -- the same scheduler, block manager and request stream, with every operator of
     the model step taken from torch (cuBLAS linears, ``F.rms_norm``, SDPA over pages gathered by indexing the block
-    table, NCCL reductions), launched eagerly."""
+    table, NCCL reductions), launched eagerly. ``kv_dtype``: ``e4m3`` or ``int8`` for a cache in 8 bits. ``temperature``: above 0
+    tokens are drawn, each request from a seed of its own."""
     fused = fused and not torch_ops
     from ..modelzoo.zoo import build_model, default_registry
     from .executor import ExecutorConfig, PagedLlamaExecutor
     from .kv_cache import KVCacheBlockManager
     from .scheduler import (BatchConstraints, CapacityConstraints, CompletionConfiguration, ContinuousBatchScheduler, Request,
-                            SchedulerConfiguration)
+                            SamplingParameters, SchedulerConfiguration)
     info = default_registry().get(model_name)
     dev = torch.device(device)
     dtype = torch.bfloat16 if dev.type == "cuda" else torch.float32
@@ -64,7 +66,8 @@ def run(model_name: str = "llama-tiny", n_requests: int = 32, rate: float = 0.0,
     mc = model.cfg
     p_max, t_max = _max_len(prompt_len), _max_len(max_tokens)
     kv_heads = mc.n_kv_heads // W
-    per_block = 2 * block_size * kv_heads * mc.head_dim * mc.n_layers * (2 if dtype == torch.bfloat16 else 4)
+    kv_type = {None: dtype, "e4m3": torch.float8_e4m3fn, "int8": torch.int8}[kv_dtype]
+    per_block = 2 * block_size * kv_heads * mc.head_dim * mc.n_layers * kv_type.itemsize
     need = (p_max + t_max + block_size) // block_size * max(max_batch, 1) + 8
     if dev.type == "cuda":
         free, _ = torch.cuda.mem_get_info(dev)
@@ -74,7 +77,7 @@ def run(model_name: str = "llama-tiny", n_requests: int = 32, rate: float = 0.0,
         from ..dist.process_group import ReduceOp
         pg.all_reduce(t, ReduceOp.MIN)
         need = int(t.item())
-    kv = KVCacheBlockManager(need, block_size, mc.head_dim, mc.n_layers, kv_heads, device=dev, dtype=dtype)
+    kv = KVCacheBlockManager(need, block_size, mc.head_dim, mc.n_layers, kv_heads, device=dev, dtype=kv_type)
     ex = PagedLlamaExecutor(model, kv, ExecutorConfig(max_batch=max_batch, max_seq_len=p_max + t_max + block_size,
                                                       prefill_chunk=max(p_max, 16), torch_ops=torch_ops), tp=tp)
     leader = None
@@ -91,7 +94,8 @@ def run(model_name: str = "llama-tiny", n_requests: int = 32, rate: float = 0.0,
     if leader is not None:
         leader.live_ids_fn = lambda: [q.id for q in sched.batch_manager.running]
     rng = random.Random(seed)
-    reqs = [Request([rng.randrange(1, mc.vocab_size) for _ in range(_rng_len(prompt_len, rng))], max_tokens=_rng_len(max_tokens, rng))
+    reqs = [Request([rng.randrange(1, mc.vocab_size) for _ in range(_rng_len(prompt_len, rng))], max_tokens=_rng_len(max_tokens, rng),
+                    sampling=SamplingParameters(temperature, top_p=0.95, seed=rng.getrandbits(64)) if temperature > 0 else None)
             for _ in range(n_requests)]
     n_prompt_tokens = sum(len(q.prompt_tokens) for q in reqs)
     # warm-up: one short request end to end (loads kernels, fills caches of tensor maps)
@@ -121,7 +125,7 @@ def run(model_name: str = "llama-tiny", n_requests: int = 32, rate: float = 0.0,
     snap = sched.metrics.snapshot()
     return {"impl": "torch" if torch_ops else "ours", "model": model_name, "tensor_parallel": W, "fused_reduce": bool(tp is not None and tp.fused), "requests": n_requests, "arrival_rate": rate,
             "prompt_len": prompt_len, "max_tokens": max_tokens,
-            "max_batch": max_batch, "wall_s": wall, "generated_tokens": gen, "decode_tokens_per_s": gen / wall,
+            "kv_dtype": str(kv_type).replace("torch.", ""), "temperature": temperature, "max_batch": max_batch, "wall_s": wall, "generated_tokens": gen, "decode_tokens_per_s": gen / wall,
             "total_tokens_per_s": (gen + n_prompt_tokens) / wall, "ttft_p50_ms": pct(ttft, 0.5) * 1e3, "ttft_p99_ms": pct(ttft, 0.99) * 1e3,
             "latency_p50_ms": pct(lat, 0.5) * 1e3, "latency_p99_ms": pct(lat, 0.99) * 1e3, "iterations": sched.iterations,
             "kv_blocks": need, "scheduler": {k: v for k, v in snap.items() if isinstance(v, (int, float))}}
@@ -139,6 +143,8 @@ def main(argv=None):
     ap.add_argument("--no-fused", action="store_true", help="tensor parallel: reduce partial sums with NCCL instead of the peer-memory kernel")
     ap.add_argument("--max-batch", type=int, default=32)
     ap.add_argument("--device", default="cuda" if torch.cuda.is_available() else "cpu")
+    ap.add_argument("--kv-dtype", choices=["e4m3", "int8"], help="hold the KV cache in 8 bits")
+    ap.add_argument("--temperature", type=float, default=0.0, help="above 0: draw tokens (top-p 0.95)")
     a = ap.parse_args(argv)
     spec = lambda v: tuple(int(x) for x in v.split(":")) if ":" in str(v) else int(v)
     pg = None
@@ -149,7 +155,7 @@ def main(argv=None):
         pg = init_process_group("nccl")
         a.device = f"cuda:{torch.cuda.current_device()}"
     out = run(a.model, a.requests, a.rate, spec(a.prompt_len), spec(a.max_tokens), a.max_batch, device=a.device, pg=pg, fused=not a.no_fused,
-              torch_ops=a.impl == "torch")
+              torch_ops=a.impl == "torch", kv_dtype=a.kv_dtype, temperature=a.temperature)
     if pg is None or pg.rank == 0:
         print(json.dumps(out))
     if pg is not None:

@@ -1,6 +1,8 @@
 """Model executor for the continuous-batching scheduler: a Llama-style decoder running on the paged
 KV cache with the native kernels (GEMM with fused SwiGLU / residual epilogues, RMSNorm, RoPE,
-KV-cache write, FlashAttention-style prefill, paged decode, greedy sampling).
+KV-cache write, FlashAttention-style prefill, paged decode, greedy or drawn tokens). A block manager with an 8-bit cache is
+read and written through its scales; the first chunk of a prompt attends to its own rows as they were projected, later chunks and
+decode steps to what the cache holds.
 
 ``execute_batch`` is the ``IModelExecutor.ExecuteBatchAsync`` of the reference
 (src/MLFramework/Inference/ContinuousBatching/IModelExecutor.cs:8-16). Its attention path is what
@@ -51,6 +53,8 @@ class PagedLlamaExecutor:
         p = next(model.parameters())
         self.device, self.dtype = p.device, p.dtype
         self.native = p.is_cuda and p.dtype == torch.bfloat16 and self.mc.head_dim == 128 and not self.cfg.torch_ops
+        if self.cfg.torch_ops and kv.scales[0] is not None:
+            raise ValueError("the torch arm has no path for a cache in 8 bits")
         W = tp.world if tp is not None else 1
         self.hq, self.hkv = self.mc.n_heads // W, self.mc.n_kv_heads // W
         self.max_blocks = (self.cfg.max_seq_len + kv.block_size - 1) // kv.block_size
@@ -126,7 +130,7 @@ class PagedLlamaExecutor:
         o_w = attn.proj.weight if attn is not None else blk.o.weight
         gu_w = blk.mlp.gate_up.weight if hasattr(blk, "mlp") else blk.gate_up.weight
         dn_w = blk.mlp.down.weight if hasattr(blk, "mlp") else blk.down.weight
-        cache = self.kv.caches[li]
+        cache, kv_scale = self.kv.caches[li], self.kv.scales[li]
         T = x.shape[0]
         if self.native:
             # A decode step (few rows, whole weights) streams weights: plain products let the GEMM split K over all SMs
@@ -139,7 +143,7 @@ class PagedLlamaExecutor:
                 q = qkv[:, :self.hq * D].view(T, self.hq, D)
                 k = qkv[:, self.hq * D:(self.hq + self.hkv) * D].view(T, self.hkv, D)
                 v = qkv[:, (self.hq + self.hkv) * D:].view(T, self.hkv, D)
-                native.rope_kv_write_(qkv, positions, slots, cache, self.hq, self.hkv, mc.rope_theta)
+                native.rope_kv_write_(qkv, positions, slots, cache, self.hq, self.hkv, mc.rope_theta, kv_scale=kv_scale)
                 a = attend(li, q, k, v)
             multi = self.tp is not None and self.tp.world > 1
             # few rows: the residual stream takes the product as an accumulation; up to 128 rows (K is split over the SMs
@@ -175,11 +179,7 @@ class PagedLlamaExecutor:
         v = qkv[:, (self.hq + self.hkv) * D:].reshape(T, self.hkv, D)
         q = reference.rope_ref(q, positions, mc.rope_theta).to(x.dtype)
         k = reference.rope_ref(k, positions, mc.rope_theta).to(x.dtype)
-        flat = cache.view(-1, 2, self.kv.block_size, self.hkv, D)
-        ok = slots >= 0
-        blk_i, off = slots[ok] // self.kv.block_size, slots[ok] % self.kv.block_size
-        flat[blk_i, 0, off] = k[ok]
-        flat[blk_i, 1, off] = v[ok]
+        reference.kv_write_ref(cache.view(-1, 2, self.kv.block_size, self.hkv, D), k, v, slots, kv_scale)
         a = attend(li, q, k, v)
         x = self._reduce(F.linear(a.reshape(T, self.hq * D).to(x.dtype), o_w), x)
         h, _ = reference.rms_norm_ref(x, blk.norm2.weight, mc.norm_eps)
@@ -259,10 +259,39 @@ class PagedLlamaExecutor:
             return out.view(*ids.shape, d)
         return self.m.embed(ids)
 
-    def _logits_argmax(self, x_last: torch.Tensor) -> torch.Tensor:
+    # ---- drawn tokens: what each row is drawn with, packed as int32 [5, rows] (u, temperature, top_p and min_p by their bits, top_k)
+    def _draws(self, reqs: Sequence[Request], rows: int) -> Optional[torch.Tensor]:
+        """None where every request takes its likeliest token; padding rows do."""
+        each = [r.next_draw() for r in reqs]
+        if not any(d is not None for d in each):
+            return None
+        cols = [d or (0.0, 0.0, 0, 1.0, 0.0) for d in each] + [(0.0, 0.0, 0, 1.0, 0.0)] * (rows - len(each))
+        u, t, k, p, m = zip(*cols)
+        host = torch.empty(5, rows, dtype=torch.int32, pin_memory=self.device.type == "cuda")
+        for i, v in enumerate((u, t, p, m)):
+            host[i].view(torch.float32).copy_(torch.frombuffer(array("f", v), dtype=torch.float32))
+        host[4].copy_(torch.frombuffer(array("i", k), dtype=torch.int32))
+        return host
+
+    def _draws_on_device(self, reqs: Sequence[Request]) -> Optional[torch.Tensor]:
+        host = self._draws(reqs, len(reqs))
+        return host.to(self.device, non_blocking=True) if host is not None else None
+
+    def _logits_draw(self, logits: torch.Tensor, draws: torch.Tensor) -> torch.Tensor:
+        u, t, p, m = draws[:4].view(torch.float32)
+        if self.tp is not None and self.tp.world > 1:
+            logits = self.tp.pg.all_gather(logits.contiguous(), dim=-1)        # the same logits and numbers on every rank: the same tokens
+        if self.native:
+            return native.sample_rows(logits, self.mc.vocab_size, u, t, draws[4], p, m)
+        return reference.sample_ref(logits, self.mc.vocab_size, u, t, draws[4], p, m)[0]
+
+    def _logits_argmax(self, x_last: torch.Tensor, draws: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """The next tokens: the likeliest ones, or with ``draws`` what :func:`native.sample_rows` makes of them."""
         mc = self.mc
         if self.native:
             _, logits = self._norm_product(x_last.contiguous(), self.m.norm_f.weight, self.m.lm_head, x_last.shape[0] <= 256)
+            if draws is not None:
+                return self._logits_draw(logits, draws)
             if self.tp is not None and self.tp.world > 1 and self.tp.fused:
                 cand = self.tp.symm_buffer("serve.argmax", max(self.cfg.max_batch, 1) * 8)
                 return self.tp.symm.tp_argmax(logits, self.tp.rank * logits.shape[1], mc.vocab_size, cand)
@@ -272,6 +301,8 @@ class PagedLlamaExecutor:
             return native.argmax_rows(logits, mc.vocab_size)
         h, _ = reference.rms_norm_ref(x_last, self.m.norm_f.weight, mc.norm_eps)
         logits = F.linear(h.to(x_last.dtype), self.m.lm_head)
+        if draws is not None:
+            return self._logits_draw(logits, draws)
         if self.tp is not None and self.tp.world > 1:
             logits = self.tp.pg.all_gather(logits, dim=-1)
         return logits[:, :mc.vocab_size].float().argmax(-1)
@@ -292,7 +323,7 @@ class PagedLlamaExecutor:
         start = r.prefilled
         chunk = r.prompt_tokens[start:start + self.cfg.prefill_chunk]
         n = len(chunk)
-        name = self._prefill_key(1, n) if start == 0 and n == len(r.prompt_tokens) else None
+        name = self._prefill_key(1, n, [r]) if start == 0 and n == len(r.prompt_tokens) else None
         if name is not None:
             return self._prefill_graph(name, [r], n)[r.id]
         slots, _ = self.kv.append_tokens(r.id, n)
@@ -308,7 +339,7 @@ class PagedLlamaExecutor:
         table = self.kv.build_tables([r.id], self.max_blocks, dev)[0] if start > 0 or not self.native else None
         total = start + n
 
-        paged_prefill = self.native and start > 0 and self.kv.block_size == 16
+        paged_prefill = self.native and start > 0 and self.kv.block_size == 16 and self.kv.scales[0] is None
 
         def attend(li, q, k, v):
             if paged_prefill:
@@ -318,10 +349,12 @@ class PagedLlamaExecutor:
             if start == 0:
                 kk, vv = k, v
             elif self.native:
-                kk, vv = native.kv_gather(self.kv.caches[li], table[0], total)
+                kk, vv = native.kv_gather(self.kv.caches[li], table[0], total, kv_scale=self.kv.scales[li])
             else:
-                nb = (total + self.kv.block_size - 1) // self.kv.block_size
-                c = self.kv.caches[li][table[0, :nb].long()]
+                pages = table[0, :(total + self.kv.block_size - 1) // self.kv.block_size].long()
+                c = self.kv.caches[li][pages]
+                if self.kv.scales[li] is not None:
+                    c = reference.kv_values_ref(c, self.kv.scales[li][pages])
                 kk = c[:, 0].reshape(-1, self.hkv, self.mc.head_dim)[:total]
                 vv = c[:, 1].reshape(-1, self.hkv, self.mc.head_dim)[:total]
             if self.native and start == 0:
@@ -338,7 +371,7 @@ class PagedLlamaExecutor:
             x = self._block(li, blk, x, pos, slots, attend)
         r.prefilled = total
         if r.prefilled >= len(r.prompt_tokens):
-            return int(self._logits_argmax(x[-1:])[0])
+            return int(self._logits_argmax(x[-1:], self._draws_on_device([r]))[0])
         return None
 
     # ---- short prompts through a captured graph
@@ -347,7 +380,7 @@ class PagedLlamaExecutor:
         """Rows that a prompt of ``n`` tokens is padded to: the row counts of the few-row product's tiles, then steps of 64."""
         return 32 if n <= 32 else 64 if n <= 64 else (n + 127) // 128 * 128 if n <= 128 else (n + 63) // 64 * 64
 
-    def _prefill_key(self, B: int, n: int) -> Optional[str]:
+    def _prefill_key(self, B: int, n: int, reqs: Sequence[Request]) -> Optional[str]:
         """Name of the graph that prefills ``B`` whole prompts of ``n`` tokens, or None where prompts run launch by launch:
         above 512 rows the GPU is busy for longer than the host takes to launch, and beyond 32 graphs further shapes are not
         worth the memory of another one. A bucket's first ``graph_warmup_steps`` passes run launch by launch; the pass after them
@@ -359,7 +392,7 @@ class PagedLlamaExecutor:
         Tp = self._prompt_bucket(n)
         if B * Tp > 512:
             return None
-        name = f"prefill_B{B}_T{Tp}"
+        name = f"prefill_B{B}_T{Tp}" + ("_drawn" if any(r.next_draw() is not None for r in reqs) else "")
         if name not in self._prompts_seen:
             if len(self._prompts_seen) >= 32:
                 return None
@@ -374,7 +407,11 @@ class PagedLlamaExecutor:
         padded row count may take another product kernel or split of K than the prompt's own: sums in another order."""
         B, Tp = len(reqs), self._prompt_bucket(n)
         T = B * Tp
-        host = self._host_rows(1, 3 * T + B)[0]
+        draws = self._draws(reqs, B)
+        end = 3 * T + B
+        host = self._host_rows(1, end + ((5 * B + 1) // 2 if draws is not None else 0))[0]
+        if draws is not None:
+            host[end:].view(torch.int32)[:5 * B].copy_(draws.view(-1))
         ids, pos, slots = host[:3 * T].view(3, B, Tp)
         host[:3 * T] = 0
         pos.copy_(torch.arange(Tp))
@@ -385,7 +422,7 @@ class PagedLlamaExecutor:
                 raise MemoryError(f"KV cache exhausted while prefilling request {r.id}")
             self._put_ids(ids[i, :n], r.prompt_tokens)
             slots[i, :n].copy_(s)
-        torch.arange(n - 1, T, Tp, out=host[3 * T:])
+        torch.arange(n - 1, T, Tp, out=host[3 * T:end])
 
         def step(buf):
             def attend(li, q, k, v):
@@ -393,7 +430,7 @@ class PagedLlamaExecutor:
             x = self._embed(buf[:T].view(B, Tp)).reshape(T, -1)
             for li, blk in enumerate(self.m.blocks):
                 x = self._block(li, blk, x, buf[T:2 * T], buf[2 * T:3 * T], attend)
-            return self._logits_argmax(x[buf[3 * T:]])
+            return self._logits_argmax(x[buf[3 * T:end]], buf[end:].view(torch.int32)[:5 * B].view(5, B) if draws is not None else None)
         toks = self._prompt_graphs.run_from_host(name, step, host, self.device).tolist()
         for r in reqs:
             r.prefilled = n
@@ -404,7 +441,7 @@ class PagedLlamaExecutor:
     def _prefill_many(self, reqs: List[Request], n: int) -> Dict[int, int]:
         dev = self.device
         B = len(reqs)
-        name = self._prefill_key(B, n) if all(len(r.prompt_tokens) == n for r in reqs) else None
+        name = self._prefill_key(B, n, reqs) if all(len(r.prompt_tokens) == n for r in reqs) else None
         if name is not None:
             return self._prefill_graph(name, reqs, n)
         slot_list = []
@@ -435,24 +472,27 @@ class PagedLlamaExecutor:
         if not done:
             return {}
         rows = torch.tensor([i * n + n - 1 for i in done], dtype=torch.int64, device=dev)
-        toks = self._logits_argmax(x[rows]).tolist()
+        toks = self._logits_argmax(x[rows], self._draws_on_device([reqs[i] for i in done])).tolist()
         return {reqs[i].id: int(t) for i, t in zip(done, toks)}
 
     # ---- one decode step for a set of requests
-    def _decode_core(self, last, pos, slots, table, lens, max_len: int) -> torch.Tensor:
-        """Device-only part of a decode step (no host reads): embed, all blocks, head, arg-max."""
+    def _decode_core(self, last, pos, slots, table, lens, max_len: int, draws: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Device-only part of a decode step (no host reads): embed, all blocks, head, arg-max or draw."""
         def attend(li, q, k, v):
             if self.cfg.torch_ops:
                 return self._attend_torch_decode(li, q, table, lens, max_len)
-            return reference.paged_attention_ref(q, self.kv.caches[li], table.cpu(), lens.cpu().tolist()).to(q.dtype)
+            cache, kv_scale = self.kv.caches[li], self.kv.scales[li]
+            if kv_scale is not None:
+                cache = reference.kv_values_ref(cache, kv_scale)
+            return reference.paged_attention_ref(q, cache, table.cpu(), lens.cpu().tolist()).to(q.dtype)
 
         def attend_packed(li, qkv):
             return native.paged_decode_rope(qkv, self.kv.caches[li], table, lens, slots, self.hq, self.hkv, max_len, self.mc.rope_theta,
-                                            split_tokens=self.cfg.decode_split_tokens, inputs_static=True)
+                                            split_tokens=self.cfg.decode_split_tokens, inputs_static=True, kv_scale=self.kv.scales[li])
         x = self._embed(last[None])[0]
         for li, blk in enumerate(self.m.blocks):
             x = self._block(li, blk, x, pos, slots, attend, attend_packed if self.native else None)
-        return self._logits_argmax(x)
+        return self._logits_argmax(x, draws)
 
     @staticmethod
     def _bucket(n: int, lo: int = 1) -> int:
@@ -470,9 +510,12 @@ class PagedLlamaExecutor:
         # handful of captured graphs covers every step. Padding rows write nowhere (slot -1) and attend to
         # one token of block 0; their outputs are dropped.
         Bp = self._bucket(B) if self._graphs is not None else B
-        # one buffer, one copy: token ids, positions, slots (int64 [3, Bp]), then lengths and block tables (int32)
-        head = 3 * Bp
-        host = torch.empty(head + (Bp * (1 + self.max_blocks) + 1) // 2, dtype=torch.int64, pin_memory=dev.type == "cuda")
+        draws = self._draws(reqs, Bp)
+        # drawn tokens of a sharded vocabulary are gathered by the process group, which is not captured
+        graphs = self._graphs if draws is None or self.tp is None or self.tp.world == 1 else None
+        # one buffer, one copy: token ids, positions, slots (int64 [3, Bp]), then lengths, block tables and draws (int32)
+        head, end = 3 * Bp, Bp * (1 + self.max_blocks)
+        host = torch.empty(head + (end + (5 * Bp if draws is not None else 0) + 1) // 2, dtype=torch.int64, pin_memory=dev.type == "cuda")
         host32 = host[head:].view(torch.int32)
         self._put_ids(host[:B], last_l)
         host[B:Bp] = 0
@@ -483,15 +526,18 @@ class PagedLlamaExecutor:
         if done < B:
             raise MemoryError(f"KV cache exhausted while decoding request {ids[done]}")
         max_len = top + 1
+        if draws is not None:
+            host32[end:end + 5 * Bp].copy_(draws.view(-1))
 
         def step(buf, length):
             b32 = buf[head:].view(torch.int32)
-            return self._decode_core(buf[:Bp], buf[Bp:2 * Bp], buf[2 * Bp:head], b32[Bp:Bp * (1 + width)].view(Bp, width), b32[:Bp], length)
+            return self._decode_core(buf[:Bp], buf[Bp:2 * Bp], buf[2 * Bp:head], b32[Bp:Bp * (1 + width)].view(Bp, width), b32[:Bp], length,
+                                     b32[end:end + 5 * Bp].view(5, Bp) if draws is not None else None)
 
-        if self._graphs is None:
+        if graphs is None:
             return step(host.to(dev, non_blocking=True), max_len).tolist()
         Lp = min(self._bucket(max_len, 512), max(self.cfg.max_seq_len, 512))
-        out = self._graphs.run_from_host(f"decode_B{Bp}_L{Lp}", lambda buf: step(buf, Lp), host, dev)
+        out = graphs.run_from_host(f"decode_B{Bp}_L{Lp}" + ("_drawn" if draws is not None else ""), lambda buf: step(buf, Lp), host, dev)
         return (out if B == Bp else out[:B]).tolist()
 
     # ---- scheduler entry point

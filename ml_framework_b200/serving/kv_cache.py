@@ -1,7 +1,8 @@
 """KV-cache block manager, block tables and block sharing for paged attention.
 
 ``KVCacheBlockManager`` wraps the native pool (``csrc/serving/block_manager.cpp``) and owns the
-device cache tensor ``[num_blocks, 2, block_size, Hkv, head_dim]`` per layer. API and behaviour
+device cache tensor ``[num_blocks, 2, block_size, Hkv, head_dim]`` per layer; with an 8-bit ``dtype`` (float8_e4m3fn or
+int8) it also owns the scales ``[num_blocks, 2, Hkv]`` that ``native.paged_decode`` describes. API and behaviour
 follow src/MLFramework/Inference/PagedAttention/KVCacheBlockManager.cs:39-247 (allocate one /
 many (all-or-nothing) / free block / free sequence / stats / has_available_blocks),
 BlockTable.cs:38-192 (per-sequence ordered blocks, token -> block, sequence length) and the
@@ -18,6 +19,7 @@ from typing import Dict, List, Optional, Sequence, Tuple
 import torch
 
 from .. import _lib
+from ..ops import native
 
 
 @dataclass
@@ -57,7 +59,10 @@ class KVCacheBlockManager:
         self.head_dim, self.num_layers, self.num_kv_heads = head_dim, num_layers, num_kv_heads
         self.device = torch.device(device) if device is not None else torch.device("cpu")
         self.caches: List[torch.Tensor] = []
+        self.scales: List[Optional[torch.Tensor]] = [None] * num_layers      # of each layer; None: a cache without scales
         if allocate_cache:
+            if dtype in (torch.float8_e4m3fn, torch.int8):
+                self.scales = [torch.zeros(total_blocks, 2, num_kv_heads, device=self.device) for _ in range(num_layers)]
             self.caches = [torch.zeros(total_blocks, 2, block_size, num_kv_heads, head_dim, dtype=dtype, device=self.device)
                            for _ in range(num_layers)]
 
@@ -91,12 +96,32 @@ class KVCacheBlockManager:
             return None, None
         cow = (cs.value, cd.value) if cs.value >= 0 else None
         if cow is not None:
-            self._copy_block(*cow)
+            self._copy_blocks([cow])
         return slots[:n], cow
 
-    def _copy_block(self, src: int, dst: int):
-        for cache in self.caches:
-            cache[dst].copy_(cache[src])
+    def _copy_blocks(self, pairs: Sequence[Tuple[int, int]]):
+        """Block dst of every layer (and its scales) becomes what block src is; no block is both read and written."""
+        tensors = self.caches + [s for s in self.scales if s is not None]
+        if not tensors or not pairs:
+            return
+        if self.device.type == "cuda":
+            with torch.cuda.device(self.device):
+                native.kv_copy_blocks_(tensors, pairs)
+            return
+        src, dst = [a for a, _ in pairs], [b for _, b in pairs]
+        for t in tensors:
+            raw = t.view(torch.uint8) if t.element_size() == 1 else t
+            raw[dst] = raw[src]
+
+    def compact(self) -> int:
+        """Moves the blocks in use to the lowest numbers, contents and all, so that the free ones lie behind them in one run.
+        Sequences keep their tokens and their sharing; block tables built before are void. Returns the number of blocks moved."""
+        pairs = array("i", bytes(8 * self.total_blocks))
+        n = self._L.mlf_bm_compact(self._h, C.c_void_p(pairs.buffer_info()[0]))
+        if n < 0:
+            _lib.check(n, "mlf_bm_compact")
+        self._copy_blocks([(pairs[2 * i], pairs[2 * i + 1]) for i in range(n)])
+        return n
 
     def append_decode(self, seq_ids: Sequence[int], max_blocks: int, rows: int, width: int, pos: torch.Tensor, slots: torch.Tensor,
                       lens: torch.Tensor, table: torch.Tensor) -> Tuple[int, int]:
@@ -113,9 +138,7 @@ class KVCacheBlockManager:
         rc = self._L.mlf_bm_append_decode(self._h, p(ids.buffer_info()[0]), n, rows, max_blocks, width, p(pos.data_ptr()),
                                           p(slots.data_ptr()), p(lens.data_ptr()), p(table.data_ptr()), cow, C.byref(done), C.byref(top))
         if self.caches:
-            for i in range(done.value):
-                if cow[2 * i] >= 0:
-                    self._copy_block(cow[2 * i], cow[2 * i + 1])
+            self._copy_blocks([(cow[2 * i], cow[2 * i + 1]) for i in range(done.value) if cow[2 * i] >= 0])
         if rc != -1:
             _lib.check(rc, "mlf_bm_append_decode")
         return done.value, top.value

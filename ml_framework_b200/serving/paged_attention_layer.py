@@ -6,7 +6,8 @@ argument: prefill computes attention over the prompt and stores K / V page by pa
 attends to every cached token through the block table), Phases/PrefillOrchestrator.cs:31-78,
 Phases/DecodeOrchestrator.cs, Kernels/IPagedAttentionKernel.cs. On bf16 CUDA tensors with head dimension 128 the
 hand-written kernels run (``rope_kv_write``, the tcgen05 prefill kernel, the paged decode kernel); anything else
-evaluates the same mathematics in PyTorch (``ops/reference.py``).
+evaluates the same mathematics in PyTorch (``ops/reference.py``). A block manager with an 8-bit cache is read and written
+through its scales; later chunks of a prompt then attend to the gathered values.
 """
 from __future__ import annotations
 
@@ -57,7 +58,7 @@ class PagedAttentionLayer(nn.Module):
 
     def forward(self, x: torch.Tensor, kv: KVCacheBlockManager, seq_ids: Sequence[int], phase: AttentionPhase,
                 n_tokens: Optional[Sequence[int]] = None) -> torch.Tensor:
-        cache = kv.caches[self.layer_index]
+        cache, scale = kv.caches[self.layer_index], kv.scales[self.layer_index]
         dev, D = x.device, self.head_dim
         if phase == AttentionPhase.DECODE:
             n_tokens = [1] * len(seq_ids)
@@ -82,25 +83,23 @@ class PagedAttentionLayer(nn.Module):
             qkv = gemm(x, self.qkv.weight, bias=self.qkv.bias)
             q, k, v = self._split(qkv)
             if self.rope_theta is not None:
-                native.rope_kv_write_(qkv, positions, slots, cache, self.n_heads, self.n_kv_heads, self.rope_theta)
+                native.rope_kv_write_(qkv, positions, slots, cache, self.n_heads, self.n_kv_heads, self.rope_theta, kv_scale=scale)
             else:
-                native.kv_cache_write(cache, k, v, slots)
+                native.kv_cache_write(cache, k, v, slots, kv_scale=scale)
         else:
             qkv = F.linear(x, self.qkv.weight, self.qkv.bias)
             q, k, v = self._split(qkv)
             if self.rope_theta is not None:
                 q = reference.rope_ref(q, positions, self.rope_theta).to(x.dtype)
                 k = reference.rope_ref(k, positions, self.rope_theta).to(x.dtype)
-            flat = cache.view(-1, 2, kv.block_size, self.n_kv_heads, D)
-            flat[slots // kv.block_size, 0, slots % kv.block_size] = k.to(cache.dtype)
-            flat[slots // kv.block_size, 1, slots % kv.block_size] = v.to(cache.dtype)
+            reference.kv_write_ref(cache.view(-1, 2, kv.block_size, self.n_kv_heads, D), k, v, slots, scale)
         max_blocks = max(kv.blocks_needed(st + n) for st, n in zip(starts, n_tokens))
         table, lens = kv.build_tables(list(seq_ids), max_blocks, dev)
         if phase == AttentionPhase.DECODE:
             if nat:
-                a = native.paged_decode(q, cache, table, lens, int(max(st + 1 for st in starts)))
+                a = native.paged_decode(q, cache, table, lens, int(max(st + 1 for st in starts)), kv_scale=scale)
             else:
-                a = reference.paged_attention_ref(q.float(), cache.float(), table, lens).to(x.dtype)
+                a = reference.paged_attention_ref(q.float(), reference.kv_values_ref(cache, scale), table, lens).to(x.dtype)
         else:
             outs, off = [], 0
             for i, (n, st) in enumerate(zip(n_tokens, starts)):
@@ -108,14 +107,15 @@ class PagedAttentionLayer(nn.Module):
                 total = st + n
                 if nat and st == 0:
                     o, _ = native.flash_fwd(qi, k[off:off + n], v[off:off + n], 1, n, causal=True, want_lse=False)
-                elif nat and kv.block_size == 16:
+                elif nat and kv.block_size == 16 and scale is None:
                     o = native.flash_fwd_paged(qi, cache, table[i:i + 1], 1, n, total, causal=True)    # pages read in the kernel
                 elif nat:
-                    kk, vv = native.kv_gather(cache, table[i], total)
+                    kk, vv = native.kv_gather(cache, table[i], total, kv_scale=scale)
                     o = native.flash_fwd_prefix(qi, kk, vv, 1, n, total, causal=True)
                 else:
                     nb = kv.blocks_needed(total)
-                    c = cache[table[i, :nb].long()]
+                    pages = table[i, :nb].long()
+                    c = reference.kv_values_ref(cache[pages], scale[pages] if scale is not None else None)
                     kk = c[:, 0].reshape(-1, self.n_kv_heads, D)[:total]
                     vv = c[:, 1].reshape(-1, self.n_kv_heads, D)[:total]
                     o, _ = reference.attention_ref(qi[None].float(), kk[None].float(), vv[None].float(), causal=True, start_pos=st)

@@ -21,11 +21,12 @@ import collections
 import enum
 import heapq
 import itertools
+import random
 import threading
 import time
 from concurrent.futures import Future
 from dataclasses import dataclass, field
-from typing import Callable, Deque, Dict, List, Optional, Sequence
+from typing import Callable, Deque, Dict, List, Optional, Sequence, Tuple
 
 from .kv_cache import KVCacheBlockManager
 
@@ -59,6 +60,36 @@ _ids = itertools.count(1)
 
 
 @dataclass
+class SamplingParameters:
+    """How a request's tokens are drawn (``native.sample_rows`` has the definition). ``temperature`` 0: the likeliest token.
+    ``seed``: the draws of a request are a function of it and of the token's position; None: a seed of its own for every request."""
+    temperature: float = 1.0
+    top_k: int = 0                     # 0: no limit
+    top_p: float = 1.0                 # 1: no limit
+    min_p: float = 0.0                 # 0: no limit
+    seed: Optional[int] = None
+
+    def __post_init__(self):
+        if not 0.0 <= self.temperature < float("inf"):
+            raise ValueError(f"temperature must be finite and not negative, got {self.temperature}")
+        if self.top_k < 0 or self.top_k >= 1 << 31 or not 0.0 <= self.top_p <= 1.0 or not 0.0 <= self.min_p <= 1.0:
+            raise ValueError(f"top_k must not be negative, top_p and min_p lie in [0, 1]: got {self.top_k}, {self.top_p}, {self.min_p}")
+
+
+def uniform_at(seed: int, position: int) -> float:
+    """A number of [0, 1) for a token's position, a multiple of 2^-24: SplitMix64 (Steele, Lea, Flood 2014) of the seed's
+    stream at that position."""
+    mask = (1 << 64) - 1
+
+    def mix(z):
+        z = ((z ^ (z >> 30)) * 0xBF58476D1CE4E5B9) & mask
+        z = ((z ^ (z >> 27)) * 0x94D049BB133111EB) & mask
+        return z ^ (z >> 31)
+    state = mix((seed + 0x9E3779B97F4A7C15) & mask)
+    return (mix((state + (position + 1) * 0x9E3779B97F4A7C15) & mask) >> 40) / float(1 << 24)
+
+
+@dataclass
 class Request:
     prompt_tokens: List[int]
     max_tokens: int = 256
@@ -75,6 +106,20 @@ class Request:
     finish_time: Optional[float] = None
     prefilled: int = 0                 # prompt tokens already in the KV cache
     text: str = ""
+    sampling: Optional[SamplingParameters] = None        # None: the likeliest token every time
+    draw: Optional[tuple] = None       # what the next token is drawn with, where another rank has settled it
+    _seed: Optional[int] = None
+
+    def next_draw(self) -> Optional[Tuple[float, float, int, float, float]]:
+        """(u, temperature, top_k, top_p, min_p) of the next token; None: the likeliest one."""
+        if self.draw is not None:
+            return self.draw
+        s = self.sampling
+        if s is None or s.temperature <= 0.0:
+            return None
+        if self._seed is None:
+            self._seed = s.seed if s.seed is not None else random.getrandbits(64)
+        return uniform_at(self._seed, self.total_tokens), s.temperature, s.top_k, s.top_p, s.min_p
 
     @property
     def total_tokens(self) -> int:
@@ -642,6 +687,13 @@ class PrefillHandler:
 class GenerationOptions:
     stop_strings: Sequence[str] = ()
     temperature: float = 0.0
+    top_k: int = 0
+    top_p: float = 1.0
+    min_p: float = 0.0
+    seed: Optional[int] = None
+
+    def sampling(self) -> Optional[SamplingParameters]:
+        return SamplingParameters(self.temperature, self.top_k, self.top_p, self.min_p, self.seed) if self.temperature else None
 
 
 class ContinuousBatchSchedulerClient:
@@ -653,7 +705,8 @@ class ContinuousBatchSchedulerClient:
     def submit(self, prompt: str, max_tokens: int = 256, priority: Priority = Priority.NORMAL,
                options: Optional[GenerationOptions] = None) -> Request:
         ids = self.tok.encode(prompt)
-        r = Request(ids, max_tokens, priority, prompt, (options or GenerationOptions()).stop_strings)
+        opt = options or GenerationOptions()
+        r = Request(ids, max_tokens, priority, prompt, opt.stop_strings, sampling=opt.sampling())
         self.s.enqueue(r)
         return r
 

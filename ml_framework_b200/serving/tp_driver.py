@@ -28,8 +28,8 @@ class TPLeaderExecutor:
         live = {r.id for r in batch.requests} | {r.id for r in batch.prefill} | {r.id for r in batch.decode}
         if self.live_ids_fn is not None:
             live |= set(self.live_ids_fn())
-        plan = {"prefill": [(r.id, list(r.prompt_tokens), r.prefilled) for r in batch.prefill],
-                "decode": [(r.id, (r.generated[-1] if r.generated else r.prompt_tokens[-1])) for r in batch.decode],
+        plan = {"prefill": [(r.id, list(r.prompt_tokens), r.prefilled, r.next_draw()) for r in batch.prefill],
+                "decode": [(r.id, (r.generated[-1] if r.generated else r.prompt_tokens[-1]), r.next_draw()) for r in batch.decode],
                 "live": sorted(live)}
         self.pg.broadcast_object(plan, src=0)
         return self.ex.execute_batch(batch)
@@ -51,17 +51,17 @@ def follower_loop(executor: PagedLlamaExecutor, pg) -> int:
             executor.kv.free_sequence_blocks(rid)
             del shadow[rid]
         prefill, decode = [], []
-        for rid, prompt, prefilled in plan["prefill"]:
+        for rid, prompt, prefilled, draw in plan["prefill"]:
             r = shadow.get(rid)
             if r is None:
                 r = Request(list(prompt))
                 r.id = rid
                 shadow[rid] = r
-            r.prefilled = prefilled
+            r.prefilled, r.draw = prefilled, draw
             prefill.append(r)
-        for rid, last in plan["decode"]:
+        for rid, last, draw in plan["decode"]:
             r = shadow[rid]
-            r.generated = [last]                                   # the executor reads only the last token
+            r.generated, r.draw = [last], draw                     # the executor reads only the last token and how to draw the next
             decode.append(r)
         executor.execute_batch(Batch(requests=list(shadow.values()), prefill=prefill, decode=decode))
         iters += 1
