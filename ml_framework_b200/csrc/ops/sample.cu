@@ -11,14 +11,16 @@
 // their order, so that a row gives the same token in any batch and with any number of CTAs, and a border between
 // two tokens is as sharp as the weights themselves.
 //
-// A cluster of CTAs takes a row, and each lane keeps its 32 logits in shared memory where eight CTAs can (up to 131072; rows of more
-// are read again in every pass, from the caches): a pass costs its arithmetic and an exchange through distributed shared memory.
-// (1) Largest logit, and the mean of a sample. (2) Where k or p limits the row: counts (and weights, for p alone) in bins
-// of equal width from the largest logit down to about the mean, which spread the atomics of a few thousand candidates over as many
-// addresses. (3) The bins down to the one that decides hold few tokens as a rule: these go to a list in one CTA, where the token is
-// decided. Where a p alone keeps too many, only the deciding bin is listed, and where even that is too long the deciding value
-// is found digit by digit over the row, 11 + 11 + 10 bits of the order-preserving integer of a float. (4) The token from sums of
-// 256 neighbours.
+// A cluster of CTAs takes a row, and each lane keeps its logits in shared memory where eight CTAs can (rows of more are read again in
+// every pass, from the caches): a pass costs its arithmetic and an exchange through distributed shared memory.
+// (1) Largest logit, and mean and variance of a sample.
+// (2) Where k limits the row, or a p under which few tokens are expected: the bins of equal width that hold the k (256) largest
+// of the maxima of eight neighbours hold at least as many tokens, and hardly more. These go to a list in one CTA, where the token
+// is decided: eight logits cost one comparison in both passes.
+// (3) Where p alone keeps many tokens: the weights of all of them in bins, and the deciding bin alone in the list.
+// (4) Where a list is too long (many equal logits), the deciding value digit by digit over the row, 11 + 11 + 10 bits of the
+// order-preserving integer of a float.
+// (5) After (3), (4) or no limit: the token from sums of 256 neighbours.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 
@@ -35,9 +37,12 @@ constexpr int SM_WARPS = 16;
 constexpr int SM_THREADS = SM_WARPS * 32;
 constexpr int SM_STEP = 256;                   // logits that a warp takes at a time, eight a lane
 constexpr int SM_HELD = 4;                     // such steps that a warp can keep in shared memory
-constexpr int SM_STEPS = 64;                   // at most, per warp
+constexpr int SM_STEPS = 32;                   // at most, per warp
 constexpr int SM_BINS = 2048;
-constexpr int SM_LIST = 2048;
+constexpr int SM_GROUPS = 64;                  // sums of neighbouring bins that CTAs exchange
+constexpr int SM_COARSE = 512;                 // bins of the maxima
+constexpr int SM_LIST = 2048;                  // tokens that a list takes
+constexpr int SM_FEW = 256;                    // tokens that a p alone is expected to keep, where they are listed
 constexpr int SM_CLUSTER = 8;                  // CTAs per row, at most
 constexpr int SM_ONE = 40;                     // log2 of the weight of the largest logit
 
@@ -57,23 +62,27 @@ __constant__ unsigned c_exp2[32] = {           // 2^(j / 32) in units of 2^-31
     0xce248c15u, 0xd2a81d92u, 0xd744fccbu, 0xdbfbb798u, 0xe0ccdeecu, 0xe5b906e7u, 0xeac0c6e8u, 0xefe4b99cu, 0xf5257d15u, 0xfa83b2dbu};
 
 struct SampleSmem {
-  u64 list[SM_LIST];
   union {
-    struct { unsigned lo[SM_BINS], hi[SM_BINS]; };          // weights of the bins
-    u64 local[SM_LIST];                                     // the list's entries of this CTA, later scratch of the list
-    ulonglong2 pair[SM_THREADS];
+    u64 list[2 * SM_LIST];                     // every CTA has a part of it in rank 0
+    struct {
+      u64 part[SM_LIST];
+      alignas(16) unsigned lo[SM_BINS];        // weights of the bins
+      alignas(16) unsigned hi[SM_BINS];
+    };
   };
   union {
     alignas(16) unsigned cnt[SM_BINS];         // counts of the bins
     u64 step[SM_WARPS * SM_STEPS];             // sums of 256 logits' values
+    ulonglong2 pair[SM_THREADS];               // tokens of the list with their weights
   };
-  u64 slot[6][4][SM_CLUSTER];                  // one set per exchange of a launch: values of every CTA
+  u64 slot[8][3][SM_CLUSTER];                  // one set per exchange of a launch: values of every CTA
+  u64 last;
   u64 warp[SM_WARPS];
-  u64 res[4];
-  unsigned exp2[32];
-  int n_list, base;
+  u64 res[5];
+  u64 group[SM_GROUPS * SM_CLUSTER];
+  uint2 exp2[32];
   int n_local;
-  alignas(16) uint4 held[1];                   // SM_HELD steps, as far as the launch has room for them
+  alignas(16) uint4 held[1];                   // SM_HELD steps of logits, or the maxima of all steps, as far as the launch goes
 };
 
 // Order-preserving integer of a float that is not NaN; -0 and subnormal numbers are 0.
@@ -87,30 +96,31 @@ __device__ __forceinline__ float sm_entry_value(u64 e) { return sm_value(~(unsig
 
 struct SampleWeight {
   float m, ch, cl;                             // log2(e) / T in two floats
-  const unsigned* table;
+  const uint2* table;                          // 2^(j / 32) in units of 2^-31: the integer, and its bits as a float
   __device__ __forceinline__ u64 operator()(float x) const {     // NaN and -inf: 0
-    if (x == m) return 1ull << SM_ONE;
+    if (m == INFINITY) return x == m ? 1ull << SM_ONE : 0ull;
     const float s = __fsub_rn(x, m), t = __fsub_rn(s, x);
     const float r = __fadd_rn(__fsub_rn(x, __fsub_rn(s, t)), -__fadd_rn(m, t));     // x - m = s + r
     const float p = __fmul_rn(s, ch);
-    if (!(p > -(SM_ONE + 2.f))) return 0ull;
+    if (!(p > -(SM_ONE + 1.f))) return x == m ? 1ull << SM_ONE : 0ull;              // 0 times an infinite log2(e) / T is 0
     const float e = __fmaf_rn(r, ch, __fmaf_rn(s, cl, __fmaf_rn(s, ch, -p)));
     const float big = __fmaf_rn(p, 32.f, 12582912.f);                               // p in 32nds, an integer in the low bits
     const int j = __float_as_int(big) - 0x4b400000;
     const float f = __fadd_rn(__fmaf_rn(__fsub_rn(big, 12582912.f), -0.03125f, p), e);
     // 2^f - 1 = e^(f ln 2) - 1, |f| <= 1 / 64: four terms of the series, the fifth is 2^-39
     const float q = __fmul_rn(f, __fmaf_rn(f, __fmaf_rn(f, __fmaf_rn(f, 0.0096181291f, 0.055504109f), 0.24022651f), 0.69314718f));
-    const unsigned tj = table[j & 31];
-    const u64 w = (u64)(tj + (unsigned)__float2int_rn(__fmul_rn(q, (float)tj))) << (SM_ONE - 31);
-    const int down = -(j >> 5);
-    return down > 0 ? (w + (1ull << (down - 1))) >> down : w;
+    const uint2 tj = table[j & 31];
+    const unsigned w = tj.x + (unsigned)__float2int_rn(__fmul_rn(q, __uint_as_float(tj.y)));
+    const int up = SM_ONE - 31 + (j >> 5);     // the exponent: shift left, or right with rounding as the upper word of a product
+    return up >= 0 ? (u64)w << up : ((u64)w * (1u << (32 + up)) + 0x80000000ull) >> 32;
   }
 };
+static_assert(SM_ONE <= 41, "right shifts of 32 bits at most");
 
+// Sum over a warp of numbers below 2^44, in two halves of 22 bits.
 __device__ __forceinline__ u64 sm_warp_sum(u64 v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
+  const unsigned lo = __reduce_add_sync(0xffffffffu, (unsigned)v & 0x3fffffu), hi = __reduce_add_sync(0xffffffffu, (unsigned)(v >> 22));
+  return ((u64)hi << 22) + lo;
 }
 __device__ __forceinline__ u64 sm_warp_scan(u64 v) {       // inclusive
   const int lane = threadIdx.x & 31;
@@ -171,6 +181,7 @@ struct SampleRow {
   const T* row;
   int vocab, steps, first, vec;
   uint4* held;                                 // this lane's 16 bytes of step 0 in shared memory; a step is WORDS / 4 pieces of 512 lanes
+  float* maxima;                               // else: this lane's largest logit of step 0, 512 lanes a step
 
   __device__ __forceinline__ int index(int step) const { return first + step * SM_STEP + (threadIdx.x & 31) * 8; }
   __device__ __forceinline__ void fetch(int step, unsigned (&w)[WORDS]) const {
@@ -227,6 +238,46 @@ struct SampleRow {
     for (int j = 0; j < 8; ++j)
       x[j] = __uint_as_float(sizeof(T) == 4 ? w[j % WORDS] : j & 1 ? w[j / 2] & 0xffff0000u : w[j / 2] << 16);
   }
+  // the largest of a lane's eight logits; NaN only where all are
+  __device__ __forceinline__ static float maximum(const unsigned (&w)[WORDS]) {
+    if (sizeof(T) == 2) {
+      const __nv_bfloat162 h = __hmax2(__hmax2(*reinterpret_cast<const __nv_bfloat162*>(&w[0]), *reinterpret_cast<const __nv_bfloat162*>(&w[1])),
+                                       __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&w[2]), *reinterpret_cast<const __nv_bfloat162*>(&w[3])));
+      return fmaxf(__low2float(h), __high2float(h));
+    }
+    float v = __uint_as_float(w[0]);
+#pragma unroll
+    for (int j = 1; j < WORDS; ++j) v = fmaxf(v, __uint_as_float(w[j]));
+    return v;
+  }
+  __device__ __forceinline__ float maximum(int step) const {
+    if (!HELD) return maxima[step * SM_THREADS];
+    unsigned w[WORDS];
+    words(step, w);
+    return maximum(w);
+  }
+  // The first pass: f(step, maximum) with the maxima noted; four steps' loads at a time.
+  template <typename F>
+  __device__ __forceinline__ void first_pass(F f) const {
+    if (HELD) {
+      each([&](int st) { f(st, maximum(st)); });
+      return;
+    }
+    constexpr int AHEAD = 4;
+    for (int st = 0; st < steps; st += AHEAD) {
+      unsigned w[AHEAD][WORDS];
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j)
+        if (st + j < steps) fetch(st + j, w[j]);
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j)
+        if (st + j < steps) {
+          const float v = maximum(w[j]);
+          maxima[(st + j) * SM_THREADS] = v;
+          f(st + j, v);
+        }
+    }
+  }
   template <typename F>
   __device__ __forceinline__ void each(F f) const {
 #pragma unroll 1
@@ -236,52 +287,103 @@ struct SampleRow {
 
 struct SampleSplit { unsigned bin; u64 cnt, w, target; };   // the deciding bin (SM_BINS: none), what lies above it, what was looked for
 
-// First bin at which the cluster's running count (by_weight: weight) reaches `target`, or all there is where that is less (all_there).
-__device__ __forceinline__ SampleSplit sm_find(cg::cluster_group& cl, SampleSmem& s, int C, bool by_weight, bool weights, u64 target, bool all_there, unsigned* in_bin) {
-  constexpr int PER = SM_BINS / SM_THREADS;
-  const int b0 = threadIdx.x * PER;
-  unsigned c[PER];
-  u64 w[PER], sum_c = 0, sum_w = 0;
-#pragma unroll
-  for (int j = 0; j < PER; ++j) { c[j] = 0; w[j] = 0; }
-  for (int r = 0; r < C; ++r) {
-    const uint4 x = *reinterpret_cast<const uint4*>(cl.map_shared_rank(s.cnt, r) + b0);
-    c[0] += x.x; c[1] += x.y; c[2] += x.z; c[3] += x.w;
-    if (weights) {
-      const uint4 lo = *reinterpret_cast<const uint4*>(cl.map_shared_rank(s.lo, r) + b0), hi = *reinterpret_cast<const uint4*>(cl.map_shared_rank(s.hi, r) + b0);
-      w[0] += (u64)hi.x << 32 | lo.x; w[1] += (u64)hi.y << 32 | lo.y; w[2] += (u64)hi.z << 32 | lo.z; w[3] += (u64)hi.w << 32 | lo.w;
-    }
-  }
-#pragma unroll
-  for (int j = 0; j < PER; ++j) { sum_c += c[j]; sum_w += w[j]; }
-  u64 all;
-  u64 before_c = sm_block_scan(sum_c, s, &all), before_w = 0;
-  if (all_there && !by_weight) target = min(target, all);
-  if (weights) before_w = sm_block_scan(sum_w, s, &all);
-  if (threadIdx.x == 0) s.res[0] = SM_BINS;
-  __syncthreads();
+// First bin at which the cluster's running count (by_weight: weight) reaches target(weights of all), or all there is where that is
+// less (all_there). Every CTA tells the others the sums of 64 groups of its bins (`group`: 64 x SM_CLUSTER values of counts, then of
+// weights, as far as they are asked for) and its `here`, whose sum is handed to target; the deciding group's bins are then
+// read from every CTA. One exchange, and a sixteenth of what reading all bins of all CTAs moved.
+template <typename F>
+__device__ __forceinline__ SampleSplit sm_find(cg::cluster_group& cl, SampleSmem& s, u64* group, u64* slot, int C, int rank, bool counts, bool by_weight, u64 here,
+                                               F target_of, bool all_there, unsigned* in_bin) {
+  constexpr int PER = SM_BINS / SM_THREADS, GROUP = SM_BINS / SM_GROUPS;      // bins of a thread, of a group
+  static_assert(PER * SM_THREADS == SM_BINS && GROUP == 32 && GROUP / PER == SM_CLUSTER, "a lane of a group for every CTA, a lane for every bin");
+  const int tid = threadIdx.x, lane = tid & 31;
+  u64* group_w = group + (counts ? SM_GROUPS * SM_CLUSTER : 0);
+  __syncthreads();                             // this CTA's bins are complete
+  u64 sum_c = 0, sum_w = 0;
 #pragma unroll
   for (int j = 0; j < PER; ++j) {
-    const u64 b = by_weight ? before_w : before_c, a = by_weight ? w[j] : c[j];
-    if (a > 0 && b < target && b + a >= target) {
-      s.res[0] = b0 + j;
-      s.res[1] = before_c;
-      s.res[2] = before_w;
-      s.res[3] = c[j];
+    if (counts) sum_c += s.cnt[tid * PER + j];
+    sum_w += (u64)s.hi[tid * PER + j] << 32 | s.lo[tid * PER + j];
+  }
+#pragma unroll
+  for (int o = 1; o < GROUP / PER; o <<= 1) {
+    sum_c += __shfl_xor_sync(0xffffffffu, sum_c, o);
+    sum_w += __shfl_xor_sync(0xffffffffu, sum_w, o);
+  }
+  const int g = tid / (GROUP / PER), q0 = tid % (GROUP / PER);          // GROUP / PER = 8 lanes of a group: one CTA each
+  if (q0 < C) {
+    if (counts) cl.map_shared_rank(group, q0)[g * SM_CLUSTER + rank] = sum_c;
+    cl.map_shared_rank(group_w, q0)[g * SM_CLUSTER + rank] = sum_w;
+  }
+  if (tid < C) cl.map_shared_rank(slot, tid)[rank] = here;
+  cl.sync();
+  u64 all = 0;
+  for (int i = 0; i < C; ++i) all += slot[i];
+  u64 target = target_of(all);
+  if (tid < 32) {
+    // two groups a lane, then one bin a lane
+    u64 c[2] = {0, 0}, w[2] = {0, 0};
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      for (int i = 0; i < C; ++i) {
+        if (counts) c[j] += group[(2 * lane + j) * SM_CLUSTER + i];
+        w[j] += group_w[(2 * lane + j) * SM_CLUSTER + i];
+      }
+    const u64 end_c = sm_warp_scan(c[0] + c[1]), end_w = sm_warp_scan(w[0] + w[1]);
+    if (all_there && !by_weight) target = min(target, __shfl_sync(0xffffffffu, end_c, 31));
+    u64 bc = end_c - c[0] - c[1], bw = end_w - w[0] - w[1];
+    int mine = -1;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const u64 b = by_weight ? bw : bc, a = by_weight ? w[j] : c[j];
+      if (mine < 0) {
+        if (a > 0 && b < target && b + a >= target) mine = 2 * lane + j;
+        else { bc += c[j]; bw += w[j]; }
+      }
     }
-    before_c += c[j];
-    before_w += w[j];
+    const unsigned hit = __ballot_sync(0xffffffffu, mine >= 0);
+    if (hit == 0) {
+      if (lane == 0) { s.res[0] = SM_BINS; s.res[1] = s.res[2] = s.res[3] = 0; }
+    } else {
+      const int owner = __ffs(hit) - 1;
+      const int bin = __shfl_sync(0xffffffffu, mine, owner) * GROUP + lane;
+      bc = __shfl_sync(0xffffffffu, bc, owner);
+      bw = __shfl_sync(0xffffffffu, bw, owner);
+      u64 n = 0, v = 0;
+      for (int i = 0; i < C; ++i) {
+        if (counts) n += cl.map_shared_rank(s.cnt, i)[bin];
+        v += (u64)cl.map_shared_rank(s.hi, i)[bin] << 32 | cl.map_shared_rank(s.lo, i)[bin];
+      }
+      bc += sm_warp_scan(n) - n;
+      bw += sm_warp_scan(v) - v;
+      const u64 b = by_weight ? bw : bc, a = by_weight ? v : n;
+      if (a > 0 && b < target && b + a >= target) { s.res[0] = bin; s.res[1] = bc; s.res[2] = bw; s.res[3] = n; }
+    }
+    if (lane == 0) s.res[4] = target;
   }
   __syncthreads();
   SampleSplit out;
   out.bin = (unsigned)s.res[0];
   out.cnt = s.res[1];
   out.w = s.res[2];
-  out.target = target;
+  out.target = s.res[4];
   *in_bin = (unsigned)s.res[3];
   return out;
 }
-static_assert(SM_BINS == 4 * SM_THREADS, "four bins a thread");
+
+// The same by counts in SM_COARSE bins, one a thread, which every CTA reads from all (after an exchange).
+__device__ __forceinline__ SampleSplit sm_find_coarse(cg::cluster_group& cl, SampleSmem& s, int C, u64 target) {
+  u64 n = 0, all;
+  for (int i = 0; i < C; ++i) n += cl.map_shared_rank(s.cnt, i)[threadIdx.x];
+  if (threadIdx.x == 0) s.res[0] = SM_COARSE;
+  const u64 before = sm_block_scan(n, s, &all);
+  if (n > 0 && before < target && before + n >= target) s.res[0] = threadIdx.x;
+  __syncthreads();
+  SampleSplit out;
+  out.bin = (unsigned)s.res[0];
+  return out;
+}
+static_assert(SM_COARSE == SM_THREADS, "one bin a thread");
 
 // One weight into a bin: 64 bits from two native 32-bit atomics, whatever their order.
 __device__ __forceinline__ void sm_add(SampleSmem& s, int b, u64 w) {
@@ -300,9 +402,9 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_rows_kernel(const Sample
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   pdl_trigger();
   cl.barrier_arrive();                         // no CTA of the cluster is written to before it runs
-  if (tid < 32) s.exp2[tid] = c_exp2[tid];
-  if (tid == 0) s.n_list = s.n_local = 0;
-  for (int i = tid; i < SM_BINS; i += SM_THREADS) s.cnt[i] = s.lo[i] = s.hi[i] = 0;
+  if (tid < 32) s.exp2[tid] = make_uint2(c_exp2[tid], __float_as_uint((float)c_exp2[tid]));
+  if (tid == 0) s.n_local = 0;
+  for (int i = tid; i < SM_COARSE; i += SM_THREADS) s.cnt[i] = 0;
   pdl_wait();
   const int r = blockIdx.x / C;
   SampleRow<T, HELD> row;
@@ -312,35 +414,17 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_rows_kernel(const Sample
   row.steps = max(0, min(p.steps, (p.vocab - row.first + SM_STEP - 1) / SM_STEP));
   row.vec = p.vec;
   row.held = s.held + tid;
+  row.maxima = reinterpret_cast<float*>(s.held) + tid;
   row.hold();
   const float temp = p.temperature[r], top_p = p.top_p ? p.top_p[r] : 1.f, min_p = p.min_p ? p.min_p[r] : 0.f, u = p.u[r];
   const int top_k = p.top_k ? p.top_k[r] : 0;
   const bool greedy = !(temp > 0.f) || min_p > 1.f;          // the first token of the order alone
 
-  // ---- (1) the largest logit, with its first index where that is the answer, and a mean
-  float best = -INFINITY, sum = 0.f;
+  // ---- (1) the largest logit, with its first index where that is the answer; mean and variance of the first step
+  float best = -INFINITY, sum = 0.f, square = 0.f;
   int best_st = 0, n_sum = 0;
-  row.each([&](int st) {
-    unsigned w[SampleRow<T, HELD>::WORDS];
-    row.words(st, w);
-    float v;
-    if (sizeof(T) == 2) {
-      __nv_bfloat162 h = __hmax2(__hmax2(*reinterpret_cast<__nv_bfloat162*>(&w[0]), *reinterpret_cast<__nv_bfloat162*>(&w[1])),
-                                 __hmax2(*reinterpret_cast<__nv_bfloat162*>(&w[2]), *reinterpret_cast<__nv_bfloat162*>(&w[3])));
-      v = fmaxf(__low2float(h), __high2float(h));
-    } else {
-      v = __uint_as_float(w[0]);
-#pragma unroll
-      for (int j = 1; j < SampleRow<T, HELD>::WORDS; ++j) v = fmaxf(v, __uint_as_float(w[j]));
-    }
+  row.first_pass([&](int st, float v) {
     if (v > best) { best = v; best_st = st; }
-    if (st == 0) {
-      float x[8];
-      row.values(st, x);
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (x[j] > -INFINITY) { sum += x[j]; ++n_sum; }
-    }
   });
   u64 top;
   if (greedy) {
@@ -360,33 +444,50 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_rows_kernel(const Sample
     }
   } else {
     top = (u64)__reduce_max_sync(0xffffffffu, sm_key(best)) << 32;
+    if (row.steps > 0) {
+      float x[8];
+      row.values(0, x);
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (x[j] > -INFINITY) { sum += x[j]; square += x[j] * x[j]; ++n_sum; }
+    }
     n_sum = __reduce_add_sync(0xffffffffu, n_sum);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    for (int o = 16; o > 0; o >>= 1) {
+      sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      square += __shfl_xor_sync(0xffffffffu, square, o);
+    }
   }
-  if (lane == 0) { s.list[warp] = top; s.list[SM_WARPS + warp] = (u64)__float_as_uint(sum) << 32 | (unsigned)n_sum; }
+  if (lane == 0) {
+    s.list[warp] = top;
+    s.list[SM_WARPS + warp] = (u64)__float_as_uint(sum) << 32 | __float_as_uint(square);
+    s.list[2 * SM_WARPS + warp] = (u64)n_sum;
+  }
   __syncthreads();
   cl.barrier_wait();
   if (tid < C) {                               // thread i tells CTA i
-    u64 t = 0;
-    float f = 0.f;
-    unsigned n = 0;
+    u64 t = 0, n = 0;
+    float f = 0.f, g = 0.f;
+#pragma unroll
     for (int i = 0; i < SM_WARPS; ++i) {
       t = max(t, s.list[i]);
       f += __uint_as_float((unsigned)(s.list[SM_WARPS + i] >> 32));
-      n += (unsigned)s.list[SM_WARPS + i];
+      g += __uint_as_float((unsigned)s.list[SM_WARPS + i]);
+      n += s.list[2 * SM_WARPS + i];
     }
     u64* to = cl.map_shared_rank(&s.slot[0][0][0], tid);
     to[rank] = t;
-    to[SM_CLUSTER + rank] = (u64)__float_as_uint(f) << 32 | n;
+    to[SM_CLUSTER + rank] = (u64)__float_as_uint(f) << 32 | __float_as_uint(g);
+    to[2 * SM_CLUSTER + rank] = n;
   }
   cl.sync();
-  float mean = 0.f, n_mean = 0.f;
+  float mean = 0.f, var = 0.f, n_mean = 0.f;
   top = 0;
   for (int i = 0; i < C; ++i) {
     top = max(top, s.slot[0][0][i]);
     mean += __uint_as_float((unsigned)(s.slot[0][1][i] >> 32));
-    n_mean += (float)(unsigned)s.slot[0][1][i];
+    var += __uint_as_float((unsigned)s.slot[0][1][i]);
+    n_mean += (float)(unsigned)s.slot[0][2][i];
   }
   const float m = sm_value((unsigned)(top >> 32));
   if (m == -INFINITY || greedy) {
@@ -397,16 +498,16 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_rows_kernel(const Sample
     return;
   }
   mean = __fdiv_rn(mean, n_mean);
+  var = __fdiv_rn(var, n_mean) - mean * mean;
   SampleWeight weight;
   const double scale = 1.4426950408889634074 / (double)temp;
   weight.m = m;
   weight.ch = (float)scale;
   weight.cl = isinf(weight.ch) ? 0.f : (float)(scale - (double)weight.ch);
   weight.table = s.exp2;
-  auto finish = [&](long long token, u64 total) {           // one thread of the row
+  auto finish = [&](long long token, float x, u64 total) {  // one thread of the row
     p.tokens[r] = token;
     if (p.logprobs) {
-      const float x = (float)row.row[token];
       const double lw = x == m ? 0. : ((double)x - (double)m) / (double)temp;
       p.logprobs[r] = (float)(lw - log((double)total * (1. / (double)(1ull << SM_ONE))));
     }
@@ -430,7 +531,7 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_rows_kernel(const Sample
     ++ex;
     return make_ulonglong2(all, below);
   };
-  // ---- (4) the first index at which the running sum of value(logit, index) reaches target(total): found(index, total) in one thread
+  // ---- (5) the first index at which the running sum of value(logit, index) reaches target(total): found(index, logit, total) in one thread
   auto locate = [&](auto value, auto target, auto found) {
     row.each([&](int st) {
       float x[8];
@@ -477,106 +578,140 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_rows_kernel(const Sample
     u64 from = to - v;
     if (from < t && to >= t) {
       int j = 0;
+      float at_x = x[0];
 #pragma unroll
-      for (int q = 0; q < 8; ++q) {
+      for (int q = 0; q < 7; ++q) {
         from += e[q];
-        if (from < t) j = q + 1;
+        if (from < t) { j = q + 1; at_x = x[q + 1]; }
       }
-      found(i + j, a.x);
+      found(i + j, at_x, a.x);
     }
   };
 
   if (need_k || need_p) {
-    // ---- (2) bins of equal width from the largest logit down; p alone may reach below the mean
-    float per = __fdiv_rn((float)(SM_BINS - 1), (m - mean) * (need_k ? 1.f : 1.5f));
-    if (!(per > 0.f && per < 3e38f)) per = 0.f;
-    auto bin_of = [&](float x) {                            // NaN, -inf and what is below: the last one, in which nothing is counted
-      const float f = __fmul_rn(__fsub_rn(m, x), per);
-      return x > -INFINITY && f < (float)(SM_BINS - 1) ? (int)f : SM_BINS - 1;
+    u64 w_all = 0, target_p = ~0ull;
+    float per;
+    int n_bins;
+    auto bins = [&](int n, float width) {
+      n_bins = n;
+      per = __fdiv_rn((float)(n - 1), width);
+      if (!(per > 0.f && per < 3e38f)) per = 0.f;
     };
-    u64 w_here = 0;
-    row.each([&](int st) {
-      float x[8];
-      row.values(st, x);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int b = bin_of(x[j]);
-        if (b < SM_BINS - 1) atomicAdd(&s.cnt[b], 1u);
-        if (!need_k) {
-          const u64 w = weight(x[j]);
-          if (b < SM_BINS - 1) sm_add(s, b, w);
-          w_here += w;
-        }
-      }
-    });
-    u64 w_all = 0;
-    if (!need_k) {
+    auto bin_of = [&](float x) {                            // what is below the range: the last one; the order of the logits
+      const float f = __fmul_rn(__fsub_rn(m, x), per);
+      return f < (float)(n_bins - 1) ? (int)f : n_bins - 1;
+    };
+    auto block_sum = [&](u64 here) {
       u64 t;
-      sm_block_scan(w_here, s, &t);
-      w_all = exchange_sum(t).x;
-    } else {
-      cl.sync();
-    }
-    unsigned in_bin;
-    const u64 target_p = need_k ? ~0ull : max(1ull, sm_reach(top_p, w_all));
-    const SampleSplit sp = sm_find(cl, s, C, !need_k, !need_k, need_k ? (u64)top_k : target_p, false, &in_bin);
-    const bool whole = sp.cnt + in_bin <= SM_LIST;          // every candidate fits the list, not just the deciding bin
-    if (sp.bin < SM_BINS && (whole || (!need_k && in_bin <= SM_LIST))) {
-      // ---- (3) the list: gathered here, then in rank 0
-      if (!need_k) cl.sync();                  // the others have read the weights, whose place it takes
+      sm_block_scan(here, s, &t);
+      return t;
+    };
+    auto reach = [&](u64 all) {
+      w_all = all;
+      return target_p = max(1ull, sm_reach(top_p, all));
+    };
+    // The list: tokens that wanted() names, in rank 0; how many, or 0 where they do not fit. room: entries of a CTA's part.
+    int room = 0;
+    auto gather = [&](auto wanted) {
+      u64* to = cl.map_shared_rank(s.list, 0) + rank * room;
       row.each([&](int st) {
+        if (!wanted(row.maximum(st), true)) return;
         float x[8];
         row.values(st, x);
         const int i = row.index(st);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int b = bin_of(x[j]);
-          if (whole ? b <= (int)sp.bin : b == (int)sp.bin) s.local[atomicAdd(&s.n_local, 1)] = sm_entry(x[j], i + j);
-        }
+        for (int j = 0; j < 8; ++j)
+          if (x[j] > -INFINITY && wanted(x[j], false)) {
+            const int at = atomicAdd(&s.n_local, 1);
+            if (at < room) to[at] = sm_entry(x[j], i + j);
+          }
       });
       __syncthreads();
-      if (tid == 0) s.base = atomicAdd(cl.map_shared_rank(&s.n_list, 0), s.n_local);
-      __syncthreads();
-      u64* to = cl.map_shared_rank(s.list, 0) + s.base;
-      for (int i = tid; i < s.n_local; i += SM_THREADS) to[i] = s.local[i];
+      if (tid < C) cl.map_shared_rank(&s.slot[ex][0][0], tid)[rank] = (u64)s.n_local;
       cl.sync();
-      if (rank != 0 && whole) return;
-      if (rank == 0) {
-        const int n = (int)(whole ? sp.cnt + in_bin : in_bin), n_k = need_k ? top_k : n;
-        const u64 above = whole ? 0 : sp.w;    // weights that are kept and not in the list
-        auto last_one = [&](u64 e) {           // one thread: the last token that p keeps, to every CTA
-          for (int q = 0; q < C; ++q) cl.map_shared_rank(&s.slot[5][0][0], q)[0] = e;
-        };
-        if (n <= SM_THREADS) {
-          // a token per thread: what comes before it is counted and summed directly
-          u64 mine = ~0ull, w = 0, before = above;
-          int ahead = 0;
-          if (tid < n) {
-            mine = s.list[tid];
-            w = weight(sm_entry_value(mine));
-            s.pair[tid] = make_ulonglong2(mine, w);
-          }
-          __syncthreads();
-          if (tid < n)
-            for (int j = 0; j < n; ++j) {
-              const ulonglong2 o = s.pair[j];
-              if (o.x < mine) { ++ahead; before += o.y; }
-            }
+      int n = 0, most = 0;
+      for (int i = 0; i < C; ++i) {
+        const int c = (int)s.slot[ex][0][i];
+        n += c;
+        most = max(most, c);
+      }
+      if (tid == 0) s.n_local = 0;
+      ++ex;
+      return n <= SM_LIST && most <= room ? n : 0;
+    };
+    auto entry = [&](int i) {                               // rank 0: the i-th of the list, across the CTAs' parts
+      int q = 0;
+      for (; q < C - 1; ++q) {
+        const int c = (int)s.slot[ex - 1][0][q];
+        if (i < c) break;
+        i -= c;
+      }
+      return s.list[q * room + i];
+    };
+    bool open = true;
+    // p alone: a normal distribution with this mean and variance has V exp((mean - m) / T + var / 2 T^2) of the largest logit's weight, and
+    // z standard deviations above the mean 256 tokens, below which all but the upper tail beyond z - sigma / T of that weight
+    // lies. Where that is more than p leaves out, 256 tokens will not do. Only the way depends on it, not the token.
+    bool flat = false;
+    if (!need_k && p.vocab > SM_LIST) {
+      const float inv_t = __fdiv_rn(1.f, temp), t = sqrtf(2.f * __logf((float)p.vocab / SM_FEW));
+      const float z = t - (2.30753f + 0.27061f * t) / (1.f + t * (0.99229f + 0.04481f * t));      // Hastings' approximation of the normal quantile
+      const float bulk = __expf(__logf((float)p.vocab) + ((mean - m) + 0.5f * var * inv_t) * inv_t);
+      flat = bulk * normcdff(z - sqrtf(fmaxf(var, 0.f)) * inv_t) > (1.f - top_p) * (bulk + 2.f);
+    }
+    if (!flat) {
+      // ---- (2)
+      bins(SM_COARSE, m - mean);
+      u64 w_here = 0;
+      row.each([&](int st) {
+        const float v = row.maximum(st);
+        const int b = bin_of(v);
+        if (v > -INFINITY && b < SM_COARSE - 1) atomicAdd(&s.cnt[b], 1u);
+        if (!need_k) {
+          float x[8];
+          row.values(st, x);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) w_here += weight(x[j]);
+        }
+      });
+      if (need_k) cl.sync();
+      else reach(exchange_sum(block_sum(w_here)).x);
+      const SampleSplit sp = sm_find_coarse(cl, s, C, need_k ? (u64)top_k : (u64)SM_FEW);
+      const int upto = sp.bin < SM_COARSE ? (int)sp.bin : SM_COARSE - 1;           // fewer in the bins: everything
+      room = min(SM_LIST, 2 * SM_LIST / C);
+      const int n = gather([&](float x, bool) { return x > -INFINITY && bin_of(x) <= upto; });
+      if (n > 0) {
+        if (rank == 0) {
+          const int n_k = need_k ? min(top_k, n) : n;
           u64 target = target_p;
-          if (need_k && need_p) {
-            u64 all;
-            sm_block_scan(tid < n && ahead < n_k ? w : 0ull, s, &all);
-            target = sm_reach(top_p, all);
-          }
-          if (!whole) {
-            if (tid < n && before < target && before + w >= target) last_one(mine);
-          } else {
+          bool enough = true;
+          if (n <= SM_THREADS) {
+            // a token per thread: what comes before it is counted and summed directly
+            u64 mine = ~0ull, w = 0, before = 0;
+            int ahead = 0;
+            if (tid < n) {
+              mine = entry(tid);
+              w = weight(sm_entry_value(mine));
+              s.pair[tid] = make_ulonglong2(mine, w);
+            }
+            __syncthreads();
+            if (tid < n)
+              for (int j = 0; j < n; ++j) {
+                const ulonglong2 o = s.pair[j];
+                if (o.x < mine) { ++ahead; before += o.y; }
+              }
+            if (need_p) {
+              u64 all;
+              sm_block_scan(tid < n && ahead < n_k ? w : 0ull, s, &all);
+              if (need_k) target = sm_reach(top_p, all);
+              enough = all >= target;
+            }
             // kept: what begins below the target, is among the first k and not below min_p; the first token always
             const bool in = tid < n && ahead < n_k && (ahead == 0 || ((!need_p || before < target) && sm_entry_value(mine) >= least));
             __syncthreads();
             if (tid < n) s.pair[tid] = make_ulonglong2(mine, in ? w : 0ull);
             __syncthreads();
-            if (in) {
+            if (in && enough) {
               u64 all = 0;
               before = 0;
               for (int j = 0; j < n; ++j) {
@@ -585,71 +720,156 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_rows_kernel(const Sample
                 before += (unsigned)o.x < (unsigned)mine ? o.y : 0;
               }
               const u64 t = sm_above(u, all);
-              if (before < t && before + w >= t) finish((long long)(unsigned)mine, all);
+              if (before < t && before + w >= t) finish((long long)(unsigned)mine, sm_entry_value(mine), all);
             }
-            return;
-          }
-        } else {
-          int pow2 = 2;
-          while (pow2 < n) pow2 <<= 1;
-          for (int i = n + tid; i < pow2; i += SM_THREADS) s.list[i] = ~0ull;
-          sm_sort(s.list, pow2);
-          constexpr int PER = SM_LIST / SM_THREADS;
-          const int each = pow2 / SM_THREADS;
-          u64 w[PER], mine = 0, all;
+          } else {
+            constexpr int PER = SM_LIST / SM_THREADS;
+            int pow2 = 2 * SM_THREADS;
+            while (pow2 < n) pow2 <<= 1;
+            u64 e[PER];
 #pragma unroll
-          for (int j = 0; j < PER; ++j) {
-            const int i = tid * each + j;
-            w[j] = j < each && i < n && i < n_k ? weight(sm_entry_value(s.list[i])) : 0ull;
-            mine += w[j];
-          }
-          u64 before = above + sm_block_scan(mine, s, &all);
-          const u64 target = need_k && need_p ? sm_reach(top_p, all) : target_p;
-          u64 kept = 0;
+            for (int j = 0; j < PER; ++j) e[j] = tid + j * SM_THREADS < n ? entry(tid + j * SM_THREADS) : ~0ull;
+            __syncthreads();
 #pragma unroll
-          for (int j = 0; j < PER; ++j) {
-            const int i = tid * each + j;
-            const bool there = j < each && i < n && i < n_k;
-            if (!whole && there && before < target && before + w[j] >= target) last_one(s.list[i]);
-            if (there && (i == 0 || ((!need_p || before < target) && sm_entry_value(s.list[i]) >= least))) ++kept;
-            before += w[j];
-          }
-          if (whole) {
-            u64 n_kept;
-            sm_block_scan(kept, s, &n_kept);
-            const int nk = (int)n_kept;
-            int pow2k = 2;                     // the same by index
-            while (pow2k < nk) pow2k <<= 1;
-            for (int i = tid; i < pow2k; i += SM_THREADS) {
-              const u64 e = s.list[i];
-              s.local[i] = i < nk ? e << 32 | e >> 32 : ~0ull;
-            }
-            sm_sort(s.local, pow2k);
-            const int each_k = (pow2k + SM_THREADS - 1) / SM_THREADS;
-            mine = 0;
+            for (int j = 0; j < PER; ++j)
+              if (tid + j * SM_THREADS < pow2) s.list[tid + j * SM_THREADS] = e[j];
+            sm_sort(s.list, pow2);
+            const int each = pow2 / SM_THREADS;
+            u64 w[PER], mine = 0, all;
 #pragma unroll
             for (int j = 0; j < PER; ++j) {
-              const int i = tid * each_k + j;
-              w[j] = j < each_k && i < nk ? weight(sm_value(~(unsigned)s.local[i])) : 0ull;
+              const int i = tid * each + j;
+              w[j] = j < each && i < n_k ? weight(sm_entry_value(s.list[i])) : 0ull;
               mine += w[j];
             }
-            before = sm_block_scan(mine, s, &all);
-            const u64 t = sm_above(u, all);
+            u64 before = sm_block_scan(mine, s, &all);
+            if (need_k && need_p) target = sm_reach(top_p, all);
+            enough = !need_p || all >= target;
+            u64 kept = 0;
 #pragma unroll
             for (int j = 0; j < PER; ++j) {
-              if (before < t && before + w[j] >= t) finish((long long)(s.local[tid * each_k + j] >> 32), all);
+              const int i = tid * each + j;
+              if (j < each && i < n_k && (i == 0 || ((!need_p || before < target) && sm_entry_value(s.list[i]) >= least))) ++kept;
               before += w[j];
             }
-            return;
+            u64 n_kept;
+            sm_block_scan(kept, s, &n_kept);
+            if (enough) {
+              const int nk = (int)n_kept;
+              u64* by_index = s.list + SM_LIST;             // the same by index
+              int pow2k = 2;
+              while (pow2k < nk) pow2k <<= 1;
+              for (int i = tid; i < pow2k; i += SM_THREADS) {
+                const u64 x = s.list[i];
+                by_index[i] = i < nk ? x << 32 | x >> 32 : ~0ull;
+              }
+              sm_sort(by_index, pow2k);
+              const int each_k = (pow2k + SM_THREADS - 1) / SM_THREADS;
+              mine = 0;
+#pragma unroll
+              for (int j = 0; j < PER; ++j) {
+                const int i = tid * each_k + j;
+                w[j] = j < each_k && i < nk ? weight(sm_value(~(unsigned)by_index[i])) : 0ull;
+                mine += w[j];
+              }
+              before = sm_block_scan(mine, s, &all);
+              const u64 t = sm_above(u, all);
+#pragma unroll
+              for (int j = 0; j < PER; ++j) {
+                const int i = tid * each_k + j;
+                if (before < t && before + w[j] >= t) finish((long long)(by_index[i] >> 32), sm_value(~(unsigned)by_index[i]), all);
+                before += w[j];
+              }
+            }
           }
+          if (!need_k && tid < C) *cl.map_shared_rank(&s.last, tid) = enough ? 1ull : 0ull;
+        }
+        if (need_k) return;
+        cl.sync();
+        open = s.last == 0;
+        if (!open) return;
+      }
+    }
+    if (!need_k) {
+      // ---- (3) down to half as far below the mean as the largest logit is above it
+      for (int i = tid; i < SM_BINS; i += SM_THREADS) s.lo[i] = s.hi[i] = 0;
+      __syncthreads();
+      bins(SM_BINS, 1.5f * (m - mean));
+      u64 w_here = 0;
+      row.each([&](int st) {
+        float x[8];
+        row.values(st, x);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const u64 w = weight(x[j]);
+          const int b = bin_of(x[j]);
+          if (b < SM_BINS - 1 && w > 0) sm_add(s, b, w);
+          w_here += w;
+        }
+      });
+      unsigned in_bin;
+      const SampleSplit sp = sm_find(cl, s, s.group, s.slot[ex++][0], C, rank, false, true, block_sum(w_here), reach, false, &in_bin);
+      if (sp.bin < SM_BINS) {
+        room = SM_LIST / C;
+        const int n = gather([&](float x, bool any) { return any ? bin_of(x) <= (int)sp.bin : bin_of(x) == (int)sp.bin; });
+        if (n > 0) {
+          // the last token that p keeps: the one at which the running weight reaches the target
+          if (rank == 0) {
+            constexpr int PER = SM_LIST / SM_THREADS;
+            auto last_one = [&](u64 e) {
+              for (int q = 0; q < C; ++q) *cl.map_shared_rank(&s.last, q) = e;
+            };
+            if (n <= SM_THREADS) {
+              u64 mine = ~0ull, w = 0, before = sp.w;
+              if (tid < n) {
+                mine = entry(tid);
+                w = weight(sm_entry_value(mine));
+                s.pair[tid] = make_ulonglong2(mine, w);
+              }
+              __syncthreads();
+              if (tid < n) {
+                for (int j = 0; j < n; ++j) {
+                  const ulonglong2 o = s.pair[j];
+                  if (o.x < mine) before += o.y;
+                }
+                if (before < target_p && before + w >= target_p) last_one(mine);
+              }
+            } else {
+              int pow2 = 2 * SM_THREADS;
+              while (pow2 < n) pow2 <<= 1;
+              u64 e[PER];
+#pragma unroll
+              for (int j = 0; j < PER; ++j) e[j] = tid + j * SM_THREADS < n ? entry(tid + j * SM_THREADS) : ~0ull;
+              __syncthreads();
+#pragma unroll
+              for (int j = 0; j < PER; ++j)
+                if (tid + j * SM_THREADS < pow2) s.list[tid + j * SM_THREADS] = e[j];
+              sm_sort(s.list, pow2);
+              const int each = pow2 / SM_THREADS;
+              u64 w[PER], mine = 0, all;
+#pragma unroll
+              for (int j = 0; j < PER; ++j) {
+                const int i = tid * each + j;
+                w[j] = j < each && i < n ? weight(sm_entry_value(s.list[i])) : 0ull;
+                mine += w[j];
+              }
+              u64 before = sp.w + sm_block_scan(mine, s, &all);
+#pragma unroll
+              for (int j = 0; j < PER; ++j) {
+                if (before < target_p && before + w[j] >= target_p) last_one(s.list[tid * each + j]);
+                before += w[j];
+              }
+            }
+          }
+          cl.sync();
+          last_x = sm_entry_value(s.last);
+          last_i = (int)(unsigned)s.last;
+          open = false;
         }
       }
-      cl.sync();
-      const u64 e = s.slot[5][0][0];
-      last_x = sm_entry_value(e);
-      last_i = (int)(unsigned)e;
-    } else {
-      // ---- the deciding value by digits of its key, over the row
+    }
+    if (open) {
+      // ---- (4)
       auto decide = [&](bool by_weight, u64 target, u64* n_class, u64* n_above, u64* w_above) {
         unsigned prefix = 0;
         *n_above = *w_above = 0;
@@ -671,9 +891,9 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_rows_kernel(const Sample
               if (need_p) sm_add(s, b, weight(x[j]));
             }
           });
-          cl.sync();
           unsigned in_class;
-          const SampleSplit d = sm_find(cl, s, C, by_weight, need_p, target, level == 0, &in_class);
+          const u64 goal = target;
+          const SampleSplit d = sm_find(cl, s, s.part, s.slot[7][0], C, rank, true, by_weight, 0ull, [&](u64) { return goal; }, level == 0, &in_class);
           prefix = prefix << bits | ((1u << bits) - 1 - d.bin);
           done += bits;
           target = d.target - (by_weight ? d.w : d.cnt);
@@ -705,11 +925,11 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_rows_kernel(const Sample
       last_x = sm_value(key);
       if (n_take < n_class) {                  // some of the tokens with this logit: those of the lowest indices
         locate([&](float x, int) { return x == last_x ? 1ull : 0ull; }, [&](u64) { return n_take; },
-               [&](int i, u64) {
-                 for (int q = 0; q < C; ++q) cl.map_shared_rank(&s.slot[5][0][0], q)[0] = (u64)i;
+               [&](int i, float, u64) {
+                 for (int q = 0; q < C; ++q) *cl.map_shared_rank(&s.last, q) = (u64)i;
                });
         cl.sync();
-        last_i = (int)s.slot[5][0][0];
+        last_i = (int)s.last;
       }
     }
   }
@@ -718,18 +938,18 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_rows_kernel(const Sample
     last_i = 0x7fffffff;
   }
   locate([&](float x, int i) { return x > last_x || (x == last_x && i <= last_i) ? weight(x) : 0ull; }, [&](u64 total) { return sm_above(u, total); },
-         [&](int i, u64 total) { finish(i, total); });
+         [&](int i, float x, u64 total) { finish(i, x, total); });
 }
 
 }  // namespace mlf
 
 using namespace mlf;
 
-// CTAs per row: as many as keep the row in shared memory, and beyond that as bring the launch to two on every SM, up to SM_CLUSTER,
-// none of them with less than 4096 logits.
+// CTAs per row, up to SM_CLUSTER: as many as a warp's steps need, and as many as there are SMs for, none with less than 4096 logits.
+// SMC_TABLE
 static int sample_cluster(long long rows, int vocab) {
   int c = 1;
-  while (c < SM_CLUSTER && (vocab > c * SM_WARPS * SM_STEP * SM_HELD || (rows * c < 2 * sm_count() && vocab > c * 4096))) c *= 2;
+  while (c < SM_CLUSTER && (vocab > c * SM_WARPS * SM_STEP * SM_STEPS || (rows * c * 2 <= sm_count() && vocab > c * 4096))) c *= 2;
   return c;
 }
 
@@ -751,8 +971,8 @@ MLF_API int mlf_sample_rows(const void* logits, int is_fp32, long long rows, lon
   const bool held = p.steps <= SM_HELD;
   const auto kernel = is_fp32 ? (held ? sample_rows_kernel<float, true> : sample_rows_kernel<float, false>)
                               : (held ? sample_rows_kernel<__nv_bfloat16, true> : sample_rows_kernel<__nv_bfloat16, false>);
-  // shared memory for the most steps that are held: one size for every launch of a kernel
-  const size_t smem = sizeof(SampleSmem) + (held ? (size_t)SM_HELD * SM_THREADS * 8 * (is_fp32 ? 4 : 2) : 0);
+  // for the most steps, held or noted: one size for every launch of a kernel
+  const size_t smem = sizeof(SampleSmem) + (held ? (size_t)SM_HELD * SM_THREADS * 8 * (is_fp32 ? 4 : 2) : (size_t)SM_STEPS * SM_THREADS * sizeof(float));
   static bool attr_set[64][4] = {};
   int dev = 0;
   cudaGetDevice(&dev);

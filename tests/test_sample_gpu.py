@@ -79,6 +79,32 @@ def test_shapes_of_distributions(dtype, shape, which):
     _same(x.to(dtype), vocab, u, t, k, p, m)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("vocab", [40000, 128256, 140000])
+@pytest.mark.parametrize("shape", ["sorted", "few left", "first only", "hot bulk"])
+def test_where_candidates_lie(dtype, vocab, shape):
+    """Candidates side by side, a mask that leaves a handful, none in the first logits of every lane, a nucleus of most tokens;
+    vocabularies that shared memory holds and one that it does not."""
+    rows = 10
+    g = _gen(vocab)
+    x = 2 * torch.randn(rows, vocab, device="cuda", generator=g)
+    if shape == "sorted":
+        x = x.sort(1, descending=True)[0]
+    elif shape == "few left":
+        x = torch.where(torch.rand(rows, vocab, device="cuda", generator=g) < 1e-4, x, float("-inf"))
+        x[:, 5] = 1.0
+    elif shape == "first only":
+        x[:, 3000:] = float("-inf")
+    else:
+        x[:, 77] = 9.0
+    u = torch.rand(rows, device="cuda", generator=g)
+    t = torch.tensor([1.0, 0.5, 1.5, 1.0, 0.7, 1.0, 2.0, 0.3, 1.0, 1.0], device="cuda")
+    k = torch.tensor([0, 0, 0, 50, 300, 1500, 0, 40000, 600, 0], dtype=torch.int32, device="cuda")
+    p = torch.tensor([0.9, 0.95, 0.99, 0.9, 1.0, 0.9, 0.5, 0.9, 1.0, 0.9999], device="cuda")
+    m = torch.tensor([0, 0, 0, 0, 0.01, 0, 0, 0, 0, 0.001], device="cuda")
+    _same(x.to(dtype), vocab, u, t, k, p, m)
+
+
 def test_ends_of_u_and_odd_numbers():
     x = torch.tensor([[1.0, 3.0, 2.0, 3.0, float("nan"), float("-inf")]] * 6, device="cuda")
     x[3, 1] = float("inf")
