@@ -23,6 +23,7 @@
 // (5) After (3), (4) or no limit: the token from sums of 256 neighbours.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
+#include <float.h>
 
 #include "../common/host.h"
 #include "../common/ptx.cuh"
@@ -75,12 +76,12 @@ struct SampleSmem {
     u64 step[SM_WARPS * SM_STEPS];             // sums of 256 logits' values
     ulonglong2 pair[SM_THREADS];               // tokens of the list with their weights
   };
-  u64 slot[8][3][SM_CLUSTER];                  // one set per exchange of a launch: values of every CTA
+  u64 slot[10][3][SM_CLUSTER];                  // one set per exchange of a launch: values of every CTA
   u64 last;
   u64 warp[SM_WARPS];
   u64 res[5];
   u64 group[SM_GROUPS * SM_CLUSTER];
-  uint2 exp2[32];
+  unsigned exp2[32];
   int n_local;
   alignas(16) uint4 held[1];                   // SM_HELD steps of logits, or the maxima of all steps, as far as the launch goes
 };
@@ -94,25 +95,30 @@ __device__ __forceinline__ float sm_value(unsigned key) { return __uint_as_float
 __device__ __forceinline__ u64 sm_entry(float x, int i) { return (u64)(~sm_key(x)) << 32 | (unsigned)i; }      // ascending: the order of the tokens
 __device__ __forceinline__ float sm_entry_value(u64 e) { return sm_value(~(unsigned)(e >> 32)); }
 
+// x - m as the sum of two floats. Logits that were rounded to bf16 (8 bits): exact in one where the two are within 2^16 of each other,
+// the second is their difference's rounding where m is the larger, and where x is it is lost (2^-24 of x, which is then that
+// far below m). Others: always exact.
+template <bool BF16>
 struct SampleWeight {
-  float m, ch, cl;                             // log2(e) / T in two floats
-  const uint2* table;                          // 2^(j / 32) in units of 2^-31: the integer, and its bits as a float
+  float m, ch, cl;                             // 32 log2(e) / T in two floats
+  const unsigned* table;                       // 2^(j / 32) in units of 2^-31, one of the 32 banks each: any lanes read at once
   __device__ __forceinline__ u64 operator()(float x) const {     // NaN and -inf: 0
-    if (m == INFINITY) return x == m ? 1ull << SM_ONE : 0ull;
-    const float s = __fsub_rn(x, m), t = __fsub_rn(s, x);
-    const float r = __fadd_rn(__fsub_rn(x, __fsub_rn(s, t)), -__fadd_rn(m, t));     // x - m = s + r
-    const float p = __fmul_rn(s, ch);
-    if (!(p > -(SM_ONE + 1.f))) return x == m ? 1ull << SM_ONE : 0ull;              // 0 times an infinite log2(e) / T is 0
+    x = fminf(x, FLT_MAX);
+    const float s = __fsub_rn(x, m), t = __fadd_rn(s, m);
+    const float r = BF16 ? __fsub_rn(x, t) : __fadd_rn(__fsub_rn(x, __fsub_rn(s, __fsub_rn(s, x))), -__fadd_rn(m, __fsub_rn(s, x)));
+    const float p = fmaxf(__fmul_rn(s, ch), -2000.f);                               // 32nds of the exponent; 2^-62 is none
     const float e = __fmaf_rn(r, ch, __fmaf_rn(s, cl, __fmaf_rn(s, ch, -p)));
-    const float big = __fmaf_rn(p, 32.f, 12582912.f);                               // p in 32nds, an integer in the low bits
-    const int j = __float_as_int(big) - 0x4b400000;
-    const float f = __fadd_rn(__fmaf_rn(__fsub_rn(big, 12582912.f), -0.03125f, p), e);
-    // 2^f - 1 = e^(f ln 2) - 1, |f| <= 1 / 64: four terms of the series, the fifth is 2^-39
-    const float q = __fmul_rn(f, __fmaf_rn(f, __fmaf_rn(f, __fmaf_rn(f, 0.0096181291f, 0.055504109f), 0.24022651f), 0.69314718f));
-    const uint2 tj = table[j & 31];
-    const unsigned w = tj.x + (unsigned)__float2int_rn(__fmul_rn(q, __uint_as_float(tj.y)));
-    const int up = SM_ONE - 31 + (j >> 5);     // the exponent: shift left, or right with rounding as the upper word of a product
-    return up >= 0 ? (u64)w << up : ((u64)w * (1u << (32 + up)) + 0x80000000ull) >> 32;
+    const float big = __fadd_rn(p, 12582912.f);                                     // the next integer, in the low bits
+    const float f = __fadd_rn(__fsub_rn(p, __fsub_rn(big, 12582912.f)), e);
+    // 2^(f / 32) - 1, |f| <= 1 / 2: the series to f^3, with the middle of its fourth term in the second; off by 2^-32 at most
+    const float q = __fmul_rn(f, __fmaf_rn(f, __fmaf_rn(f, 1.6938529e-06f, 2.3459933e-04f), 2.1660849e-02f));
+    const int j = __float_as_int(big);                                              // 0x4b400000 + 32 exponent + 32nds
+    const unsigned tj = table[j & 31];
+    const unsigned w = tj + (unsigned)__float2int_rn(__fmul_rn(q, (float)tj));
+    const int up = (j >> 5) + (SM_ONE - 31 - (0x4b400000 >> 5));                    // shift left, or right with rounding: the upper word of a product
+    unsigned one;
+    asm("shl.b32 %0, 1, %1;" : "=r"(one) : "r"(32 + up));                           // 0 where that is negative
+    return up >= 0 ? (u64)w << up : ((u64)w * one + 0x80000000ull) >> 32;
   }
 };
 static_assert(SM_ONE <= 41, "right shifts of 32 bits at most");
@@ -234,9 +240,25 @@ struct SampleRow {
   __device__ __forceinline__ void values(int step, float (&x)[8]) const {
     unsigned w[WORDS];
     words(step, w);
+    unpack(w, x);
+  }
+  __device__ __forceinline__ static void unpack(const unsigned (&w)[WORDS], float (&x)[8]) {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
       x[j] = __uint_as_float(sizeof(T) == 4 ? w[j % WORDS] : j & 1 ? w[j / 2] & 0xffff0000u : w[j / 2] << 16);
+  }
+  // f(step, logits) over all steps, the next ones on their way
+  template <typename F>
+  __device__ __forceinline__ void each_values(F f) const {
+    unsigned w[WORDS];
+    if (steps > 0) words(0, w);
+#pragma unroll 1
+    for (int st = 0; st < steps; ++st) {
+      float x[8];
+      unpack(w, x);
+      if (st + 1 < steps) words(st + 1, w);
+      f(st, x);
+    }
   }
   // the largest of a lane's eight logits; NaN only where all are
   __device__ __forceinline__ static float maximum(const unsigned (&w)[WORDS]) {
@@ -402,7 +424,7 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_rows_kernel(const Sample
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   pdl_trigger();
   cl.barrier_arrive();                         // no CTA of the cluster is written to before it runs
-  if (tid < 32) s.exp2[tid] = make_uint2(c_exp2[tid], __float_as_uint((float)c_exp2[tid]));
+  if (tid < 32) s.exp2[tid] = c_exp2[tid];
   if (tid == 0) s.n_local = 0;
   for (int i = tid; i < SM_COARSE; i += SM_THREADS) s.cnt[i] = 0;
   pdl_wait();
@@ -499,11 +521,11 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_rows_kernel(const Sample
   }
   mean = __fdiv_rn(mean, n_mean);
   var = __fdiv_rn(var, n_mean) - mean * mean;
-  SampleWeight weight;
-  const double scale = 1.4426950408889634074 / (double)temp;
-  weight.m = m;
+  SampleWeight<sizeof(T) == 2> weight;
+  const double scale = fmin(32. * 1.4426950408889634074 / (double)temp, 1e30);     // beyond: the same weights, and 0 times it is 0
+  weight.m = fminf(m, FLT_MAX);
   weight.ch = (float)scale;
-  weight.cl = isinf(weight.ch) ? 0.f : (float)(scale - (double)weight.ch);
+  weight.cl = (float)(scale - (double)weight.ch);
   weight.table = s.exp2;
   auto finish = [&](long long token, float x, u64 total) {  // one thread of the row
     p.tokens[r] = token;
@@ -531,18 +553,31 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_rows_kernel(const Sample
     ++ex;
     return make_ulonglong2(all, below);
   };
-  // ---- (5) the first index at which the running sum of value(logit, index) reaches target(total): found(index, logit, total) in one thread
-  auto locate = [&](auto value, auto target, auto found) {
-    row.each([&](int st) {
-      float x[8];
-      row.values(st, x);
-      const int i = row.index(st);
+  // ---- (5) the first index at which the running sum of value(logit, index) reaches target(total): found(index, logit, total) in one thread.
+  // Logits below `floor_x` have none: steps whose maxima all are below it cost one comparison.
+  auto locate = [&](float floor_x, auto value, auto target, auto found) {
+    auto wanted = [&](int st) { return st < row.steps && __any_sync(0xffffffffu, row.maximum(st) >= floor_x); };
+    unsigned w[SampleRow<T, HELD>::WORDS];
+    bool now = wanted(0);
+    if (now) row.words(0, w);
+#pragma unroll 1
+    for (int st = 0; st < row.steps; ++st) {
       u64 v = 0;
+      if (now) {
+        float x[8];
+        row.unpack(w, x);
+        now = wanted(st + 1);
+        if (now) row.words(st + 1, w);         // the next ones on their way
+        const int i = row.index(st);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v += value(x[j], i + j);
-      v = sm_warp_sum(v);
+        for (int j = 0; j < 8; ++j) v += value(x[j], i + j);
+        v = sm_warp_sum(v);
+      } else {
+        now = wanted(st + 1);
+        if (now) row.words(st + 1, w);
+      }
       if (lane == 0) s.step[warp * p.steps + st] = v;
-    });
+    }
     for (int st = row.steps + lane; st < p.steps; st += 32) s.step[warp * p.steps + st] = 0;
     __syncthreads();
     // every warp over all of them: a run of entries per lane
@@ -790,25 +825,36 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_rows_kernel(const Sample
         if (!open) return;
       }
     }
-    if (!need_k) {
-      // ---- (3) down to half as far below the mean as the largest logit is above it
-      for (int i = tid; i < SM_BINS; i += SM_THREADS) s.lo[i] = s.hi[i] = 0;
-      __syncthreads();
-      bins(SM_BINS, 1.5f * (m - mean));
-      u64 w_here = 0;
-      row.each([&](int st) {
-        float x[8];
-        row.values(st, x);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const u64 w = weight(x[j]);
-          const int b = bin_of(x[j]);
-          if (b < SM_BINS - 1 && w > 0) sm_add(s, b, w);
-          w_here += w;
-        }
-      });
+    if (!need_k && open) {
+      // ---- (3) down to where a third of what p leaves out is expected below; where that misses the deciding value, as far below
+      // the mean as half of what the largest logit is above it
+      const float inv_t = __fdiv_rn(1.f, temp);
+      const float deep = m - (mean + var * inv_t + sqrtf(fmaxf(var, 0.f)) * normcdfinvf(fmaxf(1.f - top_p, 1e-6f) * 0.33f));
+      SampleSplit sp;
       unsigned in_bin;
-      const SampleSplit sp = sm_find(cl, s, s.group, s.slot[ex++][0], C, rank, false, true, block_sum(w_here), reach, false, &in_bin);
+      bool known = !flat;                      // the sum of all weights
+      for (int go = 0; go < 2; ++go) {
+        if (go > 0) cl.sync();                 // the others have read the bins
+        for (int i = tid; i < SM_BINS; i += SM_THREADS) s.lo[i] = s.hi[i] = 0;
+        __syncthreads();
+        bins(SM_BINS, go == 0 ? deep : 1.5f * (m - mean));
+        u64 w_here = 0;
+        row.each_values([&](int st, const float (&x)[8]) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int b = bin_of(x[j]);
+            if (b >= SM_BINS - 1 && known) continue;
+            const u64 w = weight(x[j]);
+            if (b < SM_BINS - 1) sm_add(s, b, w);
+            w_here += w;
+          }
+        });
+        const u64 target = target_p;
+        const bool fresh = !known;
+        sp = sm_find(cl, s, s.group, s.slot[ex++][0], C, rank, false, true, block_sum(w_here), [&](u64 all) { return fresh ? reach(all) : target; }, false, &in_bin);
+        known = true;
+        if (sp.bin < SM_BINS) break;
+      }
       if (sp.bin < SM_BINS) {
         room = SM_LIST / C;
         const int n = gather([&](float x, bool any) { return any ? bin_of(x) <= (int)sp.bin : bin_of(x) == (int)sp.bin; });
@@ -879,9 +925,7 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_rows_kernel(const Sample
           cl.sync();                           // the others have read the bins
           for (int i = tid; i < SM_BINS; i += SM_THREADS) s.cnt[i] = s.lo[i] = s.hi[i] = 0;
           __syncthreads();
-          row.each([&](int st) {
-            float x[8];
-            row.values(st, x);
+          row.each_values([&](int st, const float (&x)[8]) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
               const unsigned key = sm_key(x[j]);
@@ -893,7 +937,7 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_rows_kernel(const Sample
           });
           unsigned in_class;
           const u64 goal = target;
-          const SampleSplit d = sm_find(cl, s, s.part, s.slot[7][0], C, rank, true, by_weight, 0ull, [&](u64) { return goal; }, level == 0, &in_class);
+          const SampleSplit d = sm_find(cl, s, s.part, s.slot[9][0], C, rank, true, by_weight, 0ull, [&](u64) { return goal; }, level == 0, &in_class);
           prefix = prefix << bits | ((1u << bits) - 1 - d.bin);
           done += bits;
           target = d.target - (by_weight ? d.w : d.cnt);
@@ -924,7 +968,7 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_rows_kernel(const Sample
       }
       last_x = sm_value(key);
       if (n_take < n_class) {                  // some of the tokens with this logit: those of the lowest indices
-        locate([&](float x, int) { return x == last_x ? 1ull : 0ull; }, [&](u64) { return n_take; },
+        locate(last_x, [&](float x, int) { return x == last_x ? 1ull : 0ull; }, [&](u64) { return n_take; },
                [&](int i, float, u64) {
                  for (int q = 0; q < C; ++q) *cl.map_shared_rank(&s.last, q) = (u64)i;
                });
@@ -937,7 +981,9 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_rows_kernel(const Sample
     last_x = least;
     last_i = 0x7fffffff;
   }
-  locate([&](float x, int i) { return x > last_x || (x == last_x && i <= last_i) ? weight(x) : 0ull; }, [&](u64 total) { return sm_above(u, total); },
+  // behind last_i only logits above last_x: not less than the next normal number; none above infinity
+  const float next_x = last_x == INFINITY ? __int_as_float(0x7fffffff) : last_x == 0.f ? FLT_MIN : sm_value(sm_key(last_x) + 1);
+  locate(last_x, [&](float x, int i) { return weight(x >= (i <= last_i ? last_x : next_x) ? x : -INFINITY); }, [&](u64 total) { return sm_above(u, total); },
          [&](int i, float x, u64 total) { finish(i, x, total); });
 }
 
@@ -945,11 +991,16 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_rows_kernel(const Sample
 
 using namespace mlf;
 
-// CTAs per row, up to SM_CLUSTER: as many as a warp's steps need, and as many as there are SMs for, none with less than 4096 logits.
-// SMC_TABLE
+// CTAs per row: as many as a warp's steps need, none with less than 4096 logits; beyond that, more of them shorten the rows whose p keeps
+// most of a flat distribution, which take seven times as long as one with a small k, and cost every row their exchanges.
+// us at 128256 bf16 logits with 1 / 2 / 4 / 8 CTAs: 256 rows of k = 50 35 / 45 / 60 / 90, without limits 87 / 85 / 96 / 125, of all kinds
+// 215 / 139 / 132 / 153; 33 rows of 50257 fp32 logits, k = 50 23 / 20 / 16 / 21, of all kinds 75 / 50 / 40 / 32 (two CTAs fit an SM, but
+// clusters of eight only 32 times). So four CTAs for every SM, and clusters of eight where all run at once.
 static int sample_cluster(long long rows, int vocab) {
   int c = 1;
-  while (c < SM_CLUSTER && (vocab > c * SM_WARPS * SM_STEP * SM_STEPS || (rows * c * 2 <= sm_count() && vocab > c * 4096))) c *= 2;
+  while (c < SM_CLUSTER && (vocab > c * SM_WARPS * SM_STEP * SM_STEPS ||
+                            (vocab > c * 4096 && (2 * c < SM_CLUSTER ? rows * 2 * c <= 4 * sm_count() : rows * 2 * c * 4 <= 7 * sm_count()))))
+    c *= 2;
   return c;
 }
 

@@ -121,6 +121,20 @@ def test_ends_of_u_and_odd_numbers():
     assert native.sample_rows(zero, 3, u[1:2], t[:1] * 0).item() == 0
 
 
+@pytest.mark.parametrize("top", [float("inf"), 0.0, -1.1754944e-38, 3.3895314e38])
+def test_ties_at_odd_values(top):
+    """The lowest indices of equal logits at infinity, zero, the largest bf16 and minus the smallest normal number."""
+    x = torch.full((3, 5000), -5.0, device="cuda")
+    x[:, 100:4000] = top
+    if top == 0.0:
+        x[:, 200:300] = -0.0
+    u = torch.tensor([0.0, 0.5, 0.999], device="cuda")
+    k = torch.tensor([3000, 3000, 2], dtype=torch.int32, device="cuda")
+    t = torch.ones(3, device="cuda")
+    for dtype in (torch.float32, torch.bfloat16):
+        assert native.sample_rows(x.to(dtype), 5000, u, t, k).tolist() == [100, 1600, 101]
+
+
 def test_a_row_does_not_depend_on_the_others():
     """The same row alone (a cluster of CTAs), and in a batch of 600 (fewer CTAs for it)."""
     g = _gen(4)
