@@ -32,7 +32,7 @@ namespace mlf {
 constexpr int DQ_WARPS = 4;
 constexpr int DQ_THREADS = DQ_WARPS * 32;
 constexpr int DQ_TILE = 16;                                  // tokens
-constexpr int DQ_STAGES = 4;                                 // tiles in flight per warp
+constexpr int DQ_STAGES = 3;                                 // tiles in flight per warp
 constexpr int DQ_STAGE_BYTES = 2 * DQ_TILE * Q8_D + 128;     // keys, values, 16 + 16 scales
 constexpr int DQ_SMEM = DQ_WARPS * DQ_STAGES * DQ_STAGE_BYTES;
 constexpr float DQ_UP = 15.f;                                // log2 of the largest weight
@@ -47,7 +47,7 @@ struct DecodeQ8Params {
   const int* seq_lens;            // [B]
   __nv_bfloat16* out;             // [B, Hq, 128]
   float* ws;                      // [B, Hkv, splits, G, 130] (m, l, o[128]) when splits > 1
-  int B, Hq, Hkv, G, block_size, max_blocks, num_blocks, splits, unit;   // unit: tokens that a split is a multiple of
+  int B, Hq, Hkv, G, block_size, bs_shift, max_blocks, num_blocks, splits, unit;   // bs_shift: log2(block_size) or -1; unit: tokens that a split is a multiple of
   float scale_log2;
   int* err;
   // packed form: unrotated heads of packed QKV rows; the newest token goes to slots[b]
@@ -126,7 +126,8 @@ __device__ __forceinline__ unsigned q8_append_row(const DecodeQ8Params& p, float
 }
 
 // NT: tiles of eight query heads (the group's heads, zero-padded).
-template <int FMT, int NT, bool ROPE>
+// WHOLE: blocks of a multiple of 16 tokens, so that a tile lies in one.
+template <int FMT, int NT, bool ROPE, bool WHOLE>
 __global__ void __launch_bounds__(DQ_THREADS)
 paged_decode_q8_kernel(const DecodeQ8Params p) {
   extern __shared__ __align__(128) uint8_t dq_smem[];
@@ -169,30 +170,59 @@ paged_decode_q8_kernel(const DecodeQ8Params p) {
   // tiles that reach into the newest token's block wait until that token is written
   const int held_back = has_new ? (len - 1) / p.block_size * p.block_size : 0x7fffffff;
 
+  const long long row_bytes = (long long)p.Hkv * Q8_D;
+  auto block_of = [&](int t) { return p.bs_shift >= 0 ? t >> p.bs_shift : t / p.block_size; };
+  auto checked = [&](int page) {
+    if (page >= 0 && page < p.num_blocks) return page;
+    atomicCAS(p.err, 0, ERR_BAD_INDEX);
+    return 0;
+  };
+  // WHOLE: the blocks of 32 tiles of this warp, one a lane; where this lane's pieces lie in a tile
+  int pages = 0, pages_from = -1;
+  const long long k_at = (long long)hkv * Q8_D + g * row_bytes + c * 16, v_at = (long long)hkv * Q8_D + v_off + 2 * c * row_bytes + g * 16;
   auto issue = [&](int i) {                    // this warp's i-th tile
     const int t0 = t_lo + (warp + i * DQ_WARPS) * DQ_TILE;
     const uint32_t st = ring + (i % DQ_STAGES) * DQ_STAGE_BYTES;
+    if (WHOLE) {
+      if ((i & ~31) != pages_from) {
+        pages_from = i & ~31;
+        const int t = t_lo + (warp + (pages_from + lane) * DQ_WARPS) * DQ_TILE;
+        pages = t < t_hi ? checked(bt[block_of(t)]) : 0;
+      }
+      const int page = __shfl_sync(0xffffffffu, pages, i & 31), row0 = t0 - block_of(t0) * p.block_size, there = t_hi - t0;
+      const uint8_t* base = p.cache + page * blk_bytes + row0 * row_bytes;
+      if (lane < 2) dq_copy4(st + 2 * DQ_TILE * Q8_D + lane * 4, p.scale + ((long long)page * 2 + lane) * p.Hkv + hkv, 4);
+      // rows g and g + 8 of the keys, 16-byte columns c and c + 4; rows 2c, 2c + 1, 2c + 8, 2c + 9 of the values, column g
+      const uint8_t *k0 = base + k_at, *k1 = k0 + 8 * row_bytes, *v0 = base + v_at, *v1 = v0 + 8 * row_bytes;
+      const uint32_t to = st + lane * 16;
+      const int nk0 = g < there ? 16 : 0, nk1 = g + 8 < there ? 16 : 0;
+      dq_copy16(to, k0, nk0);
+      dq_copy16(to + 512, k0 + 64, nk0);
+      dq_copy16(to + 1024, k1, nk1);
+      dq_copy16(to + 1536, k1 + 64, nk1);
+      dq_copy16(to + 2048, v0, 2 * c < there ? 16 : 0);
+      dq_copy16(to + 2560, v0 + row_bytes, 2 * c + 1 < there ? 16 : 0);
+      dq_copy16(to + 3072, v1, 2 * c + 8 < there ? 16 : 0);
+      dq_copy16(to + 3584, v1 + row_bytes, 2 * c + 9 < there ? 16 : 0);
+      return;
+    }
     const int t = t0 + (lane & 15);
     const bool there = t < t_hi;
-    int page = (there ? t : t0) / p.block_size;
-    const int row = (there ? t : t0) - page * p.block_size;
-    page = bt[page];
-    if (page < 0 || page >= p.num_blocks) { atomicCAS(p.err, 0, ERR_BAD_INDEX); page = 0; }
-    const int at = there ? row : -1;
+    const int blk = block_of(there ? t : t0), at = there ? t - blk * p.block_size : -1;
+    const int page = checked(bt[blk]);
     dq_copy4(st + 2 * DQ_TILE * Q8_D + lane * 4, p.scale + ((long long)page * 2 + (lane >> 4)) * p.Hkv + hkv, there ? 4 : 0);
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {              // rows g and g + 8 of the keys, 16-byte columns c and c + 4
+    for (int j = 0; j < 2; ++j) {
       const int pg = __shfl_sync(0xffffffffu, page, g + 8 * j), r = __shfl_sync(0xffffffffu, at, g + 8 * j);
-      const uint8_t* src = p.cache + pg * blk_bytes + ((long long)max(r, 0) * p.Hkv + hkv) * Q8_D + c * 16;
+      const uint8_t* src = p.cache + pg * blk_bytes + max(r, 0) * row_bytes + hkv * Q8_D + c * 16;
       dq_copy16(st + (j * 2) * 512 + lane * 16, src, r >= 0 ? 16 : 0);
       dq_copy16(st + (j * 2 + 1) * 512 + lane * 16, src + 64, r >= 0 ? 16 : 0);
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {              // rows 2c, 2c + 1, 2c + 8, 2c + 9 of the values, column g
+    for (int j = 0; j < 4; ++j) {
       const int tr = 2 * c + (j & 1) + 8 * (j >> 1);
       const int pg = __shfl_sync(0xffffffffu, page, tr), r = __shfl_sync(0xffffffffu, at, tr);
-      dq_copy16(st + DQ_TILE * Q8_D + j * 512 + lane * 16, p.cache + pg * blk_bytes + v_off + ((long long)max(r, 0) * p.Hkv + hkv) * Q8_D + g * 16,
-                r >= 0 ? 16 : 0);
+      dq_copy16(st + DQ_TILE * Q8_D + j * 512 + lane * 16, p.cache + pg * blk_bytes + v_off + max(r, 0) * row_bytes + hkv * Q8_D + g * 16, r >= 0 ? 16 : 0);
     }
   };
   auto late = [&](int i) { return has_new && t_lo + (warp + i * DQ_WARPS) * DQ_TILE + DQ_TILE > held_back; };
@@ -282,13 +312,13 @@ paged_decode_q8_kernel(const DecodeQ8Params p) {
   }
 
   float o[NT][8][4];
-  float m_run[NT][2], l_run[NT][2];            // of heads 2c, 2c + 1 (l: this lane's tokens only)
+  float m_run[NT][2], m_use[NT][2], l_run[NT][2];   // of heads 2c, 2c + 1: maximum, what weights are relative to, sum (of this lane's tokens)
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
 #pragma unroll
     for (int mt = 0; mt < 8; ++mt) o[n][mt][0] = o[n][mt][1] = o[n][mt][2] = o[n][mt][3] = 0.f;
     m_run[n][0] = m_run[n][1] = -INFINITY;
-    l_run[n][0] = l_run[n][1] = 0.f;
+    m_use[n][0] = m_use[n][1] = l_run[n][0] = l_run[n][1] = 0.f;
   }
 
   for (int i = 0; i < mine; ++i) {
@@ -298,7 +328,7 @@ paged_decode_q8_kernel(const DecodeQ8Params p) {
     uint8_t* st = ring_p + (i % DQ_STAGES) * DQ_STAGE_BYTES;
     const int t0 = t_lo + (warp + i * DQ_WARPS) * DQ_TILE;
     const float* sc = reinterpret_cast<const float*>(st + 2 * DQ_TILE * Q8_D);
-    float ks0 = sc[g], ks1 = sc[g + 8], vs0 = sc[16 + g], vs1 = sc[16 + g + 8];
+    float ks0 = sc[WHOLE ? 0 : g], ks1 = sc[WHOLE ? 0 : g + 8], vs0 = sc[WHOLE ? 1 : 16 + g], vs1 = sc[WHOLE ? 1 : 16 + g + 8];
     if (ROPE && slot < 0 && has_new && len - 1 >= t0 && len - 1 < t0 + DQ_TILE) {   // a newest token that is nowhere in the cache
       const int r = len - 1 - t0;
       if ((r & 7) == g) {
@@ -315,7 +345,7 @@ paged_decode_q8_kernel(const DecodeQ8Params p) {
     // a block of zeros (or one that was never written) may have any scale: 2^-60 stands for what is smaller
     vs0 = fminf(fmaxf(vs0, 8.6736174e-19f), 1.1529215e18f);
     vs1 = fminf(fmaxf(vs1, 8.6736174e-19f), 1.1529215e18f);
-    const float lv0 = __log2f(vs0), lv1 = __log2f(vs1), iv0 = __frcp_rn(vs0), iv1 = __frcp_rn(vs1);
+    const float lv0 = __log2f(vs0), lv1 = __log2f(vs1), iv0 = __fdividef(1.f, vs0), iv1 = __fdividef(1.f, vs1);
     float s[NT][4];
 #pragma unroll
     for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
@@ -340,25 +370,32 @@ paged_decode_q8_kernel(const DecodeQ8Params p) {
       s[n][1] = in0 ? fmaf(s[n][1] * qf[n][1], ks0, lv0) : -INFINITY;
       s[n][2] = in1 ? fmaf(s[n][2] * qf[n][0], ks1, lv1) : -INFINITY;
       s[n][3] = in1 ? fmaf(s[n][3] * qf[n][1], ks1, lv1) : -INFINITY;
-      float alpha[2];
+      // a new maximum is met in few tiles: only then are the lanes asked for theirs and the sums brought to it
+      const float mx0 = fmaxf(s[n][0], s[n][2]), mx1 = fmaxf(s[n][1], s[n][3]);
+      if (__any_sync(0xffffffffu, mx0 > m_run[n][0] || mx1 > m_run[n][1])) {
+        float mx[2] = {mx0, mx1}, alpha[2];
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        float mx = fmaxf(s[n][e], s[n][2 + e]);
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-        const float m_new = fmaxf(m_run[n][e], mx);
-        const float m_use = m_new == -INFINITY ? 0.f : m_new - DQ_UP;
-        alpha[e] = exp2f(m_run[n][e] - DQ_UP - m_use);
-        m_run[n][e] = m_new;
-        s[n][e] = exp2f(s[n][e] - m_use);
-        s[n][2 + e] = exp2f(s[n][2 + e] - m_use);
-        l_run[n][e] = l_run[n][e] * alpha[e] + s[n][e] * iv0 + s[n][2 + e] * iv1;
+        for (int e = 0; e < 2; ++e) {
+          mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 4));
+          mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 8));
+          mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 16));
+          const float m_new = fmaxf(m_run[n][e], mx[e]);
+          m_use[n][e] = m_new == -INFINITY ? 0.f : m_new - DQ_UP;
+          alpha[e] = exp2f(m_run[n][e] - DQ_UP - m_use[n][e]);
+          m_run[n][e] = m_new;
+          l_run[n][e] *= alpha[e];
+        }
+#pragma unroll
+        for (int mt = 0; mt < 8; ++mt) {
+          o[n][mt][0] *= alpha[0]; o[n][mt][1] *= alpha[1];
+          o[n][mt][2] *= alpha[0]; o[n][mt][3] *= alpha[1];
+        }
       }
 #pragma unroll
-      for (int mt = 0; mt < 8; ++mt) {
-        o[n][mt][0] *= alpha[0]; o[n][mt][1] *= alpha[1];
-        o[n][mt][2] *= alpha[0]; o[n][mt][3] *= alpha[1];
+      for (int e = 0; e < 2; ++e) {
+        s[n][e] = exp2f(s[n][e] - m_use[n][e]);
+        s[n][2 + e] = exp2f(s[n][2 + e] - m_use[n][e]);
+        l_run[n][e] += s[n][e] * iv0 + s[n][2 + e] * iv1;
       }
       // rows are tokens here and columns in the next product
       pb[n][0] = dq_transpose(dq_half2(s[n][0], s[n][1]));
@@ -488,6 +525,8 @@ MLF_API int mlf_paged_decode_q8(const void* q, long long ldq, void* cache, float
   p.B = B; p.Hq = Hq; p.Hkv = Hkv; p.G = G; p.block_size = block_size; p.max_blocks = max_blocks; p.num_blocks = num_blocks;
   p.splits = splits;
   p.unit = block_size * ((DQ_WARPS * DQ_TILE + block_size - 1) / block_size);
+  p.bs_shift = -1;
+  for (int sh = 0; sh < 31; ++sh) if ((1 << sh) == block_size) p.bs_shift = sh;
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
   p.err = device_status_word();
   p.k_new = rope ? p.q + (long long)Hq * Q8_D : nullptr;
@@ -495,16 +534,17 @@ MLF_API int mlf_paged_decode_q8(const void* q, long long ldq, void* cache, float
   p.slots = slots;
   p.theta = theta;
   p.early = inputs_static;
-  void (*const kernels[2][2][2])(DecodeQ8Params) = {
-      {{paged_decode_q8_kernel<Q8_E4M3, 1, false>, paged_decode_q8_kernel<Q8_E4M3, 1, true>},
-       {paged_decode_q8_kernel<Q8_E4M3, 2, false>, paged_decode_q8_kernel<Q8_E4M3, 2, true>}},
-      {{paged_decode_q8_kernel<Q8_INT8, 1, false>, paged_decode_q8_kernel<Q8_INT8, 1, true>},
-       {paged_decode_q8_kernel<Q8_INT8, 2, false>, paged_decode_q8_kernel<Q8_INT8, 2, true>}}};
-  const auto kernel = kernels[fmt][G > 8 ? 1 : 0][rope ? 1 : 0];
-  static bool attr_set[64][8] = {};
+#define DQ_KERNELS(FMT, NT) \
+  {{paged_decode_q8_kernel<FMT, NT, false, false>, paged_decode_q8_kernel<FMT, NT, false, true>}, \
+   {paged_decode_q8_kernel<FMT, NT, true, false>, paged_decode_q8_kernel<FMT, NT, true, true>}}
+  void (*const kernels[2][2][2][2])(DecodeQ8Params) = {{DQ_KERNELS(Q8_E4M3, 1), DQ_KERNELS(Q8_E4M3, 2)}, {DQ_KERNELS(Q8_INT8, 1), DQ_KERNELS(Q8_INT8, 2)}};
+#undef DQ_KERNELS
+  const int nt = G > 8 ? 1 : 0, whole = block_size % DQ_TILE == 0 ? 1 : 0;
+  const auto kernel = kernels[fmt][nt][rope ? 1 : 0][whole];
+  static bool attr_set[64][16] = {};
   int dev = 0;
   cudaGetDevice(&dev);
-  bool& set = attr_set[dev & 63][fmt * 4 + (G > 8 ? 2 : 0) + (rope ? 1 : 0)];
+  bool& set = attr_set[dev & 63][fmt * 8 + nt * 4 + (rope ? 2 : 0) + whole];
   if (!set) {
     MLF_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, DQ_SMEM));
     set = true;
