@@ -17,8 +17,12 @@
 // The query is brought to f16 by a power of two per head that puts its largest element into [2^7, 2^8): exact for elements down
 // to 2^-22 of the largest, whose bf16 significands f16 holds whole.
 //
-// A warp takes every fourth tile of 16 tokens of its CTA's run and keeps a ring of them in flight with asynchronous 16-byte copies;
-// a lane reads back only what it copied itself, so no barrier stands in the loop.
+// A warp takes every fourth pair of tiles of its CTA's run and keeps two pairs in flight. Where a tile of 16 tokens lies in one block
+// (blocks of a multiple of 16), TMA fetches it, one box of 16 rows of 128 bytes for the keys and one for the values, and the
+// warp waits at a barrier of its own; asynchronous 16-byte copies by the lanes, which the other block sizes take, reached 5.0 TB/s
+// without any arithmetic and 4.4 with it where the boxes reach TMA_RATE. The box's rows are swizzled: the 16-byte column x of row r lies at
+// column x ^ (r & 7), so that a lane that takes columns 2 c and 2 c + 1 of key rows g and g + 8, and column g of four value
+// rows, shares no bank with the seven that read at the same time.
 #include <float.h>
 
 #include "../common/host.h"
@@ -32,9 +36,13 @@ namespace mlf {
 constexpr int DQ_WARPS = 4;
 constexpr int DQ_THREADS = DQ_WARPS * 32;
 constexpr int DQ_TILE = 16;                                  // tokens
-constexpr int DQ_STAGES = 3;                                 // tiles in flight per warp
-constexpr int DQ_STAGE_BYTES = 2 * DQ_TILE * Q8_D + 128;     // keys, values, 16 + 16 scales
+constexpr int DQ_PAIR = 2;                                   // tiles that a warp works on at once
+constexpr int DQ_STAGES = 2;                                 // pairs in flight per warp
+constexpr int DQ_TILE_BYTES = 2 * DQ_TILE * Q8_D + 128;      // keys, values, 16 + 16 scales
+constexpr int DQ_STAGE_BYTES = DQ_PAIR * DQ_TILE_BYTES;
 constexpr int DQ_SMEM = DQ_WARPS * DQ_STAGES * DQ_STAGE_BYTES;
+constexpr int DQ_BOX_STAGE = DQ_PAIR * 2 * DQ_TILE * Q8_D;   // of the TMA form: scales stay in registers
+constexpr int DQ_BOX_SMEM = DQ_WARPS * DQ_STAGES * DQ_BOX_STAGE + 1024;
 constexpr float DQ_UP = 15.f;                                // log2 of the largest weight
 constexpr int DQ_RED = Q8_D + 2;                             // floats of a partial result: maximum, sum, output
 
@@ -69,7 +77,7 @@ template <int N>
 __device__ __forceinline__ void dq_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 // D(16x8, fp32) += A(16x16, f16, row) B(16x8, f16, col)
 __device__ __forceinline__ void dq_mma(float (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ unsigned dq_transpose(unsigned a) {    // an 8 x 8 matrix of f16, a row's pair per lane
@@ -129,13 +137,25 @@ __device__ __forceinline__ unsigned q8_append_row(const DecodeQ8Params& p, float
 // WHOLE: blocks of a multiple of 16 tokens, so that a tile lies in one.
 template <int FMT, int NT, bool ROPE, bool WHOLE>
 __global__ void __launch_bounds__(DQ_THREADS)
-paged_decode_q8_kernel(const DecodeQ8Params p) {
-  extern __shared__ __align__(128) uint8_t dq_smem[];
+paged_decode_q8_kernel(const DecodeQ8Params p, const __grid_constant__ CUtensorMap tm) {
+  extern __shared__ __align__(128) uint8_t dq_raw[];
+  uint8_t* dq_smem = WHOLE ? dq_raw + (1024 - (smem_u32(dq_raw) & 1023)) % 1024 : dq_raw;      // swizzled boxes start on 1024 bytes
+  __shared__ __align__(8) uint64_t s_full[DQ_WARPS * DQ_STAGES];
+  __shared__ int s_abort;
   __shared__ __align__(16) uint8_t s_new[2][Q8_D];
   __shared__ float s_new_scale[2];
   __shared__ float2 s_cs[ROPE ? Q8_D / 2 : 1];
   const int b = blockIdx.x, hkv = blockIdx.y, sp = blockIdx.z;
   pdl_trigger();
+  if (WHOLE) {
+    if (threadIdx.x == 0) {
+      s_abort = 0;
+      tma_prefetch_desc(&tm);
+    }
+    if (threadIdx.x < DQ_WARPS * DQ_STAGES) mbar_init(smem_u32(&s_full[threadIdx.x]), 1);
+    mbar_fence_init();
+    __syncthreads();
+  }
   // Lengths, table and cached rows may be read ahead of the kernels before this one where those do not write them.
   const bool early = ROPE && p.early != 0;
   if (!early) pdl_wait();
@@ -162,10 +182,12 @@ paged_decode_q8_kernel(const DecodeQ8Params p) {
   }
   const int* bt = p.block_table + (long long)b * p.max_blocks;
   const long long v_off = (long long)p.block_size * p.Hkv * Q8_D, blk_bytes = 2 * v_off;
-  const int tiles = (t_hi - t_lo + DQ_TILE - 1) / DQ_TILE;
-  const int mine = tiles > warp ? (tiles - warp + DQ_WARPS - 1) / DQ_WARPS : 0;      // tiles warp, warp + 4, ...
-  const uint32_t ring = smem_u32(dq_smem) + warp * DQ_STAGES * DQ_STAGE_BYTES;
-  uint8_t* ring_p = dq_smem + warp * DQ_STAGES * DQ_STAGE_BYTES;
+  constexpr int SPAN = DQ_PAIR * DQ_TILE;
+  const int pairs = (t_hi - t_lo + SPAN - 1) / SPAN;
+  const int mine = pairs > warp ? (pairs - warp + DQ_WARPS - 1) / DQ_WARPS : 0;      // pairs of tiles warp, warp + 4, ...
+  constexpr int STAGE = WHOLE ? DQ_BOX_STAGE : DQ_STAGE_BYTES, TILE_BYTES = STAGE / DQ_PAIR;
+  uint8_t* ring_p = dq_smem + warp * DQ_STAGES * STAGE;
+  const uint32_t ring = smem_u32(ring_p), full = smem_u32(&s_full[warp * DQ_STAGES]);
   const bool has_new = ROPE && t_hi == len;
   // tiles that reach into the newest token's block wait until that token is written
   const int held_back = has_new ? (len - 1) / p.block_size * p.block_size : 0x7fffffff;
@@ -177,59 +199,73 @@ paged_decode_q8_kernel(const DecodeQ8Params p) {
     atomicCAS(p.err, 0, ERR_BAD_INDEX);
     return 0;
   };
-  // WHOLE: the blocks of 32 tiles of this warp, one a lane; where this lane's pieces lie in a tile
+  // WHOLE: the blocks of 16 pairs of tiles of this warp and their scales, a tile a lane; scales of the 16 pairs before stay in use for a while
   int pages = 0, pages_from = -1;
-  const long long k_at = (long long)hkv * Q8_D + g * row_bytes + c * 16, v_at = (long long)hkv * Q8_D + v_off + 2 * c * row_bytes + g * 16;
-  auto issue = [&](int i) {                    // this warp's i-th tile
-    const int t0 = t_lo + (warp + i * DQ_WARPS) * DQ_TILE;
-    const uint32_t st = ring + (i % DQ_STAGES) * DQ_STAGE_BYTES;
+  float scales[2][2];
+  scales[0][0] = scales[0][1] = scales[1][0] = scales[1][1] = 1.f;
+  auto issue = [&](int i) {                    // this warp's i-th pair
+    const int first = t_lo + (warp + i * DQ_WARPS) * SPAN;
+    const uint32_t st = ring + (i % DQ_STAGES) * STAGE;
     if (WHOLE) {
-      if ((i & ~31) != pages_from) {
-        pages_from = i & ~31;
-        const int t = t_lo + (warp + (pages_from + lane) * DQ_WARPS) * DQ_TILE;
+      if ((i & ~15) != pages_from) {
+        pages_from = i & ~15;
+        const int t = t_lo + (warp + (pages_from + (lane >> 1)) * DQ_WARPS) * SPAN + (lane & 1) * DQ_TILE;
         pages = t < t_hi ? checked(bt[block_of(t)]) : 0;
+        const float* sc = p.scale + (long long)pages * 2 * p.Hkv + hkv;
+        const float sk = t < t_hi ? sc[0] : 1.f, sv = t < t_hi ? sc[p.Hkv] : 1.f;
+        if ((i >> 4) & 1) { scales[1][0] = sk; scales[1][1] = sv; }
+        else { scales[0][0] = sk; scales[0][1] = sv; }
       }
-      const int page = __shfl_sync(0xffffffffu, pages, i & 31), row0 = t0 - block_of(t0) * p.block_size, there = t_hi - t0;
-      const uint8_t* base = p.cache + page * blk_bytes + row0 * row_bytes;
-      if (lane < 2) dq_copy4(st + 2 * DQ_TILE * Q8_D + lane * 4, p.scale + ((long long)page * 2 + lane) * p.Hkv + hkv, 4);
-      // rows g and g + 8 of the keys, 16-byte columns c and c + 4; rows 2c, 2c + 1, 2c + 8, 2c + 9 of the values, column g
-      const uint8_t *k0 = base + k_at, *k1 = k0 + 8 * row_bytes, *v0 = base + v_at, *v1 = v0 + 8 * row_bytes;
-      const uint32_t to = st + lane * 16;
-      const int nk0 = g < there ? 16 : 0, nk1 = g + 8 < there ? 16 : 0;
-      dq_copy16(to, k0, nk0);
-      dq_copy16(to + 512, k0 + 64, nk0);
-      dq_copy16(to + 1024, k1, nk1);
-      dq_copy16(to + 1536, k1 + 64, nk1);
-      dq_copy16(to + 2048, v0, 2 * c < there ? 16 : 0);
-      dq_copy16(to + 2560, v0 + row_bytes, 2 * c + 1 < there ? 16 : 0);
-      dq_copy16(to + 3072, v1, 2 * c + 8 < there ? 16 : 0);
-      dq_copy16(to + 3584, v1 + row_bytes, 2 * c + 9 < there ? 16 : 0);
+      const int page0 = __shfl_sync(0xffffffffu, pages, 2 * (i & 15)), page1 = __shfl_sync(0xffffffffu, pages, 2 * (i & 15) + 1);
+      if (elect_one()) {
+        const uint32_t bar = full + 8 * (i % DQ_STAGES);
+        const bool two = first + DQ_TILE < t_hi;
+        mbar_expect_tx(bar, two ? STAGE : TILE_BYTES);
+#pragma unroll
+        for (int h = 0; h < DQ_PAIR; ++h) {
+          if (h == 1 && !two) break;
+          const int t0 = first + h * DQ_TILE, row = (h ? page1 : page0) * 2 * p.block_size + t0 - block_of(t0) * p.block_size;
+          tma_load_2d(st + h * TILE_BYTES, &tm, hkv * Q8_D, row, bar);
+          tma_load_2d(st + h * TILE_BYTES + DQ_TILE * Q8_D, &tm, hkv * Q8_D, row + p.block_size, bar);
+        }
+      }
       return;
     }
-    const int t = t0 + (lane & 15);
-    const bool there = t < t_hi;
-    const int blk = block_of(there ? t : t0), at = there ? t - blk * p.block_size : -1;
-    const int page = checked(bt[blk]);
-    dq_copy4(st + 2 * DQ_TILE * Q8_D + lane * 4, p.scale + ((long long)page * 2 + (lane >> 4)) * p.Hkv + hkv, there ? 4 : 0);
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int pg = __shfl_sync(0xffffffffu, page, g + 8 * j), r = __shfl_sync(0xffffffffu, at, g + 8 * j);
-      const uint8_t* src = p.cache + pg * blk_bytes + max(r, 0) * row_bytes + hkv * Q8_D + c * 16;
-      dq_copy16(st + (j * 2) * 512 + lane * 16, src, r >= 0 ? 16 : 0);
-      dq_copy16(st + (j * 2 + 1) * 512 + lane * 16, src + 64, r >= 0 ? 16 : 0);
-    }
+    for (int h = 0; h < DQ_PAIR; ++h) {
+      const uint32_t to = st + h * TILE_BYTES;
+      const int t = first + h * DQ_TILE + (lane & 15), tt = t < t_hi ? t : t_lo;
+      const int blk = block_of(tt), at = t < t_hi ? t - blk * p.block_size : -1;
+      const int page = checked(bt[blk]);
+      dq_copy4(to + 2 * DQ_TILE * Q8_D + lane * 4, p.scale + ((long long)page * 2 + (lane >> 4)) * p.Hkv + hkv, at >= 0 ? 4 : 0);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int tr = 2 * c + (j & 1) + 8 * (j >> 1);
-      const int pg = __shfl_sync(0xffffffffu, page, tr), r = __shfl_sync(0xffffffffu, at, tr);
-      dq_copy16(st + DQ_TILE * Q8_D + j * 512 + lane * 16, p.cache + pg * blk_bytes + v_off + max(r, 0) * row_bytes + hkv * Q8_D + g * 16, r >= 0 ? 16 : 0);
+      for (int j = 0; j < 2; ++j) {            // rows g and g + 8 of the keys, 16-byte columns 2c and 2c + 1
+        const int pg = __shfl_sync(0xffffffffu, page, g + 8 * j), r = __shfl_sync(0xffffffffu, at, g + 8 * j);
+        const uint8_t* src = p.cache + pg * blk_bytes + max(r, 0) * row_bytes + hkv * Q8_D + c * 32;
+        dq_copy16(to + (j * 2) * 512 + lane * 16, src, r >= 0 ? 16 : 0);
+        dq_copy16(to + (j * 2 + 1) * 512 + lane * 16, src + 16, r >= 0 ? 16 : 0);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {            // rows 2c, 2c + 1, 2c + 8, 2c + 9 of the values, column g
+        const int tr = 2 * c + (j & 1) + 8 * (j >> 1);
+        const int pg = __shfl_sync(0xffffffffu, page, tr), r = __shfl_sync(0xffffffffu, at, tr);
+        dq_copy16(to + DQ_TILE * Q8_D + j * 512 + lane * 16, p.cache + pg * blk_bytes + v_off + max(r, 0) * row_bytes + hkv * Q8_D + g * 16, r >= 0 ? 16 : 0);
+      }
     }
   };
-  auto late = [&](int i) { return has_new && t_lo + (warp + i * DQ_WARPS) * DQ_TILE + DQ_TILE > held_back; };
+  // where this lane's 16 bytes lie in a tile: keys, half 0 / 1 of its columns in row g + 8 j; values, the j-th of its rows
+  auto key_at = [&](int half, int j) {
+    return WHOLE ? (g + 8 * j) * Q8_D + (((2 * c + half) ^ g) << 4) : (2 * j + half) * 512 + lane * 16;
+  };
+  auto value_at = [&](int j) {
+    const int row = 2 * c + (j & 1) + 8 * (j >> 1);
+    return DQ_TILE * Q8_D + (WHOLE ? row * Q8_D + ((g ^ (row & 7)) << 4) : j * 512 + lane * 16);
+  };
+  auto late = [&](int i) { return has_new && t_lo + (warp + i * DQ_WARPS) * SPAN + SPAN > held_back; };
 #pragma unroll
   for (int i = 0; i < DQ_STAGES; ++i) {
     if (i < mine && !late(i)) issue(i);
-    dq_commit();
+    if (!WHOLE) dq_commit();
   }
   if (ROPE) {
     if (tid < Q8_D / 2) s_cs[tid] = rope_cos_sin((float)(len - 1), __logf(p.theta), rope_exponent<Q8_D>(tid));
@@ -257,13 +293,14 @@ paged_decode_q8_kernel(const DecodeQ8Params p) {
       const unsigned w = q8_append_row<FMT>(p, x, hkv, warp, slot, now);
       *reinterpret_cast<unsigned*>(&s_new[warp][lane * 4]) = w;
       if (lane == 0) s_new_scale[warp] = now;
-      __threadfence();                         // the copies below read past the L1
+      __threadfence();                         // the copies below read past the L1, or through TMA
+      if (WHOLE) fence_proxy_async_all();
     }
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < DQ_STAGES; ++i)
       if (i < mine && late(i)) issue(i);
-    dq_commit();
+    if (!WHOLE) dq_commit();
   }
 
   // Q^T as the B operand: head n = g of each tile of eight, the 32 elements that this lane's pieces of a key row hold
@@ -280,7 +317,7 @@ paged_decode_q8_kernel(const DecodeQ8Params p) {
         // rows are 4-byte aligned at least
         float2 a = make_float2(0.f, 0.f), e = a;
         if (head < p.G) {
-          const uint32_t* src = reinterpret_cast<const uint32_t*>(p.q + (long long)b * p.ldq + (long long)(hkv * p.G + head) * Q8_D + h * 64 + c * 16 + j * 4);
+          const uint32_t* src = reinterpret_cast<const uint32_t*>(p.q + (long long)b * p.ldq + (long long)(hkv * p.G + head) * Q8_D + c * 32 + h * 16 + j * 4);
           a = unpack_bf16x2(src[0]);
           e = unpack_bf16x2(src[1]);
         }
@@ -288,10 +325,11 @@ paged_decode_q8_kernel(const DecodeQ8Params p) {
       }
     if (ROPE) {
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        rope_rotate(x[j], x[16 + j], s_cs[c * 16 + j]);
-        x[j] = __bfloat162float(__float2bfloat16(x[j]));
-        x[16 + j] = __bfloat162float(__float2bfloat16(x[16 + j]));
+      for (int j = 0; j < 32; ++j) {           // the pair of column 32 c + j is 64 further, two lanes of the four on
+        const float other = __shfl_xor_sync(0xffffffffu, x[j], 2);
+        float lo = c < 2 ? x[j] : other, hi = c < 2 ? other : x[j];
+        rope_rotate(lo, hi, s_cs[(c & 1) * 32 + j]);
+        x[j] = __bfloat162float(__float2bfloat16(c < 2 ? lo : hi));
       }
     }
     float amax = 0.f;
@@ -322,58 +360,91 @@ paged_decode_q8_kernel(const DecodeQ8Params p) {
   }
 
   for (int i = 0; i < mine; ++i) {
-    if (has_new && late(i)) dq_wait<0>();      // its group is not the i-th one
-    else dq_wait<DQ_STAGES - 1>();
-    __syncwarp();                              // the scales are other lanes' copies
-    uint8_t* st = ring_p + (i % DQ_STAGES) * DQ_STAGE_BYTES;
-    const int t0 = t_lo + (warp + i * DQ_WARPS) * DQ_TILE;
-    const float* sc = reinterpret_cast<const float*>(st + 2 * DQ_TILE * Q8_D);
-    float ks0 = sc[WHOLE ? 0 : g], ks1 = sc[WHOLE ? 0 : g + 8], vs0 = sc[WHOLE ? 1 : 16 + g], vs1 = sc[WHOLE ? 1 : 16 + g + 8];
-    if (ROPE && slot < 0 && has_new && len - 1 >= t0 && len - 1 < t0 + DQ_TILE) {   // a newest token that is nowhere in the cache
-      const int r = len - 1 - t0;
-      if ((r & 7) == g) {
-        uint8_t* kd = st + (r >> 3) * 1024 + lane * 16;
-        *reinterpret_cast<uint4*>(kd) = *reinterpret_cast<const uint4*>(&s_new[0][c * 16]);
-        *reinterpret_cast<uint4*>(kd + 512) = *reinterpret_cast<const uint4*>(&s_new[0][64 + c * 16]);
-        if (r < 8) { ks0 = s_new_scale[0]; vs0 = s_new_scale[1]; }
-        else { ks1 = s_new_scale[0]; vs1 = s_new_scale[1]; }
-      }
-      if (((r & 7) >> 1) == c)
-        *reinterpret_cast<uint4*>(st + DQ_TILE * Q8_D + ((r & 1) + 2 * (r >> 3)) * 512 + lane * 16) = *reinterpret_cast<const uint4*>(&s_new[1][g * 16]);
+    if (WHOLE) {
+      if (!mbar_wait_warp(full + 8 * (i % DQ_STAGES), (i / DQ_STAGES) & 1, &s_abort, p.err, ERR_WAIT_ATTN)) break;
+    } else {
+      if (has_new && late(i)) dq_wait<0>();    // its group is not the i-th one
+      else dq_wait<DQ_STAGES - 1>();
+      __syncwarp();                            // the scales are other lanes' copies
     }
-    const bool in0 = t0 + g < t_hi, in1 = t0 + g + 8 < t_hi;
-    // a block of zeros (or one that was never written) may have any scale: 2^-60 stands for what is smaller
-    vs0 = fminf(fmaxf(vs0, 8.6736174e-19f), 1.1529215e18f);
-    vs1 = fminf(fmaxf(vs1, 8.6736174e-19f), 1.1529215e18f);
-    const float lv0 = __log2f(vs0), lv1 = __log2f(vs1), iv0 = __fdividef(1.f, vs0), iv1 = __fdividef(1.f, vs1);
-    float s[NT][4];
+    uint8_t* stage = ring_p + (i % DQ_STAGES) * STAGE;
+    // two tiles side by side: the products of one hide the latencies of the other's
+    float s[DQ_PAIR][NT][4], iv[DQ_PAIR][2];
+    float ks[DQ_PAIR][2], lv[DQ_PAIR][2];
+    bool in[DQ_PAIR][2];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {              // 64 of the key's 128 columns
-      const uint4 a = *reinterpret_cast<const uint4*>(st + h * 512 + lane * 16), e = *reinterpret_cast<const uint4*>(st + (2 + h) * 512 + lane * 16);
-      const unsigned aw[4] = {a.x, a.y, a.z, a.w}, ew[4] = {e.x, e.y, e.z, e.w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        unsigned a0, a2, a1, a3;
-        q8_unpack4<FMT>(aw[j], a0, a2);
-        q8_unpack4<FMT>(ew[j], a1, a3);
-#pragma unroll
-        for (int n = 0; n < NT; ++n) dq_mma(s[n], a0, a1, a2, a3, qb[n][h * 4 + j][0], qb[n][h * 4 + j][1]);
+    for (int h = 0; h < DQ_PAIR; ++h) {
+      uint8_t* st = stage + h * TILE_BYTES;
+      const int t0 = t_lo + (warp + i * DQ_WARPS) * SPAN + h * DQ_TILE;
+      float vs[2];
+      if (WHOLE) {
+        const bool odd = (i >> 4) & 1;
+        ks[h][0] = __shfl_sync(0xffffffffu, odd ? scales[1][0] : scales[0][0], 2 * (i & 15) + h);
+        vs[0] = __shfl_sync(0xffffffffu, odd ? scales[1][1] : scales[0][1], 2 * (i & 15) + h);
+        if (has_new && late(i) && t0 < t_hi) {                 // as the newest token left them
+          const float* sc = p.scale + (long long)checked(bt[block_of(t0)]) * 2 * p.Hkv + hkv;
+          ks[h][0] = sc[0];
+          vs[0] = sc[p.Hkv];
+        }
+        ks[h][1] = ks[h][0];
+        vs[1] = vs[0];
+      } else {
+        const float* sc = reinterpret_cast<const float*>(st + 2 * DQ_TILE * Q8_D);
+        ks[h][0] = sc[g]; ks[h][1] = sc[g + 8];
+        vs[0] = sc[16 + g]; vs[1] = sc[16 + g + 8];
       }
+      if (ROPE && slot < 0 && has_new && len - 1 >= t0 && len - 1 < t0 + DQ_TILE) {   // a newest token that is nowhere in the cache
+        const int r = len - 1 - t0;
+        if ((r & 7) == g) {
+          *reinterpret_cast<uint4*>(st + key_at(0, r >> 3)) = *reinterpret_cast<const uint4*>(&s_new[0][c * 32]);
+          *reinterpret_cast<uint4*>(st + key_at(1, r >> 3)) = *reinterpret_cast<const uint4*>(&s_new[0][c * 32 + 16]);
+          if (r < 8) { ks[h][0] = s_new_scale[0]; vs[0] = s_new_scale[1]; }
+          else { ks[h][1] = s_new_scale[0]; vs[1] = s_new_scale[1]; }
+        }
+        if (((r & 7) >> 1) == c) *reinterpret_cast<uint4*>(st + value_at((r & 1) + 2 * (r >> 3))) = *reinterpret_cast<const uint4*>(&s_new[1][g * 16]);
+        if (WHOLE) fence_proxy_async_smem();   // before the next box lands here
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        in[h][e] = t0 + g + 8 * e < t_hi;
+        // a block of zeros (or one that was never written) may have any scale: 2^-60 stands for what is smaller
+        vs[e] = fminf(fmaxf(vs[e], 8.6736174e-19f), 1.1529215e18f);
+        lv[h][e] = __log2f(vs[e]);
+        iv[h][e] = __fdividef(1.f, vs[e]);
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n) s[h][n][0] = s[h][n][1] = s[h][n][2] = s[h][n][3] = 0.f;
     }
-    unsigned pb[NT][2];
+#pragma unroll
+    for (int half = 0; half < 2; ++half)       // 64 of the key's 128 columns
+#pragma unroll
+      for (int h = 0; h < DQ_PAIR; ++h) {
+        const uint8_t* st = stage + h * TILE_BYTES;
+        const uint4 a = *reinterpret_cast<const uint4*>(st + key_at(half, 0)), e = *reinterpret_cast<const uint4*>(st + key_at(half, 1));
+        const unsigned aw[4] = {a.x, a.y, a.z, a.w}, ew[4] = {e.x, e.y, e.z, e.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          unsigned a0, a2, a1, a3;
+          q8_unpack4<FMT>(aw[j], a0, a2);
+          q8_unpack4<FMT>(ew[j], a1, a3);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) dq_mma(s[h][n], a0, a1, a2, a3, qb[n][half * 4 + j][0], qb[n][half * 4 + j][1]);
+        }
+      }
+    unsigned pb[DQ_PAIR][NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      // s: tokens g (0, 1) and g + 8 (2, 3), heads 2c and 2c + 1
-      s[n][0] = in0 ? fmaf(s[n][0] * qf[n][0], ks0, lv0) : -INFINITY;
-      s[n][1] = in0 ? fmaf(s[n][1] * qf[n][1], ks0, lv0) : -INFINITY;
-      s[n][2] = in1 ? fmaf(s[n][2] * qf[n][0], ks1, lv1) : -INFINITY;
-      s[n][3] = in1 ? fmaf(s[n][3] * qf[n][1], ks1, lv1) : -INFINITY;
+      float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+      for (int h = 0; h < DQ_PAIR; ++h)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {          // tokens g (0, 1) and g + 8 (2, 3), heads 2c and 2c + 1
+          s[h][n][e] = in[h][e >> 1] ? fmaf(s[h][n][e] * qf[n][e & 1], ks[h][e >> 1], lv[h][e >> 1]) : -INFINITY;
+          mx[e & 1] = fmaxf(mx[e & 1], s[h][n][e]);
+        }
       // a new maximum is met in few tiles: only then are the lanes asked for theirs and the sums brought to it
-      const float mx0 = fmaxf(s[n][0], s[n][2]), mx1 = fmaxf(s[n][1], s[n][3]);
-      if (__any_sync(0xffffffffu, mx0 > m_run[n][0] || mx1 > m_run[n][1])) {
-        float mx[2] = {mx0, mx1}, alpha[2];
+      if (__any_sync(0xffffffffu, mx[0] > m_run[n][0] || mx[1] > m_run[n][1])) {
+        float alpha[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 4));
@@ -392,35 +463,47 @@ paged_decode_q8_kernel(const DecodeQ8Params p) {
         }
       }
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        s[n][e] = exp2f(s[n][e] - m_use[n][e]);
-        s[n][2 + e] = exp2f(s[n][2 + e] - m_use[n][e]);
-        l_run[n][e] += s[n][e] * iv0 + s[n][2 + e] * iv1;
-      }
-      // rows are tokens here and columns in the next product
-      pb[n][0] = dq_transpose(dq_half2(s[n][0], s[n][1]));
-      pb[n][1] = dq_transpose(dq_half2(s[n][2], s[n][3]));
-    }
-    uint4 v[4];
+      for (int h = 0; h < DQ_PAIR; ++h) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const uint4*>(st + DQ_TILE * Q8_D + j * 512 + lane * 16);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {              // rows 16 g + 4 j .. + 3 of O^T
-      const unsigned t0w = (&v[0].x)[j], t1w = (&v[1].x)[j], t8w = (&v[2].x)[j], t9w = (&v[3].x)[j];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {            // two tokens' bytes side by side: rows 4 j + 2 h, 4 j + 2 h + 1
-        unsigned a0, a1, a2, a3;
-        q8_unpack4<FMT>(__byte_perm(t0w, t1w, h ? 0x7362 : 0x5140), a0, a1);
-        q8_unpack4<FMT>(__byte_perm(t8w, t9w, h ? 0x7362 : 0x5140), a2, a3);
-#pragma unroll
-        for (int n = 0; n < NT; ++n) dq_mma(o[n][j * 2 + h], a0, a1, a2, a3, pb[n][0], pb[n][1]);
+        for (int e = 0; e < 4; ++e) {
+          s[h][n][e] = exp2f(s[h][n][e] - m_use[n][e & 1]);
+          l_run[n][e & 1] += s[h][n][e] * iv[h][e >> 1];
+        }
+        // rows are tokens here and columns in the next product
+        pb[h][n][0] = dq_transpose(dq_half2(s[h][n][0], s[h][n][1]));
+        pb[h][n][1] = dq_transpose(dq_half2(s[h][n][2], s[h][n][3]));
       }
     }
-    __syncwarp();                              // the scales of this stage have been read
+#pragma unroll
+    for (int h = 0; h < DQ_PAIR; ++h) {
+      const uint8_t* st = stage + h * TILE_BYTES;
+      uint4 v[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const uint4*>(st + value_at(j));
+      const int left = t_hi - (t_lo + (warp + i * DQ_WARPS) * SPAN + h * DQ_TILE);
+      if (WHOLE && left < DQ_TILE) {           // rows behind the sequence hold anything, and 0 times a NaN is one
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (2 * c + (j & 1) + 8 * (j >> 1) >= left) v[j] = make_uint4(0u, 0u, 0u, 0u);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {            // rows 16 g + 4 j .. + 3 of O^T
+        const unsigned t0w = (&v[0].x)[j], t1w = (&v[1].x)[j], t8w = (&v[2].x)[j], t9w = (&v[3].x)[j];
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {          // two tokens' bytes side by side: rows 4 j + 2 q, 4 j + 2 q + 1
+          unsigned a0, a1, a2, a3;
+          q8_unpack4<FMT>(__byte_perm(t0w, t1w, q ? 0x7362 : 0x5140), a0, a1);
+          q8_unpack4<FMT>(__byte_perm(t8w, t9w, q ? 0x7362 : 0x5140), a2, a3);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) dq_mma(o[n][j * 2 + q], a0, a1, a2, a3, pb[h][n][0], pb[h][n][1]);
+        }
+      }
+    }
+    __syncwarp();                              // this stage has been read
     if (i + DQ_STAGES < mine) issue(i + DQ_STAGES);
-    dq_commit();
+    if (!WHOLE) dq_commit();
   }
-  dq_wait<0>();
+  if (!WHOLE) dq_wait<0>();
   __syncthreads();                             // the rings are free
   // ---- merge the four warps: red[warp][head][m, l, o[128]]
   float* red = reinterpret_cast<float*>(dq_smem);
@@ -537,20 +620,27 @@ MLF_API int mlf_paged_decode_q8(const void* q, long long ldq, void* cache, float
 #define DQ_KERNELS(FMT, NT) \
   {{paged_decode_q8_kernel<FMT, NT, false, false>, paged_decode_q8_kernel<FMT, NT, false, true>}, \
    {paged_decode_q8_kernel<FMT, NT, true, false>, paged_decode_q8_kernel<FMT, NT, true, true>}}
-  void (*const kernels[2][2][2][2])(DecodeQ8Params) = {{DQ_KERNELS(Q8_E4M3, 1), DQ_KERNELS(Q8_E4M3, 2)}, {DQ_KERNELS(Q8_INT8, 1), DQ_KERNELS(Q8_INT8, 2)}};
+  void (*const kernels[2][2][2][2])(DecodeQ8Params, CUtensorMap) = {{DQ_KERNELS(Q8_E4M3, 1), DQ_KERNELS(Q8_E4M3, 2)}, {DQ_KERNELS(Q8_INT8, 1), DQ_KERNELS(Q8_INT8, 2)}};
 #undef DQ_KERNELS
-  const int nt = G > 8 ? 1 : 0, whole = block_size % DQ_TILE == 0 ? 1 : 0;
+  const long long cache_rows = 2LL * num_blocks * block_size;
+  const int nt = G > 8 ? 1 : 0, whole = block_size % DQ_TILE == 0 && cache_rows < (1LL << 31) ? 1 : 0;
+  const int smem = whole ? DQ_BOX_SMEM : DQ_SMEM;
+  CUtensorMap tm = {};
+  if (whole) {
+    const int rc = make_tmap_2d(&tm, cache, 1, (uint64_t)Hkv * Q8_D, (uint64_t)cache_rows, (uint64_t)Hkv * Q8_D, Q8_D, DQ_TILE, true);
+    if (rc) return rc;
+  }
   const auto kernel = kernels[fmt][nt][rope ? 1 : 0][whole];
   static bool attr_set[64][16] = {};
   int dev = 0;
   cudaGetDevice(&dev);
   bool& set = attr_set[dev & 63][fmt * 8 + nt * 4 + (rope ? 2 : 0) + whole];
   if (!set) {
-    MLF_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, DQ_SMEM));
+    MLF_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     set = true;
   }
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  MLF_CHECK_CUDA(launch_pdl(kernel, dim3(B, Hkv, splits), dim3(DQ_THREADS), DQ_SMEM, st, p));
+  MLF_CHECK_CUDA(launch_pdl(kernel, dim3(B, Hkv, splits), dim3(DQ_THREADS), smem, st, p, tm));
   count_launch();
   if (splits > 1) {
     MLF_CHECK_CUDA(launch_pdl(paged_decode_q8_merge_kernel, dim3((unsigned)(B * Hq)), dim3(Q8_D), 0, st, (const float*)ws, p.out, Hq, Hkv, G, splits));
