@@ -550,40 +550,64 @@ paged_decode_q8_kernel(const DecodeQ8Params p, const __grid_constant__ CUtensorM
   }
 }
 
-// out = sum_s exp2(m_s - M) o_s / sum_s exp2(m_s - M) l_s over the splits of a sequence and head
+// out = sum_s exp2(m_s - M) o_s / sum_s exp2(m_s - M) l_s over the splits of a sequence and head. The splits' factors first, one a
+// thread, so that the loop over their outputs has nothing but loads in it, eight at a time.
 __global__ void __launch_bounds__(Q8_D)
 paged_decode_q8_merge_kernel(const float* ws, __nv_bfloat16* out, int Hq, int Hkv, int G, int splits) {
+  __shared__ float s_f[Q8_D], s_max[Q8_D / 32], s_sum[Q8_D / 32];
   pdl_trigger();
   pdl_wait();
   const int b = blockIdx.x / Hq, h = blockIdx.x % Hq, d = threadIdx.x;
   const float* base = ws + (((long long)b * Hkv + h / G) * splits * G + h % G) * DQ_RED;
   const long long sstride = (long long)G * DQ_RED;
-  float M = -INFINITY;
-  for (int s = 0; s < splits; ++s) M = fmaxf(M, base[s * sstride]);
-  float L = 0.f, o = 0.f;
-  for (int s = 0; s < splits; ++s) {
-    const float m = base[s * sstride];
-    if (m == -INFINITY) continue;
-    const float w = exp2f(m - M);
-    L += w * base[s * sstride + 1];
-    o += w * base[s * sstride + 2 + d];
+  float M = -INFINITY, L = 0.f, o = 0.f;       // relative to the maximum so far
+  for (int s0 = 0; s0 < splits; s0 += Q8_D) {
+    const int n = min(Q8_D, splits - s0);
+    const float m = d < n ? base[(s0 + d) * sstride] : -INFINITY, l = d < n ? base[(s0 + d) * sstride + 1] : 0.f;
+    float mx = m;
+#pragma unroll
+    for (int k = 16; k > 0; k >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, k));
+    __syncthreads();
+    if ((d & 31) == 0) s_max[d >> 5] = mx;
+    __syncthreads();
+    const float M_new = fmaxf(fmaxf(M, fmaxf(s_max[0], s_max[1])), fmaxf(s_max[2], s_max[3]));
+    const float M_use = M_new == -INFINITY ? 0.f : M_new, back = exp2f(M - M_use), f = exp2f(m - M_use);
+    float sum = f * l;
+#pragma unroll
+    for (int k = 16; k > 0; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
+    if ((d & 31) == 0) s_sum[d >> 5] = sum;
+    s_f[d] = f;
+    __syncthreads();
+    L = L * back + (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
+    o *= back;
+    M = M_new;
+    const float* at = base + s0 * sstride + 2 + d;
+    int s = 0;
+    for (; s + 8 <= n; s += 8) {
+      float x[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) x[k] = at[(s + k) * sstride];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) o += s_f[s + k] * x[k];
+    }
+    for (; s < n; ++s) o += s_f[s] * at[s * sstride];
   }
   out[(long long)blockIdx.x * Q8_D + d] = __float2bfloat16(L > 0.f ? o / L : 0.f);
 }
+static_assert(Q8_D == 128, "four warps");
 
 }  // namespace mlf
 
 using namespace mlf;
 
-MLF_API long long mlf_paged_decode_q8_ws_elems(int B, int Hq, int splits) { return (long long)B * Hq * splits * DQ_RED; }
-
 // One query token per sequence over an 8-bit cache. Without slots: q [B, Hq, 128], row pitch ldq. With slots (the packed form): q is
 // the QKV product [B, (Hq + 2 Hkv) * 128], not yet rotated; the newest token of a sequence, the last of its seq_lens, is rotated at
 // position seq_lens - 1, written to its slot (< 0: not written) as mlf_kv_write_q8 would and attended to like the cached ones.
-// fmt: 0 e4m3, 1 int8. splits > 1 needs ws. inputs_static: as for mlf_paged_decode_rope.
+// fmt: 0 e4m3, 1 int8. splits > 1 needs ws, B * Hq * splits * 130 floats (ws_elems: what is there). inputs_static: as for
+// mlf_paged_decode_rope.
 MLF_API int mlf_paged_decode_q8(const void* q, long long ldq, void* cache, float* scale, int fmt, const int* block_table, const int* seq_lens,
-                                const long long* slots, void* out, float* ws, int B, int Hq, int Hkv, int block_size, int max_blocks, int num_blocks,
-                                int splits, float softmax_scale, float theta, int inputs_static, uint64_t stream) {
+                                const long long* slots, void* out, float* ws, long long ws_elems, int B, int Hq, int Hkv, int block_size, int max_blocks,
+                                int num_blocks, int splits, float softmax_scale, float theta, int inputs_static, uint64_t stream) {
   if (B <= 0) return 0;
   MLF_REQUIRE(fmt == Q8_E4M3 || fmt == Q8_INT8, "paged_decode_q8: format %d", fmt);
   MLF_REQUIRE(Hkv > 0 && Hq > 0 && Hq % Hkv == 0, "paged_decode_q8: bad head counts %d, %d", Hq, Hkv);
@@ -592,7 +616,7 @@ MLF_API int mlf_paged_decode_q8(const void* q, long long ldq, void* cache, float
   MLF_REQUIRE(block_size > 0 && max_blocks > 0 && num_blocks > 0 && splits > 0, "paged_decode_q8: bad sizes");
   MLF_REQUIRE((long long)max_blocks * block_size < (1LL << 31) - (1 << 20), "paged_decode_q8: block table of %d x %d tokens", max_blocks, block_size);
   MLF_REQUIRE(Hkv <= 65535 && splits <= 65535, "paged_decode_q8: grid");
-  MLF_REQUIRE(splits == 1 || ws != nullptr, "paged_decode_q8: workspace required for %d splits", splits);
+  MLF_REQUIRE(splits == 1 || (ws != nullptr && ws_elems >= (long long)B * Hq * splits * DQ_RED), "paged_decode_q8: workspace too small for %d splits", splits);
   MLF_REQUIRE((reinterpret_cast<uintptr_t>(cache) & 15) == 0, "paged_decode_q8: the cache must be 16-byte aligned");
   const bool rope = slots != nullptr;
   MLF_REQUIRE(rope ? ldq % 4 == 0 && (reinterpret_cast<uintptr_t>(q) & 7) == 0 && theta > 0.f : ldq % 2 == 0 && (reinterpret_cast<uintptr_t>(q) & 3) == 0,

@@ -396,12 +396,31 @@ def flash_bwd(q, k, v, o, dout, lse, B: int, S: int, *, causal: bool = True, sca
 
 # ------------------------------------------------------------------ paged attention / KV cache
 _Q8 = {torch.float8_e4m3fn: 0, torch.int8: 1}
+_TYPES = {"p": C.c_void_p, "l": C.c_longlong, "i": C.c_int, "f": C.c_float, "u": C.c_uint64}
+
+
+def _function(name: str, types: str):
+    """Entry ``name`` of the library with its argument types, one letter each: plain numbers are then converted by the call itself,
+    which takes a quarter of the time that an object for each of twenty arguments took (decode step of one sequence: 4 us)."""
+    f = getattr(_L(), name)
+    if f.argtypes is None:
+        f.argtypes = [_TYPES[c] for c in types]
+    return f
+
+
+def _at(t: Optional[torch.Tensor]) -> Optional[int]:
+    return t.data_ptr() if t is not None else None
+
+
+def _stream() -> int:
+    return _lib.stream_handle()
 
 
 def _on_current_device(what: str, *tensors: Optional[torch.Tensor]):
     """Launches go to the current device's stream: tensors of another device, or of the host, are refused."""
+    here = torch._C._cuda_getDevice() if torch.cuda.is_initialized() else 0
     for t in tensors:
-        if t is not None and not (t.is_cuda and t.device.index == torch._C._cuda_getDevice()):
+        if t is not None and t.get_device() != here:
             raise ValueError(f"{what}: a tensor is on {t.device}, the kernel runs on the current CUDA device")
 
 
@@ -410,19 +429,19 @@ def _q8_format(what: str, kv_cache: torch.Tensor, kv_scale: Optional[torch.Tenso
     fmt = _Q8.get(kv_cache.dtype)
     if fmt is None:
         raise TypeError(f"{what}: scales belong to a cache of torch.float8_e4m3fn or torch.int8, not {kv_cache.dtype}")
-    if kv_cache.dim() != 5 or kv_cache.shape[1] != 2 or kv_cache.shape[4] != 128 or not kv_cache.is_contiguous():
-        raise ValueError(f"{what}: the cache must be contiguous [num_blocks, 2, block_size, kv_heads, 128], got {tuple(kv_cache.shape)}")
+    shape = kv_cache.shape
+    if len(shape) != 5 or shape[1] != 2 or shape[4] != 128 or not kv_cache.is_contiguous():
+        raise ValueError(f"{what}: the cache must be contiguous [num_blocks, 2, block_size, kv_heads, 128], got {tuple(shape)}")
     if kv_scale is None:
         raise ValueError(f"{what}: a cache of {kv_cache.dtype} needs kv_scale")
-    want = (kv_cache.shape[0], 2, kv_cache.shape[3])
-    if tuple(kv_scale.shape) != want or kv_scale.dtype != torch.float32 or not kv_scale.is_contiguous():
-        raise ValueError(f"{what}: kv_scale must be contiguous float32 {want}, got {kv_scale.dtype} {tuple(kv_scale.shape)}")
+    if kv_scale.shape != (shape[0], 2, shape[3]) or kv_scale.dtype != torch.float32 or not kv_scale.is_contiguous():
+        raise ValueError(f"{what}: kv_scale must be contiguous float32 {(shape[0], 2, shape[3])}, got {kv_scale.dtype} {tuple(kv_scale.shape)}")
     return fmt
 
 
-def _index(what: str, name: str, t: torch.Tensor, dtype, shape) -> torch.Tensor:
-    if t.dtype != dtype or tuple(t.shape) != tuple(shape):
-        raise ValueError(f"{what}: {name} must be {dtype} {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
+def _index(what: str, name: str, t: torch.Tensor, dtype, *shape: int) -> torch.Tensor:
+    if t.dtype != dtype or t.shape != shape:
+        raise ValueError(f"{what}: {name} must be {dtype} {shape}, got {t.dtype} {tuple(t.shape)}")
     return t.contiguous()
 
 
@@ -430,7 +449,8 @@ def _heads(what: str, name: str, t: torch.Tensor, H: Optional[int] = None) -> to
     """bf16 [T, H, 128] whose tokens are whole rows at any pitch."""
     if t.dim() != 3 or t.shape[2] != 128 or (H is not None and t.shape[1] != H) or t.dtype != torch.bfloat16:
         raise ValueError(f"{what}: {name} must be bfloat16 [tokens, {'heads' if H is None else H}, 128], got {t.dtype} {tuple(t.shape)}")
-    return t if t.stride(2) == 1 and (t.stride(1) == 128 or t.shape[1] == 1) else t.contiguous()
+    _, head, one = t.stride()
+    return t if one == 1 and (head == 128 or t.shape[1] == 1) else t.contiguous()
 
 
 def _aligned_rows(t: torch.Tensor) -> torch.Tensor:
@@ -467,6 +487,18 @@ def _decode_split(pairs: int, max_seq_len: int, sms: int) -> int:
     return -(-max_seq_len // splits)
 
 
+@lru_cache(maxsize=4096)
+def _decode_split_q8(pairs: int, max_seq_len: int, sms: int) -> int:
+    """Tokens per split of the 8-bit decode kernel for ``pairs`` (sequence, KV head) pairs on ``sms`` SMs: one round of three CTAs on
+    each, of which every one has 128 tokens at least, 256 where that makes more than eight splits, and a 96th of the
+    longest sequence; none up to 384 tokens, where the merge costs more than it saves. us with 8 KV heads: 1 x 200 none 4.8
+    (2: 6.1); 1 x 700 6 splits 6.5 (1: 8.1, 3: 7.1); 1 x 4000 16 7.7 (8: 9.0, 32: 9.5); 8 x 4000 6 19 (2: 21, 16: 23);
+    13 x 2500 4 19 (1: 27, 5: 24); 16 x 4096 3 29 (1: 40, 4: 36); 48 x 4096 none 59 (3: 63); 4 x 60001 13 86 (16: 108); one KV head,
+    1 x 60000 64 16 (32: 20, 435: 25)."""
+    most = 1 if max_seq_len <= 384 else max(min(8, -(-max_seq_len // 128)), min(96, max_seq_len // 256))
+    return -(-max_seq_len // max(1, min(3 * sms // pairs, most)))
+
+
 def _decode_q8(what: str, q: torch.Tensor, ldq: int, Hq: int, kv_cache, kv_scale, block_table, seq_lens, slots, max_seq_len: int, scale, split_tokens: int,
                theta: float, inputs_static: bool) -> torch.Tensor:
     """Attention of :func:`paged_decode` (``slots`` None) and :func:`paged_decode_rope` over an 8-bit cache."""
@@ -476,24 +508,23 @@ def _decode_q8(what: str, q: torch.Tensor, ldq: int, Hq: int, kv_cache, kv_scale
         raise ValueError(f"{what}: {Hq} query heads over {Hkv} KV heads (groups of 1 to 16)")
     if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != B:
         raise ValueError(f"{what}: block_table must be int32 [{B}, max_blocks], got {block_table.dtype} {tuple(block_table.shape)}")
-    table, lens = block_table.contiguous(), _index(what, "seq_lens", seq_lens, torch.int32, (B,))
-    slots = _index(what, "slots", slots, torch.int64, (B,)) if slots is not None else None
+    table, lens = block_table.contiguous(), _index(what, "seq_lens", seq_lens, torch.int32, B)
+    slots = _index(what, "slots", slots, torch.int64, B) if slots is not None else None
     _on_current_device(what, q, kv_cache, kv_scale, table, lens, slots)
     out = torch.empty(B, Hq, 128, dtype=q.dtype, device=q.device)
     if B == 0 or Hq == 0:
         return out
     if table.shape[1] == 0:
         return out.zero_()
-    L = _L()
-    L.mlf_paged_decode_q8_ws_elems.restype = C.c_longlong
     if split_tokens <= 0:
-        split_tokens = _decode_split(B * Hkv, max_seq_len, _sm_count(torch._C._cuda_getDevice()))
+        split_tokens = _decode_split_q8(B * Hkv, max_seq_len, _sm_count(torch._C._cuda_getDevice()))
     st = (max(split_tokens, 128) + 127) // 128 * 128
     splits = max(1, (max_seq_len + st - 1) // st)
-    ws = torch.empty(int(L.mlf_paged_decode_q8_ws_elems(B, Hq, splits)), dtype=torch.float32, device=q.device) if splits > 1 else None
-    rc = L.mlf_paged_decode_q8(_p(q), C.c_longlong(ldq), _p(kv_cache), _p(kv_scale), fmt, _p(table), _p(lens), _p(slots), _p(out), _p(ws), B, Hq, Hkv,
-                               kv_cache.shape[2], table.shape[1], kv_cache.shape[0], splits, C.c_float(scale if scale is not None else 128 ** -0.5),
-                               C.c_float(theta), int(inputs_static), _st())
+    ws = torch.empty(B * Hq * splits * 130, dtype=torch.float32, device=q.device) if splits > 1 else None      # maximum, sum, output
+    rc = _function("mlf_paged_decode_q8", "plppipppppliiiiiiiffiu")(
+        q.data_ptr(), ldq, kv_cache.data_ptr(), kv_scale.data_ptr(), fmt, table.data_ptr(), lens.data_ptr(), _at(slots), out.data_ptr(), _at(ws),
+        0 if ws is None else ws.numel(), B, Hq, Hkv, kv_cache.shape[2], table.shape[1], kv_cache.shape[0], splits,
+        scale if scale is not None else 128 ** -0.5, theta, int(inputs_static), _stream())
     _lib.check(rc, "mlf_paged_decode_q8")
     return out
 
@@ -602,14 +633,15 @@ def kv_cache_write(kv_cache: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slo
         T = k.shape[0]
         if v.shape[0] != T:
             raise ValueError(f"{what}: {T} keys and {v.shape[0]} values")
-        slots = _index(what, "slots", slots, torch.int64, (T,))
+        slots = _index(what, "slots", slots, torch.int64, T)
         _on_current_device(what, kv_cache, kv_scale, k, v, slots)
         if T == 0 or kv_cache.numel() == 0:
             return
         nb, _, bs, Hkv, _ = kv_cache.shape
         where = torch.empty(nb * bs, dtype=torch.int32, device=k.device)
-        rc = _L().mlf_kv_write_q8(_p(kv_cache), _p(kv_scale), fmt, _p(k), _p(v), _p(slots), _p(where), C.c_longlong(T), Hkv, bs, nb,
-                                  C.c_longlong(k.stride(0)), C.c_longlong(v.stride(0)), _st())
+        rc = _function("mlf_kv_write_q8", "ppippppliiillu")(
+            kv_cache.data_ptr(), kv_scale.data_ptr(), fmt, k.data_ptr(), v.data_ptr(), slots.data_ptr(), where.data_ptr(), T, Hkv, bs, nb,
+            k.stride(0), v.stride(0), _stream())
         _lib.check(rc, "mlf_kv_write_q8")
         return
     nb, _, bs, Hkv, D = kv_cache.shape
@@ -634,7 +666,7 @@ def rope_kv_write_(qkv: torch.Tensor, pos: torch.Tensor, slots: torch.Tensor, kv
             raise ValueError(f"{what}: qkv must be bfloat16 [T, ({Hq} + 2 * {Hkv}) * 128] beside a cache of {Hkv} heads, got {qkv.dtype} {tuple(qkv.shape)}")
         if qkv.data_ptr() % 16 or qkv.stride(0) % 8:
             raise ValueError(f"{what}: rows must be 16-byte aligned")
-        pos, slots = _index(what, "pos", pos, torch.int64, (T,)), _index(what, "slots", slots, torch.int64, (T,))
+        pos, slots = _index(what, "pos", pos, torch.int64, T), _index(what, "slots", slots, torch.int64, T)
         _on_current_device(what, qkv, pos, slots, kv_cache, kv_scale)
         if T == 0:
             return qkv
@@ -657,14 +689,15 @@ def kv_gather(kv_cache: torch.Tensor, block_table_row: torch.Tensor, length: int
         what = "kv_gather"
         fmt = _q8_format(what, kv_cache, kv_scale)
         nb, _, bs, Hkv, _ = kv_cache.shape
-        row = _index(what, "block_table_row", block_table_row, torch.int32, (block_table_row.numel(),))
+        row = _index(what, "block_table_row", block_table_row, torch.int32, block_table_row.numel())
         if not 0 <= length <= row.numel() * bs:
             raise ValueError(f"{what}: {length} tokens, {row.numel()} block-table entries of {bs}")
         _on_current_device(what, kv_cache, kv_scale, row)
         k = torch.empty(length, Hkv, 128, dtype=torch.bfloat16, device=kv_cache.device)
         v = torch.empty_like(k)
         if length:
-            rc = _L().mlf_kv_gather_q8(_p(kv_cache), _p(kv_scale), fmt, _p(row), int(row.numel()), int(length), Hkv, bs, nb, _p(k), _p(v), _st())
+            rc = _function("mlf_kv_gather_q8", "ppipiiiiippu")(
+                kv_cache.data_ptr(), kv_scale.data_ptr(), fmt, row.data_ptr(), row.numel(), length, Hkv, bs, nb, k.data_ptr(), v.data_ptr(), _stream())
             _lib.check(rc, "mlf_kv_gather_q8")
         return k, v
     nb, _, bs, Hkv, D = kv_cache.shape
@@ -693,8 +726,7 @@ def kv_copy_blocks_(tensors: Sequence[torch.Tensor], pairs: Sequence[Tuple[int, 
     _on_current_device("kv_copy_blocks_", *tensors)
     bases = array("Q", [t.data_ptr() for t in tensors])
     sizes = array("q", [t.numel() // nb * t.element_size() for t in tensors])
-    p = C.c_void_p
-    rc = _L().mlf_kv_copy_blocks(p(bases.buffer_info()[0]), p(sizes.buffer_info()[0]), len(tensors), p(flat.buffer_info()[0]), len(pairs), nb, _st())
+    rc = _function("mlf_kv_copy_blocks", "ppipiiu")(bases.buffer_info()[0], sizes.buffer_info()[0], len(tensors), flat.buffer_info()[0], len(pairs), nb, _stream())
     _lib.check(rc, "mlf_kv_copy_blocks")
 
 
@@ -725,14 +757,15 @@ def sample_rows(logits: torch.Tensor, vocab: int, u: torch.Tensor, temperature: 
     rows = logits.shape[0]
     if logits.stride(1) != 1:
         logits = logits.contiguous()
-    u, temperature = _index(what, "u", u, torch.float32, (rows,)), _index(what, "temperature", temperature, torch.float32, (rows,))
-    top_k = _index(what, "top_k", top_k, torch.int32, (rows,)) if top_k is not None else None
-    top_p = _index(what, "top_p", top_p, torch.float32, (rows,)) if top_p is not None else None
-    min_p = _index(what, "min_p", min_p, torch.float32, (rows,)) if min_p is not None else None
+    u, temperature = _index(what, "u", u, torch.float32, rows), _index(what, "temperature", temperature, torch.float32, rows)
+    top_k = _index(what, "top_k", top_k, torch.int32, rows) if top_k is not None else None
+    top_p = _index(what, "top_p", top_p, torch.float32, rows) if top_p is not None else None
+    min_p = _index(what, "min_p", min_p, torch.float32, rows) if min_p is not None else None
     _on_current_device(what, logits, u, temperature, top_k, top_p, min_p)
     tokens = torch.empty(rows, dtype=torch.int64, device=logits.device)
     logprobs = torch.empty(rows, dtype=torch.float32, device=logits.device) if want_logprobs else None
-    rc = _L().mlf_sample_rows(_p(logits), int(logits.dtype == torch.float32), C.c_longlong(rows), C.c_longlong(logits.stride(0)), int(vocab), _p(u),
-                              _p(temperature), _p(top_k), _p(top_p), _p(min_p), _p(tokens), _p(logprobs), _st())
+    rc = _function("mlf_sample_rows", "pillipppppppu")(
+        logits.data_ptr(), int(logits.dtype == torch.float32), rows, logits.stride(0), vocab, u.data_ptr(), temperature.data_ptr(), _at(top_k),
+        _at(top_p), _at(min_p), tokens.data_ptr(), _at(logprobs), _stream())
     _lib.check(rc, "mlf_sample_rows")
     return (tokens, logprobs) if want_logprobs else tokens

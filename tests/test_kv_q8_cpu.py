@@ -122,3 +122,19 @@ def test_values_come_back_within_half_a_step(dtype):
         assert (err <= step).all()
     else:
         assert (err <= 2.0 ** -4 * want.abs() + 2.0 ** -9 * step).all()
+
+
+def test_argument_types_follow_the_entries():
+    """The letters with which an entry is called name the types that its C++ definition has."""
+    import re
+    from pathlib import Path
+
+    import ml_framework_b200
+    root = Path(ml_framework_b200.__file__).parent
+    source = "\n".join(p.read_text() for p in sorted((root / "csrc").rglob("*.cu")))
+    calls = re.findall(r'_function\("(\w+)", "(\w+)"\)\(', (root / "ops" / "native.py").read_text())
+    assert len(calls) >= 5
+    for name, letters in calls:
+        args = re.search(r"MLF_API int " + name + r"\(([^)]*)\)\s*\{", source).group(1).split(",")
+        want = "".join("p" if "*" in a else "u" if "uint64_t" in a else "l" if "long long" in a else "f" if "float" in a else "i" for a in args)
+        assert letters == want, name
