@@ -1,11 +1,13 @@
 // Writes to a paged 8-bit cache and the way back to bf16 (layout and scales: kv_q8.cuh).
 //
-// A block and head has one scale, so the rows of a call that fall into one block belong together: q8_map_kernel notes for each
-// slot which token goes there, and in q8_write_kernel one warp takes a block's rows of one head and side, finds their largest
-// magnitude, settles the scale and rounds. A call that writes a block's first row starts the block anew; otherwise the scale
-// is the larger of the old one and the new rows' own, and where it grows the rows that the block held are rounded to it.
-// The map is read back only where the slot it stands at names the same token, so that it needs no clearing: entries of
-// earlier calls, or of nothing at all, point at tokens of other slots.
+// A block and head has one scale, so the rows of a call that fall into one block belong together: one warp takes a block's rows of
+// one head and side, finds their largest magnitude, settles the scale and rounds. A call that writes a block's first row starts
+// the block anew; otherwise the scale is the larger of the old one and the new rows' own, and where it grows the rows that the
+// block held are rounded to it. Which rows of a block a call writes: up to 256 tokens, a warp looks through all their slots. For more,
+// q8_map_kernel notes for each slot which token goes there; the map is read back only where the slot it stands at names the same
+// token, so that it needs no clearing: entries of earlier calls, or of nothing at all, point at tokens of other slots.
+//
+// Bound by HBM in long calls (a row is read in 16 bits and written in 8), by the chain of loads slots - map - slots - rows in short ones.
 #include "../common/host.h"
 #include "../common/ptx.cuh"
 #include "../mlf_api.h"
@@ -15,13 +17,14 @@ namespace mlf {
 
 constexpr int QW_WARPS = 8;
 constexpr int QW_GROUP = 16;                  // tokens whose blocks a CTA looks at: in a prompt's order about one block
+constexpr int QW_FEW = 256;                   // tokens that need no map
 
 struct Q8WriteParams {
   uint8_t* cache;
   float* scale;
   const __nv_bfloat16 *k, *v;
   const long long* slots;
-  int* map;                                   // [num_blocks * block_size]
+  int* map;                                   // [num_blocks * block_size], null up to QW_FEW tokens
   long long T, ldk, ldv;
   int Hkv, block_size, num_blocks, group;
   int* err;
@@ -41,14 +44,30 @@ __global__ void __launch_bounds__(256) q8_map_kernel(const Q8WriteParams p) {
   p.map[slot] = (int)t;                       // a slot that is given twice keeps one of its tokens
 }
 
-// The token that this call writes to `slot`, or -1.
-__device__ __forceinline__ int q8_token_at(const Q8WriteParams& p, long long slot) {
-  const int t = p.map[slot];
-  return t >= 0 && t < p.T && p.slots[t] == slot ? t : -1;
+// Lanes 0 .. 15: the token that this call writes to slot first + lane, the lowest of them without a map, or -1 (also for the
+// `count` rows' end). `found`: 16 ints of this warp.
+__device__ __forceinline__ int q8_tokens_at(const Q8WriteParams& p, long long first, int count, int* found) {
+  const int lane = threadIdx.x & 31;
+  if (p.map != nullptr) {
+    if (lane >= count) return -1;
+    const int t = p.map[first + lane];
+    return t >= 0 && t < p.T && p.slots[t] == first + lane ? t : -1;
+  }
+  __syncwarp();
+  if (lane < 16) found[lane] = 0x7fffffff;
+  __syncwarp();
+  for (int t = lane; t < p.T; t += 32) {
+    const long long at = p.slots[t] - first;
+    if (at >= 0 && at < count) atomicMin(&found[at], t);
+  }
+  __syncwarp();
+  const int t = lane < count ? found[lane] : 0x7fffffff;
+  return t == 0x7fffffff ? -1 : t;
 }
 
+// known: the tokens of the block's first 16 rows, by row
 template <int FMT>
-__device__ __forceinline__ void q8_write_rows(const Q8WriteParams& p, int blk, int h, int side) {
+__device__ __forceinline__ void q8_write_rows(const Q8WriteParams& p, int blk, int h, int side, const int* known, int* found) {
   const int lane = threadIdx.x & 31, half = lane >> 4, col = (lane & 15) * 8;
   const long long first = (long long)blk * p.block_size;
   const __nv_bfloat16* src = (side ? p.v : p.k) + (long long)h * Q8_D + col;
@@ -59,14 +78,14 @@ __device__ __forceinline__ void q8_write_rows(const Q8WriteParams& p, int blk, i
   uint4 x[8];
   int tok = -1;                               // lanes 0..15: the token of row chunk * 16 + lane
   auto load = [&](int c) {
-    const int row = c * 16 + lane;
-    tok = lane < 16 && row < p.block_size ? q8_token_at(p, first + row) : -1;
+    tok = c == 0 ? (lane < 16 ? known[lane] : -1) : q8_tokens_at(p, first + c * 16, min(16, p.block_size - c * 16), found);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int t = __shfl_sync(0xffffffffu, tok, 2 * i + half);
       x[i] = t >= 0 ? *reinterpret_cast<const uint4*>(src + t * ld) : make_uint4(0u, 0u, 0u, 0u);
     }
   };
+  const float held_scale = *scale;
   float amax = 0.f;
   bool anew = false;
   for (int c = 0; c < chunks; ++c) {
@@ -84,7 +103,7 @@ __device__ __forceinline__ void q8_write_rows(const Q8WriteParams& p, int blk, i
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-  const float fit = q8_scale_for<FMT>(amax), before = anew ? 0.f : *scale;
+  const float fit = q8_scale_for<FMT>(amax), before = anew ? 0.f : held_scale;
   const float now = fmaxf(before, fit);
   const float inv = __frcp_rn(now), ratio = before * inv;     // exact for powers of two
   const bool shrink = !anew && before < now;
@@ -112,30 +131,42 @@ __device__ __forceinline__ void q8_write_rows(const Q8WriteParams& p, int blk, i
 // heads and sides are split over blockIdx.y.
 template <int FMT>
 __global__ void __launch_bounds__(QW_WARPS * 32) q8_write_kernel(const Q8WriteParams p) {
-  __shared__ int s_blk[QW_GROUP];
+  __shared__ int s_blk[QW_GROUP], s_tok[QW_GROUP][16], s_found[QW_WARPS][16];
   pdl_trigger();
   pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int i = warp; i < p.group; i += QW_WARPS) {
     const long long t = (long long)blockIdx.x * p.group + i;
-    int blk = -1;
+    int blk = -1, tok = -1;
     if (t < p.T) {
       const long long slot = p.slots[t];
-      if (slot >= 0 && slot < (long long)p.num_blocks * p.block_size && p.map[slot] == (int)t) {
+      if (slot >= (long long)p.num_blocks * p.block_size) {
+        if (p.map == nullptr && lane == 0) atomicCAS(p.err, 0, ERR_BAD_INDEX);
+      } else if (slot >= 0) {
         blk = (int)(slot / p.block_size);
+        // this token takes the block if it is the first, by row, of those that the call writes there
         const int off = (int)(slot - (long long)blk * p.block_size);
-        bool earlier = false;
-        for (int r = lane; r < off; r += 32) earlier = earlier || q8_token_at(p, (long long)blk * p.block_size + r) >= 0;
-        if (__any_sync(0xffffffffu, earlier)) blk = -1;
+        const long long first = (long long)blk * p.block_size;
+        for (int c = 0; c * 16 <= off && blk >= 0; ++c) {
+          const int at = q8_tokens_at(p, first + c * 16, min(16, p.block_size - c * 16), s_found[warp]);
+          if (c == 0) tok = at;
+          const unsigned there = __ballot_sync(0xffffffffu, at >= 0);
+          if (there != 0) {
+            const int row = __ffs(there) - 1;
+            if (c * 16 + row != off || __shfl_sync(0xffffffffu, at, row) != (int)t) blk = -1;
+            else break;
+          }
+        }
       }
     }
     if (lane == 0) s_blk[i] = blk;
+    if (lane < 16) s_tok[i][lane] = tok;
   }
   __syncthreads();
   const int units = 2 * p.Hkv;
   for (int i = 0; i < p.group; ++i) {
     if (s_blk[i] < 0) continue;
-    for (int u = blockIdx.y * QW_WARPS + warp; u < units; u += gridDim.y * QW_WARPS) q8_write_rows<FMT>(p, s_blk[i], u >> 1, u & 1);
+    for (int u = blockIdx.y * QW_WARPS + warp; u < units; u += gridDim.y * QW_WARPS) q8_write_rows<FMT>(p, s_blk[i], u >> 1, u & 1, s_tok[i], s_found[warp]);
   }
 }
 
@@ -181,7 +212,7 @@ q8_gather_kernel(const uint8_t* cache, const float* scale, const int* block_tabl
 using namespace mlf;
 
 // k, v [T, Hkv, 128] bf16 (row pitch ldk / ldv, 16-byte aligned rows) into slots[T] = block * block_size + offset (< 0 skips).
-// map: num_blocks * block_size ints of scratch, any contents. fmt: 0 e4m3, 1 int8.
+// map: num_blocks * block_size ints of scratch, any contents; not needed for up to 256 tokens. fmt: 0 e4m3, 1 int8.
 MLF_API int mlf_kv_write_q8(void* cache, float* scale, int fmt, const void* k, const void* v, const long long* slots, int* map, long long T,
                             int Hkv, int block_size, int num_blocks, long long ldk, long long ldv, uint64_t stream) {
   if (T <= 0) return 0;
@@ -195,17 +226,18 @@ MLF_API int mlf_kv_write_q8(void* cache, float* scale, int fmt, const void* k, c
   p.k = static_cast<const __nv_bfloat16*>(k);
   p.v = static_cast<const __nv_bfloat16*>(v);
   p.slots = slots;
-  p.map = map;
+  p.map = T > QW_FEW ? map : nullptr;
+  MLF_REQUIRE(T <= QW_FEW || map != nullptr, "kv_write_q8: %lld tokens need a map", T);
   p.T = T; p.ldk = ldk; p.ldv = ldv;
   p.Hkv = Hkv; p.block_size = block_size; p.num_blocks = num_blocks;
-  p.group = T >= 256 ? QW_GROUP : 1;          // few tokens: often one to a block, and too few CTAs otherwise
+  p.group = T > QW_FEW ? QW_GROUP : 1;        // few tokens: often one to a block, and too few CTAs otherwise
   p.err = device_status_word();
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  MLF_CHECK_CUDA(launch_pdl(q8_map_kernel, dim3((unsigned)((T + 255) / 256)), dim3(256), 0, st, p));
+  if (p.map != nullptr) MLF_CHECK_CUDA(launch_pdl(q8_map_kernel, dim3((unsigned)((T + 255) / 256)), dim3(256), 0, st, p));
   const dim3 grid((unsigned)((T + p.group - 1) / p.group), (unsigned)((2 * Hkv + QW_WARPS - 1) / QW_WARPS));
   const auto kernel = fmt == Q8_E4M3 ? q8_write_kernel<Q8_E4M3> : q8_write_kernel<Q8_INT8>;
   MLF_CHECK_CUDA(launch_pdl(kernel, grid, dim3(QW_WARPS * 32), 0, st, p));
-  count_launch(2);
+  count_launch(p.map != nullptr ? 2 : 1);
   return 0;
 }
 

@@ -1032,7 +1032,7 @@ MLF_API int mlf_sample_rows(const void* logits, int is_fp32, long long rows, lon
     MLF_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     set = true;
   }
-  MLF_CHECK_CUDA(launch_pdl_cluster(kernel, dim3((unsigned)(rows * C)), dim3(SM_THREADS), smem, (unsigned)C,
+  MLF_CHECK_CUDA(launch_pdl_cluster(kernel, dim3((unsigned)(rows * C)), dim3(SM_THREADS), smem, dim3((unsigned)C),
                                     reinterpret_cast<cudaStream_t>(stream), p));
   count_launch();
   return 0;

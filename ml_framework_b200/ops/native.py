@@ -492,8 +492,8 @@ def _decode_split_q8(pairs: int, max_seq_len: int, sms: int) -> int:
     """Tokens per split of the 8-bit decode kernel for ``pairs`` (sequence, KV head) pairs on ``sms`` SMs: one round of three CTAs on
     each, of which every one has 128 tokens at least, 256 where that makes more than eight splits, and a 96th of the
     longest sequence; none up to 384 tokens, where the merge costs more than it saves. us with 8 KV heads: 1 x 200 none 4.8
-    (2: 6.1); 1 x 700 6 splits 6.5 (1: 8.1, 3: 7.1); 1 x 4000 16 7.7 (8: 9.0, 32: 9.5); 8 x 4000 6 19 (2: 21, 16: 23);
-    13 x 2500 4 19 (1: 27, 5: 24); 16 x 4096 3 29 (1: 40, 4: 36); 48 x 4096 none 59 (3: 63); 4 x 60001 13 86 (16: 108); one KV head,
+    (2: 6.1); 1 x 700 6 splits 5.4 (1: 8.4, 3: 6.6); 1 x 4000 16 7.7 (8: 8.3, 32: 9.7); 8 x 4000 6 17 (2: 24, 16: 23);
+    13 x 2500 4 18 (1: 27, 5: 25); 16 x 4096 3 27 (1: 39, 4: 37); 48 x 4096 none 58 (2: 63); 4 x 60001 13 86 (16: 108); one KV head,
     1 x 60000 64 16 (32: 20, 435: 25)."""
     most = 1 if max_seq_len <= 384 else max(min(8, -(-max_seq_len // 128)), min(96, max_seq_len // 256))
     return -(-max_seq_len // max(1, min(3 * sms // pairs, most)))
@@ -516,11 +516,14 @@ def _decode_q8(what: str, q: torch.Tensor, ldq: int, Hq: int, kv_cache, kv_scale
         return out
     if table.shape[1] == 0:
         return out.zero_()
+    sms = _sm_count(torch._C._cuda_getDevice())
     if split_tokens <= 0:
-        split_tokens = _decode_split_q8(B * Hkv, max_seq_len, _sm_count(torch._C._cuda_getDevice()))
+        split_tokens = _decode_split_q8(B * Hkv, max_seq_len, sms)
     st = (max(split_tokens, 128) + 127) // 128 * 128
     splits = max(1, (max_seq_len + st - 1) // st)
-    ws = torch.empty(B * Hq * splits * 130, dtype=torch.float32, device=q.device) if splits > 1 else None      # maximum, sum, output
+    # maximum, sum and output of each split; up to eight that are resident at once are merged within the launch
+    within = splits <= 8 and (splits == 1 or B * Hkv * splits <= 3 * sms)
+    ws = None if within else torch.empty(B * Hq * splits * 130, dtype=torch.float32, device=q.device)
     rc = _function("mlf_paged_decode_q8", "plppipppppliiiiiiiffiu")(
         q.data_ptr(), ldq, kv_cache.data_ptr(), kv_scale.data_ptr(), fmt, table.data_ptr(), lens.data_ptr(), _at(slots), out.data_ptr(), _at(ws),
         0 if ws is None else ws.numel(), B, Hq, Hkv, kv_cache.shape[2], table.shape[1], kv_cache.shape[0], splits,
@@ -543,7 +546,7 @@ def paged_decode(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Ten
 
     An 8-bit cache (float8_e4m3fn or int8) comes with ``kv_scale``, float32 [num_blocks, 2, Hkv]: a value is its number times the
     scale of its block, side (K, V) and head. Any positive scales; groups of 1 to 16 query heads per KV head; the splits
-    (a whole number of blocks each) are merged by a second kernel. A sequence of length 0 gives zeros.
+    are a whole number of blocks each. A sequence of length 0 gives zeros.
     """
     if kv_scale is not None or kv_cache.dtype in _Q8:
         q = _heads("paged_decode", "q", q)
@@ -625,7 +628,7 @@ def kv_cache_write(kv_cache: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slo
     127 for int8; larger values than 2^40 allows become the largest number). A call that writes a block's first row starts
     the block anew: rows of it that the call does not write lose their meaning. A call that writes later rows only keeps the
     larger of the block's scale and their own, and rounds the rows that the block holds to it. Rows of one block may
-    stand anywhere in the list; a slot given twice keeps one of its rows. NaN stays NaN in e4m3 and becomes 0 in int8."""
+    stand anywhere in the list; a slot given twice keeps one of its rows, whole. NaN stays NaN in e4m3 and becomes 0 in int8."""
     if kv_scale is not None or kv_cache.dtype in _Q8:
         what = "kv_cache_write"
         fmt = _q8_format(what, kv_cache, kv_scale)
@@ -638,9 +641,9 @@ def kv_cache_write(kv_cache: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slo
         if T == 0 or kv_cache.numel() == 0:
             return
         nb, _, bs, Hkv, _ = kv_cache.shape
-        where = torch.empty(nb * bs, dtype=torch.int32, device=k.device)
+        where = torch.empty(nb * bs, dtype=torch.int32, device=k.device) if T > 256 else None
         rc = _function("mlf_kv_write_q8", "ppippppliiillu")(
-            kv_cache.data_ptr(), kv_scale.data_ptr(), fmt, k.data_ptr(), v.data_ptr(), slots.data_ptr(), where.data_ptr(), T, Hkv, bs, nb,
+            kv_cache.data_ptr(), kv_scale.data_ptr(), fmt, k.data_ptr(), v.data_ptr(), slots.data_ptr(), _at(where), T, Hkv, bs, nb,
             k.stride(0), v.stride(0), _stream())
         _lib.check(rc, "mlf_kv_write_q8")
         return
@@ -719,13 +722,13 @@ def kv_copy_blocks_(tensors: Sequence[torch.Tensor], pairs: Sequence[Tuple[int, 
         raise ValueError("kv_copy_blocks_: pairs must be (source, destination) block numbers")
     if not tensors or not flat:
         return
-    nb = tensors[0].shape[0] if tensors[0].dim() else 0
+    nb = len(tensors[0]) if tensors[0].dim() else 0
     for t in tensors:
-        if t.numel() == 0 or t.shape[0] != nb or not t.is_contiguous():
+        if t.dim() == 0 or len(t) != nb or t.numel() == 0 or not t.is_contiguous():
             raise ValueError(f"kv_copy_blocks_: tensors must be contiguous with the same number of blocks, got {tuple(t.shape)} beside {nb}")
     _on_current_device("kv_copy_blocks_", *tensors)
     bases = array("Q", [t.data_ptr() for t in tensors])
-    sizes = array("q", [t.numel() // nb * t.element_size() for t in tensors])
+    sizes = array("q", [t.nbytes // nb for t in tensors])
     rc = _function("mlf_kv_copy_blocks", "ppipiiu")(bases.buffer_info()[0], sizes.buffer_info()[0], len(tensors), flat.buffer_info()[0], len(pairs), nb, _stream())
     _lib.check(rc, "mlf_kv_copy_blocks")
 

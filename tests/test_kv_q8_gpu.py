@@ -187,6 +187,23 @@ def test_attention(dtype, Hq, Hkv, bs, split, power):
 
 
 @pytest.mark.parametrize("dtype", KINDS)
+@pytest.mark.parametrize("split,bs,Hq", [(128, 16, 8), (128, 24, 8), (256, 16, 32), (0, 16, 8), (1024, 16, 2), (400, 48, 8)])
+def test_attention_many_splits(dtype, split, bs, Hq):
+    """Splits that a cluster merges (two to eight) and more, which a second kernel does; sequences that end in any of them."""
+    lens = [20000, 1, 0, 129, 1025, 2048, 7777, 17000]
+    g = _gen(split)
+    table, nb = _tables(lens, bs, g)
+    cache, scale = _random_cache(nb, bs, 2, dtype, g)
+    scale = scale * 2.0 ** -4
+    q = torch.randn(len(lens), Hq, D, device="cuda", generator=g).to(torch.bfloat16)
+    sl = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    want, tol = _exact(q, cache, scale, table, lens, D ** -0.5)
+    got = native.paged_decode(q, cache, table, sl, max(lens), split_tokens=split, kv_scale=scale)
+    _check(got, want, tol)
+    assert (got[2] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", KINDS)
 def test_attention_wide_ranges(dtype):
     """Scales 2^-40 to 2^40 side by side, queries of very different size, one key that takes all the weight."""
     lens, bs, Hkv, G = [300, 77], 16, 2, 4
