@@ -3,11 +3,13 @@
 // A block and head has one scale, so the rows of a call that fall into one block belong together: one warp takes a block's rows of
 // one head and side, finds their largest magnitude, settles the scale and rounds. A call that writes a block's first row starts
 // the block anew; otherwise the scale is the larger of the old one and the new rows' own, and where it grows the rows that the
-// block held are rounded to it. Which rows of a block a call writes: up to 256 tokens, a warp looks through all their slots. For more,
-// q8_map_kernel notes for each slot which token goes there; the map is read back only where the slot it stands at names the same
-// token, so that it needs no clearing: entries of earlier calls, or of nothing at all, point at tokens of other slots.
+// block held are rounded to it. Which rows of a block a call writes: up to 2048 tokens, a CTA looks through all slots of the call
+// (16 KB, from the L2). For more, or blocks of more than 64 rows, q8_map_kernel notes for each slot which token goes there; the map is
+// read back only where the slot it stands at names the same token, so that it needs no clearing: entries of earlier calls, or of
+// nothing at all, point at tokens of other slots.
 //
-// Bound by HBM in long calls (a row is read in 16 bits and written in 8), by the chain of loads slots - map - slots - rows in short ones.
+// Bound by HBM in long calls (a row is read in 16 bits and written in 8), by the chain of loads slots - rows (slots - map - slots -
+// rows) in short ones. WRITE_FIGURES
 #include "../common/host.h"
 #include "../common/ptx.cuh"
 #include "../mlf_api.h"
@@ -17,16 +19,17 @@ namespace mlf {
 
 constexpr int QW_WARPS = 8;
 constexpr int QW_GROUP = 16;                  // tokens whose blocks a CTA looks at: in a prompt's order about one block
-constexpr int QW_FEW = 256;                   // tokens that need no map
+constexpr int QW_FEW = 2048;                  // tokens, and rows of a block, that need no map
+constexpr int QW_ROWS = 64;
 
 struct Q8WriteParams {
   uint8_t* cache;
   float* scale;
   const __nv_bfloat16 *k, *v;
   const long long* slots;
-  int* map;                                   // [num_blocks * block_size], null up to QW_FEW tokens
+  int* map;                                   // [num_blocks * block_size]; null: every CTA looks through the slots
   long long T, ldk, ldv;
-  int Hkv, block_size, num_blocks, group;
+  int Hkv, block_size, bs_shift, num_blocks, group;       // bs_shift: log2(block_size) or -1
   int* err;
 };
 
@@ -44,30 +47,21 @@ __global__ void __launch_bounds__(256) q8_map_kernel(const Q8WriteParams p) {
   p.map[slot] = (int)t;                       // a slot that is given twice keeps one of its tokens
 }
 
-// Lanes 0 .. 15: the token that this call writes to slot first + lane, the lowest of them without a map, or -1 (also for the
-// `count` rows' end). `found`: 16 ints of this warp.
-__device__ __forceinline__ int q8_tokens_at(const Q8WriteParams& p, long long first, int count, int* found) {
-  const int lane = threadIdx.x & 31;
-  if (p.map != nullptr) {
-    if (lane >= count) return -1;
-    const int t = p.map[first + lane];
-    return t >= 0 && t < p.T && p.slots[t] == first + lane ? t : -1;
-  }
-  __syncwarp();
-  if (lane < 16) found[lane] = 0x7fffffff;
-  __syncwarp();
-  for (int t = lane; t < p.T; t += 32) {
-    const long long at = p.slots[t] - first;
-    if (at >= 0 && at < count) atomicMin(&found[at], t);
-  }
-  __syncwarp();
-  const int t = lane < count ? found[lane] : 0x7fffffff;
-  return t == 0x7fffffff ? -1 : t;
+// slot / block_size: a division of 64 bits takes as long as a load
+__device__ __forceinline__ int q8_block(const Q8WriteParams& p, long long slot) {
+  if (p.bs_shift >= 0) return (int)(slot >> p.bs_shift);
+  return slot <= 0x7fffffff ? (int)((unsigned)slot / (unsigned)p.block_size) : (int)(slot / p.block_size);
 }
 
-// known: the tokens of the block's first 16 rows, by row
+// The token that the map has for `slot`, or -1.
+__device__ __forceinline__ int q8_token_at(const Q8WriteParams& p, long long slot) {
+  const int t = p.map[slot];
+  return t >= 0 && t < p.T && p.slots[t] == slot ? t : -1;
+}
+
+// A block's rows of one head and side. known: the tokens of its rows (-1: not written by this call), the first 16 of them with a map.
 template <int FMT>
-__device__ __forceinline__ void q8_write_rows(const Q8WriteParams& p, int blk, int h, int side, const int* known, int* found) {
+__device__ __forceinline__ void q8_write_rows(const Q8WriteParams& p, int blk, int h, int side, const int* known) {
   const int lane = threadIdx.x & 31, half = lane >> 4, col = (lane & 15) * 8;
   const long long first = (long long)blk * p.block_size;
   const __nv_bfloat16* src = (side ? p.v : p.k) + (long long)h * Q8_D + col;
@@ -78,7 +72,9 @@ __device__ __forceinline__ void q8_write_rows(const Q8WriteParams& p, int blk, i
   uint4 x[8];
   int tok = -1;                               // lanes 0..15: the token of row chunk * 16 + lane
   auto load = [&](int c) {
-    tok = c == 0 ? (lane < 16 ? known[lane] : -1) : q8_tokens_at(p, first + c * 16, min(16, p.block_size - c * 16), found);
+    const int row = c * 16 + lane;
+    tok = -1;
+    if (lane < 16 && row < p.block_size) tok = p.map == nullptr || c == 0 ? known[row] : q8_token_at(p, first + row);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int t = __shfl_sync(0xffffffffu, tok, 2 * i + half);
@@ -127,83 +123,124 @@ __device__ __forceinline__ void q8_write_rows(const Q8WriteParams& p, int blk, i
   if (lane == 0) *scale = now;
 }
 
-// A CTA finds, among `group` tokens, those that are the first of their block's rows in this call, and writes those blocks; the
-// heads and sides are split over blockIdx.y.
+// A CTA looks at the blocks of `group` tokens and writes those whose first row, of the rows that the call writes there, one of these
+// tokens is; the heads and sides are split over blockIdx.y.
 template <int FMT>
 __global__ void __launch_bounds__(QW_WARPS * 32) q8_write_kernel(const Q8WriteParams p) {
-  __shared__ int s_blk[QW_GROUP], s_tok[QW_GROUP][16], s_found[QW_WARPS][16];
+  __shared__ int s_blk[QW_GROUP], s_tok[QW_GROUP][QW_ROWS], s_blocks;
   pdl_trigger();
   pdl_wait();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int i = warp; i < p.group; i += QW_WARPS) {
-    const long long t = (long long)blockIdx.x * p.group + i;
-    int blk = -1, tok = -1;
-    if (t < p.T) {
-      const long long slot = p.slots[t];
-      if (slot >= (long long)p.num_blocks * p.block_size) {
-        if (p.map == nullptr && lane == 0) atomicCAS(p.err, 0, ERR_BAD_INDEX);
-      } else if (slot >= 0) {
-        blk = (int)(slot / p.block_size);
-        // this token takes the block if it is the first, by row, of those that the call writes there
-        const int off = (int)(slot - (long long)blk * p.block_size);
-        const long long first = (long long)blk * p.block_size;
-        for (int c = 0; c * 16 <= off && blk >= 0; ++c) {
-          const int at = q8_tokens_at(p, first + c * 16, min(16, p.block_size - c * 16), s_found[warp]);
-          if (c == 0) tok = at;
-          const unsigned there = __ballot_sync(0xffffffffu, at >= 0);
-          if (there != 0) {
-            const int row = __ffs(there) - 1;
-            if (c * 16 + row != off || __shfl_sync(0xffffffffu, at, row) != (int)t) blk = -1;
-            else break;
-          }
-        }
-      }
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const long long from = (long long)blockIdx.x * p.group, end = (long long)p.num_blocks * p.block_size;
+  if (p.map == nullptr) {
+    // the blocks of the group, each once; then every token of the call that goes to one of them
+    if (warp == 0) {
+      const long long slot = lane < p.group && from + lane < p.T ? p.slots[from + lane] : -1;
+      if (slot >= end) atomicCAS(p.err, 0, ERR_BAD_INDEX);
+      const int blk = slot >= 0 && slot < end ? q8_block(p, slot) : -1;
+      const unsigned same = __match_any_sync(0xffffffffu, blk);        // every lane takes part
+      const bool once = blk >= 0 && __ffs(same) - 1 == lane;
+      const unsigned all = __ballot_sync(0xffffffffu, once);
+      if (once) s_blk[__popc(all & ((1u << lane) - 1u))] = blk;
+      if (lane == 0) s_blocks = __popc(all);
     }
-    if (lane == 0) s_blk[i] = blk;
-    if (lane < 16) s_tok[i][lane] = tok;
+    for (int i = tid; i < QW_GROUP * QW_ROWS; i += QW_WARPS * 32) (&s_tok[0][0])[i] = 0x7fffffff;
+    __syncthreads();
+    const int n = s_blocks;
+    for (int t = tid; t < p.T; t += QW_WARPS * 32) {
+      const long long slot = p.slots[t];
+      if (slot < 0 || slot >= end) continue;
+      const int blk = q8_block(p, slot);
+      for (int i = 0; i < n; ++i)
+        if (s_blk[i] == blk) atomicMin(&s_tok[i][slot - (long long)blk * p.block_size], t);       // a slot that is given twice: the lower token
+    }
+    __syncthreads();
+    for (int i = warp; i < n; i += QW_WARPS) {
+      int first = -1;
+      for (int r0 = 0; r0 < p.block_size; r0 += 32) {
+        const int r = r0 + lane, t = r < p.block_size ? s_tok[i][r] : 0x7fffffff;
+        const unsigned there = __ballot_sync(0xffffffffu, t != 0x7fffffff);
+        if (first < 0 && there != 0) first = __shfl_sync(0xffffffffu, t, __ffs(there) - 1);
+        __syncwarp();
+        if (r < p.block_size && t == 0x7fffffff) s_tok[i][r] = -1;
+      }
+      if (lane == 0 && (first < from || first >= from + p.group)) s_blk[i] = -1;                   // another CTA's
+    }
+  } else {
+    if (tid == 0) s_blocks = p.group;
+    for (int i = warp; i < p.group; i += QW_WARPS) {
+      const long long t = from + i, slot = t < p.T ? p.slots[t] : -1;
+      int blk = -1;
+      if (slot >= 0 && slot < end) {
+        blk = q8_block(p, slot);
+        const long long first = (long long)blk * p.block_size;
+        const int off = (int)(slot - first);
+        bool mine = p.map[slot] == (int)t;
+        for (int r0 = 0; r0 <= off && mine; r0 += 32) {
+          const int r = r0 + lane, at = r < p.block_size ? q8_token_at(p, first + r) : -1;
+          if (r < 16) s_tok[i][r] = at;
+          if (__any_sync(0xffffffffu, at >= 0 && r < off)) mine = false;
+        }
+        if (!mine) blk = -1;
+      }
+      if (lane == 0) s_blk[i] = blk;
+    }
   }
   __syncthreads();
-  const int units = 2 * p.Hkv;
-  for (int i = 0; i < p.group; ++i) {
+  const int units = 2 * p.Hkv, blocks = s_blocks;
+  for (int i = 0; i < blocks; ++i) {
     if (s_blk[i] < 0) continue;
-    for (int u = blockIdx.y * QW_WARPS + warp; u < units; u += gridDim.y * QW_WARPS) q8_write_rows<FMT>(p, s_blk[i], u >> 1, u & 1, s_tok[i], s_found[warp]);
+    for (int u = blockIdx.y * QW_WARPS + warp; u < units; u += gridDim.y * QW_WARPS) q8_write_rows<FMT>(p, s_blk[i], u >> 1, u & 1, s_tok[i]);
   }
 }
+static_assert(QW_GROUP <= 32, "a lane for every token of a group");
 
-// out_k / out_v [len, Hkv, 128] bf16 <- pages of one sequence; a thread takes 16 numbers of a key and of the value.
+// out_k / out_v [len, Hkv, 128] bf16 <- pages of one sequence; eight threads a token and head, 16 numbers of its key and of its value
+// each, of two such pairs at a time.
+constexpr int QG_PAIRS = 2;
 template <int FMT>
 __global__ void __launch_bounds__(256)
-q8_gather_kernel(const uint8_t* cache, const float* scale, const int* block_table, int len, int Hkv, int block_size, int num_blocks,
-                 __nv_bfloat16* out_k, __nv_bfloat16* out_v, int* err) {   // len <= table entries * block_size (checked by the launcher)
+q8_gather_kernel(const uint8_t* cache, const float* scale, const int* block_table, unsigned pairs, int Hkv, int block_size, int num_blocks,
+                 __nv_bfloat16* out_k, __nv_bfloat16* out_v, int* err) {   // tokens <= table entries * block_size (checked by the launcher)
   pdl_trigger();
   pdl_wait();
-  const int vec_per_tok = Hkv * (Q8_D / 16);
-  const long long total = (long long)len * vec_per_tok;
   const long long side = (long long)block_size * Hkv * Q8_D;
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
-    const int t = (int)(i / vec_per_tok), c = (int)(i - (long long)t * vec_per_tok) * 16;
-    int blk = block_table[t / block_size];
-    if (blk < 0 || blk >= num_blocks) { atomicCAS(err, 0, ERR_BAD_INDEX); blk = 0; }
-    const uint8_t* src = cache + 2 * side * blk + (long long)(t % block_size) * Hkv * Q8_D + c;
-    const float* s = scale + (long long)blk * 2 * Hkv + c / Q8_D;
-    const uint4 k = *reinterpret_cast<const uint4*>(src), v = *reinterpret_cast<const uint4*>(src + side);
-    const float sk = s[0], sv = s[Hkv];
-    const unsigned kw[4] = {k.x, k.y, k.z, k.w}, vw[4] = {v.x, v.y, v.z, v.w};
-    unsigned ok[8], ov[8];
+  const unsigned first = blockIdx.x * (32 * QG_PAIRS) + (threadIdx.x >> 3), c = (threadIdx.x & 7) * 16;
+  uint4 k[QG_PAIRS], v[QG_PAIRS];
+  float sk[QG_PAIRS], sv[QG_PAIRS];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float4 a = q8_floats<FMT>(kw[j]), b = q8_floats<FMT>(vw[j]);
-      ok[2 * j] = pack_bf16x2(a.x * sk, a.y * sk);
-      ok[2 * j + 1] = pack_bf16x2(a.z * sk, a.w * sk);
-      ov[2 * j] = pack_bf16x2(b.x * sv, b.y * sv);
-      ov[2 * j + 1] = pack_bf16x2(b.z * sv, b.w * sv);
-    }
-    uint4* dk = reinterpret_cast<uint4*>(out_k + (long long)t * Hkv * Q8_D + c);
-    uint4* dv = reinterpret_cast<uint4*>(out_v + (long long)t * Hkv * Q8_D + c);
-    dk[0] = make_uint4(ok[0], ok[1], ok[2], ok[3]);
-    dk[1] = make_uint4(ok[4], ok[5], ok[6], ok[7]);
-    dv[0] = make_uint4(ov[0], ov[1], ov[2], ov[3]);
-    dv[1] = make_uint4(ov[4], ov[5], ov[6], ov[7]);
+  for (int e = 0; e < QG_PAIRS; ++e) {
+    const unsigned i = first + 32 * e;
+    if (i >= pairs) break;
+    const unsigned t = i / (unsigned)Hkv, h = i - t * Hkv, b = t / (unsigned)block_size;
+    int blk = block_table[b];
+    if (blk < 0 || blk >= num_blocks) { atomicCAS(err, 0, ERR_BAD_INDEX); blk = 0; }
+    const uint8_t* src = cache + 2 * side * blk + ((long long)(t - b * block_size) * Hkv + h) * Q8_D + c;
+    const float* s = scale + (long long)blk * 2 * Hkv + h;
+    k[e] = *reinterpret_cast<const uint4*>(src);
+    v[e] = *reinterpret_cast<const uint4*>(src + side);
+    sk[e] = s[0];
+    sv[e] = s[Hkv];
+  }
+#pragma unroll
+  for (int e = 0; e < QG_PAIRS; ++e) {
+    const unsigned i = first + 32 * e;
+    if (i >= pairs) break;
+    auto put = [&](uint4 q, float f, __nv_bfloat16* out) {
+      const unsigned w[4] = {q.x, q.y, q.z, q.w};
+      unsigned o[8];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float4 a = q8_floats<FMT>(w[j]);
+        o[2 * j] = pack_bf16x2(a.x * f, a.y * f);
+        o[2 * j + 1] = pack_bf16x2(a.z * f, a.w * f);
+      }
+      uint4* d = reinterpret_cast<uint4*>(out + (long long)i * Q8_D + c);
+      d[0] = make_uint4(o[0], o[1], o[2], o[3]);
+      d[1] = make_uint4(o[4], o[5], o[6], o[7]);
+    };
+    put(k[e], sk[e], out_k);
+    put(v[e], sv[e], out_v);
   }
 }
 
@@ -212,7 +249,7 @@ q8_gather_kernel(const uint8_t* cache, const float* scale, const int* block_tabl
 using namespace mlf;
 
 // k, v [T, Hkv, 128] bf16 (row pitch ldk / ldv, 16-byte aligned rows) into slots[T] = block * block_size + offset (< 0 skips).
-// map: num_blocks * block_size ints of scratch, any contents; not needed for up to 256 tokens. fmt: 0 e4m3, 1 int8.
+// map: num_blocks * block_size ints of scratch, any contents; not needed for up to 2048 tokens and blocks of 64. fmt: 0 e4m3, 1 int8.
 MLF_API int mlf_kv_write_q8(void* cache, float* scale, int fmt, const void* k, const void* v, const long long* slots, int* map, long long T,
                             int Hkv, int block_size, int num_blocks, long long ldk, long long ldv, uint64_t stream) {
   if (T <= 0) return 0;
@@ -226,11 +263,14 @@ MLF_API int mlf_kv_write_q8(void* cache, float* scale, int fmt, const void* k, c
   p.k = static_cast<const __nv_bfloat16*>(k);
   p.v = static_cast<const __nv_bfloat16*>(v);
   p.slots = slots;
-  p.map = T > QW_FEW ? map : nullptr;
-  MLF_REQUIRE(T <= QW_FEW || map != nullptr, "kv_write_q8: %lld tokens need a map", T);
+  p.bs_shift = -1;
+  for (int sh = 0; sh < 31; ++sh) if ((1 << sh) == block_size) p.bs_shift = sh;
+  const bool few = T <= QW_FEW && block_size <= QW_ROWS;
+  MLF_REQUIRE(few || map != nullptr, "kv_write_q8: %lld tokens into blocks of %d need a map", T, block_size);
+  p.map = few ? nullptr : map;
   p.T = T; p.ldk = ldk; p.ldv = ldv;
   p.Hkv = Hkv; p.block_size = block_size; p.num_blocks = num_blocks;
-  p.group = T > QW_FEW ? QW_GROUP : 1;        // few tokens: often one to a block, and too few CTAs otherwise
+  p.group = T > 256 ? QW_GROUP : 1;           // few tokens: often one to a block, and too few CTAs otherwise
   p.err = device_status_word();
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (p.map != nullptr) MLF_CHECK_CUDA(launch_pdl(q8_map_kernel, dim3((unsigned)((T + 255) / 256)), dim3(256), 0, st, p));
@@ -249,12 +289,11 @@ MLF_API int mlf_kv_gather_q8(const void* cache, const float* scale, int fmt, con
   MLF_REQUIRE((long long)len <= (long long)table_len * block_size, "kv_gather_q8: %d tokens need more than the %d block-table entries given", len,
               table_len);
   MLF_REQUIRE((reinterpret_cast<uintptr_t>(cache) & 15) == 0, "kv_gather_q8: the cache must be 16-byte aligned");
-  long long g = ((long long)len * Hkv * (Q8_D / 16) + 255) / 256;
-  const long long cap = (long long)sm_count() * 8;
-  if (g > cap) g = cap;
+  MLF_REQUIRE((long long)len * Hkv < (1LL << 31), "kv_gather_q8: %d tokens of %d heads", len, Hkv);
+  const unsigned pairs = (unsigned)len * (unsigned)Hkv, g = (pairs + 32 * QG_PAIRS - 1) / (32 * QG_PAIRS);
   const auto kernel = fmt == Q8_E4M3 ? q8_gather_kernel<Q8_E4M3> : q8_gather_kernel<Q8_INT8>;
-  MLF_CHECK_CUDA(launch_pdl(kernel, dim3((unsigned)g), dim3(256), 0, reinterpret_cast<cudaStream_t>(stream), static_cast<const uint8_t*>(cache), scale,
-                            block_table, len, Hkv, block_size, num_blocks, static_cast<__nv_bfloat16*>(out_k), static_cast<__nv_bfloat16*>(out_v),
+  MLF_CHECK_CUDA(launch_pdl(kernel, dim3(g), dim3(256), 0, reinterpret_cast<cudaStream_t>(stream), static_cast<const uint8_t*>(cache), scale,
+                            block_table, pairs, Hkv, block_size, num_blocks, static_cast<__nv_bfloat16*>(out_k), static_cast<__nv_bfloat16*>(out_v),
                             device_status_word()));
   count_launch();
   return 0;

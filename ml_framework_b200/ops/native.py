@@ -641,7 +641,7 @@ def kv_cache_write(kv_cache: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slo
         if T == 0 or kv_cache.numel() == 0:
             return
         nb, _, bs, Hkv, _ = kv_cache.shape
-        where = torch.empty(nb * bs, dtype=torch.int32, device=k.device) if T > 256 else None
+        where = torch.empty(nb * bs, dtype=torch.int32, device=k.device) if T > 2048 or bs > 64 else None
         rc = _function("mlf_kv_write_q8", "ppippppliiillu")(
             kv_cache.data_ptr(), kv_scale.data_ptr(), fmt, k.data_ptr(), v.data_ptr(), slots.data_ptr(), _at(where), T, Hkv, bs, nb,
             k.stride(0), v.stride(0), _stream())

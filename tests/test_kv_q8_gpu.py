@@ -35,7 +35,7 @@ def _gen(seed):
 
 # ------------------------------------------------------------------ writes
 @pytest.mark.parametrize("dtype", KINDS)
-@pytest.mark.parametrize("bs,Hkv", [(16, 8), (16, 1), (24, 3), (8, 2), (40, 5), (1, 2)])
+@pytest.mark.parametrize("bs,Hkv", [(16, 8), (16, 1), (24, 3), (8, 2), (40, 5), (1, 2), (72, 2)])
 @pytest.mark.parametrize("T", [1, 2, 15, 16, 17, 37, 255, 256, 300])
 def test_write_matches_the_statement(dtype, bs, Hkv, T):
     g = _gen(T * 100 + bs)
@@ -60,6 +60,12 @@ def test_write_matches_the_statement(dtype, bs, Hkv, T):
             native.kv_cache_write(c, k[order], v[order], slots[order], kv_scale=s)
         assert torch.equal(s, want_s)
         assert torch.equal(_bytes(c), _bytes(want_c))
+
+
+@pytest.mark.parametrize("bs,T", [(16, 2048), (16, 2049), (24, 2200), (72, 300), (72, 2100)])
+def test_long_writes(bs, T):
+    """Calls, and blocks, beyond what a CTA looks through."""
+    test_write_matches_the_statement(torch.int8, bs, 2, T)
 
 
 @pytest.mark.parametrize("dtype", KINDS)
