@@ -59,14 +59,43 @@ __device__ __forceinline__ int q8_token_at(const Q8WriteParams& p, long long slo
   return t >= 0 && t < p.T && p.slots[t] == slot ? t : -1;
 }
 
+// Eight bf16 numbers times inv in 8 bits. plain: no NaN, and none beyond the format.
+template <int FMT>
+__device__ __noinline__ uint2 q8_pack_any(uint4 x, float inv) {
+  const float2 a = unpack_bf16x2(x.x), b = unpack_bf16x2(x.y), e = unpack_bf16x2(x.z), f = unpack_bf16x2(x.w);
+  return make_uint2(q8_pack4<FMT>(a.x * inv, a.y * inv, b.x * inv, b.y * inv), q8_pack4<FMT>(e.x * inv, e.y * inv, f.x * inv, f.y * inv));
+}
+template <int FMT>
+__device__ __forceinline__ uint2 q8_pack8(uint4 x, float inv, bool plain) {
+  if (FMT == Q8_E4M3) {                       // the conversion minds NaN and the largest numbers itself
+    const float2 a = unpack_bf16x2(x.x), b = unpack_bf16x2(x.y), e = unpack_bf16x2(x.z), f = unpack_bf16x2(x.w);
+    return make_uint2(q8_pack4<FMT>(a.x * inv, a.y * inv, b.x * inv, b.y * inv), q8_pack4<FMT>(e.x * inv, e.y * inv, f.x * inv, f.y * inv));
+  }
+  if (!plain) return q8_pack_any<FMT>(x, inv);
+  // rounded by adding 1.5 * 2^23: the integer is the low byte of the sum (one instruction for a conversion's two, at four times its rate)
+  const unsigned w[4] = {x.x, x.y, x.z, x.w};
+  unsigned lo[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float2 f = unpack_bf16x2(w[j]);
+    lo[j] = __byte_perm(__float_as_uint(__fmaf_rn(f.x, inv, 12582912.f)), __float_as_uint(__fmaf_rn(f.y, inv, 12582912.f)), 0x0040);
+  }
+  return make_uint2(__byte_perm(lo[0], lo[1], 0x5410), __byte_perm(lo[2], lo[3], 0x5410));
+}
+template <int FMT>
+__device__ __noinline__ void q8_shrink8(uint2* at, float ratio) {
+  const uint2 held = *at;
+  *at = make_uint2(q8_shrink4<FMT>(held.x, ratio), q8_shrink4<FMT>(held.y, ratio));
+}
+
 // A block's rows of one head and side. known: the tokens of its rows (-1: not written by this call), the first 16 of them with a map.
 template <int FMT>
 __device__ __forceinline__ void q8_write_rows(const Q8WriteParams& p, int blk, int h, int side, const int* known) {
   const int lane = threadIdx.x & 31, half = lane >> 4, col = (lane & 15) * 8;
-  const long long first = (long long)blk * p.block_size;
+  const long long first = (long long)blk * p.block_size, pitch = (long long)p.Hkv * Q8_D;
   const __nv_bfloat16* src = (side ? p.v : p.k) + (long long)h * Q8_D + col;
   const long long ld = side ? p.ldv : p.ldk;
-  uint8_t* dst = p.cache + (((long long)blk * 2 + side) * p.block_size * p.Hkv + h) * Q8_D + col;
+  uint8_t* dst = p.cache + (((long long)blk * 2 + side) * p.block_size * p.Hkv + h) * Q8_D + col + half * pitch;
   float* scale = p.scale + ((long long)blk * 2 + side) * p.Hkv + h;
   const int chunks = (p.block_size + 15) / 16;
   uint4 x[8];
@@ -82,42 +111,37 @@ __device__ __forceinline__ void q8_write_rows(const Q8WriteParams& p, int blk, i
     }
   };
   const float held_scale = *scale;
-  float amax = 0.f;
+  // the largest magnitude, by its bits (a NaN's are above all others')
+  __nv_bfloat162 most = __float2bfloat162_rn(0.f), numbers = most;              // with NaN, and without
   bool anew = false;
   for (int c = 0; c < chunks; ++c) {
     load(c);
     if (c == 0) anew = __shfl_sync(0xffffffffu, tok, 0) >= 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const unsigned w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+      const unsigned w[4] = {x[i].x & 0x7fff7fffu, x[i].y & 0x7fff7fffu, x[i].z & 0x7fff7fffu, x[i].w & 0x7fff7fffu};
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float2 f = unpack_bf16x2(w[j]);
-        amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
+        most = __hmax2_nan(most, *reinterpret_cast<const __nv_bfloat162*>(&w[j]));
+        numbers = __hmax2(numbers, *reinterpret_cast<const __nv_bfloat162*>(&w[j]));
       }
     }
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  const unsigned with_nan = __reduce_max_sync(0xffffffffu, max(__float_as_uint(__low2float(most)), __float_as_uint(__high2float(most))));
+  const float amax = __uint_as_float(__reduce_max_sync(0xffffffffu, max(__float_as_uint(__low2float(numbers)), __float_as_uint(__high2float(numbers)))));
   const float fit = q8_scale_for<FMT>(amax), before = anew ? 0.f : held_scale;
   const float now = fmaxf(before, fit);
   const float inv = __frcp_rn(now), ratio = before * inv;     // exact for powers of two
-  const bool shrink = !anew && before < now;
+  const bool shrink = !anew && before < now, plain = with_nan <= 0x7f800000u && amax * inv <= 127.f;
   for (int c = 0; c < chunks; ++c) {
     if (chunks > 1) load(c);
+    uint8_t* to = dst + c * 16 * pitch;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const int row = c * 16 + 2 * i + half;
       const int t = __shfl_sync(0xffffffffu, tok, 2 * i + half);
-      if (row >= p.block_size) continue;
-      uint2* to = reinterpret_cast<uint2*>(dst + (long long)row * p.Hkv * Q8_D);
-      if (t >= 0) {
-        const float2 a = unpack_bf16x2(x[i].x), b = unpack_bf16x2(x[i].y), e = unpack_bf16x2(x[i].z), f = unpack_bf16x2(x[i].w);
-        *to = make_uint2(q8_pack4<FMT>(a.x * inv, a.y * inv, b.x * inv, b.y * inv), q8_pack4<FMT>(e.x * inv, e.y * inv, f.x * inv, f.y * inv));
-      } else if (shrink) {
-        const uint2 held = *to;
-        *to = make_uint2(q8_shrink4<FMT>(held.x, ratio), q8_shrink4<FMT>(held.y, ratio));
-      }
+      if (t >= 0) *reinterpret_cast<uint2*>(to) = q8_pack8<FMT>(x[i], inv, plain);
+      else if (shrink && c * 16 + 2 * i + half < p.block_size) q8_shrink8<FMT>(reinterpret_cast<uint2*>(to), ratio);
+      to += 2 * pitch;
     }
   }
   if (lane == 0) *scale = now;
@@ -126,7 +150,7 @@ __device__ __forceinline__ void q8_write_rows(const Q8WriteParams& p, int blk, i
 // A CTA looks at the blocks of `group` tokens and writes those whose first row, of the rows that the call writes there, one of these
 // tokens is; the heads and sides are split over blockIdx.y.
 template <int FMT>
-__global__ void __launch_bounds__(QW_WARPS * 32) q8_write_kernel(const Q8WriteParams p) {
+__global__ void __launch_bounds__(QW_WARPS * 32, 4) q8_write_kernel(const Q8WriteParams p) {
   __shared__ int s_blk[QW_GROUP], s_tok[QW_GROUP][QW_ROWS], s_blocks;
   pdl_trigger();
   pdl_wait();
@@ -147,12 +171,19 @@ __global__ void __launch_bounds__(QW_WARPS * 32) q8_write_kernel(const Q8WritePa
     for (int i = tid; i < QW_GROUP * QW_ROWS; i += QW_WARPS * 32) (&s_tok[0][0])[i] = 0x7fffffff;
     __syncthreads();
     const int n = s_blocks;
-    for (int t = tid; t < p.T; t += QW_WARPS * 32) {
-      const long long slot = p.slots[t];
-      if (slot < 0 || slot >= end) continue;
-      const int blk = q8_block(p, slot);
-      for (int i = 0; i < n; ++i)
-        if (s_blk[i] == blk) atomicMin(&s_tok[i][slot - (long long)blk * p.block_size], t);       // a slot that is given twice: the lower token
+    constexpr int EACH = QW_FEW / (QW_WARPS * 32);
+    long long slots[EACH];
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) {
+      const int t = tid + j * QW_WARPS * 32;
+      slots[j] = t < p.T ? p.slots[t] : -1;
+    }
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) {
+      if (slots[j] < 0 || slots[j] >= end) continue;
+      const int blk = q8_block(p, slots[j]);
+      for (int i = 0; i < n; ++i)      // a slot that is given twice: the lower token
+        if (s_blk[i] == blk) atomicMin(&s_tok[i][slots[j] - (long long)blk * p.block_size], tid + j * QW_WARPS * 32);
     }
     __syncthreads();
     for (int i = warp; i < n; i += QW_WARPS) {
@@ -195,9 +226,10 @@ __global__ void __launch_bounds__(QW_WARPS * 32) q8_write_kernel(const Q8WritePa
 }
 static_assert(QW_GROUP <= 32, "a lane for every token of a group");
 
-// out_k / out_v [len, Hkv, 128] bf16 <- pages of one sequence; eight threads a token and head, 16 numbers of its key and of its value
-// each, of two such pairs at a time.
-constexpr int QG_PAIRS = 2;
+// out_k / out_v [len, Hkv, 128] bf16 <- pages of one sequence; sixteen threads a token and head, eight numbers of its key and of its
+// value each (16 bytes out: with sixteen numbers a thread, every store left half of its sectors to the next one), of four such
+// pairs at a time.
+constexpr int QG_PAIRS = 4;
 template <int FMT>
 __global__ void __launch_bounds__(256)
 q8_gather_kernel(const uint8_t* cache, const float* scale, const int* block_table, unsigned pairs, int Hkv, int block_size, int num_blocks,
@@ -205,39 +237,41 @@ q8_gather_kernel(const uint8_t* cache, const float* scale, const int* block_tabl
   pdl_trigger();
   pdl_wait();
   const long long side = (long long)block_size * Hkv * Q8_D;
-  const unsigned first = blockIdx.x * (32 * QG_PAIRS) + (threadIdx.x >> 3), c = (threadIdx.x & 7) * 16;
-  uint4 k[QG_PAIRS], v[QG_PAIRS];
+  const unsigned first = blockIdx.x * (16 * QG_PAIRS) + (threadIdx.x >> 4), c = (threadIdx.x & 15) * 8;
+  uint2 k[QG_PAIRS], v[QG_PAIRS];
   float sk[QG_PAIRS], sv[QG_PAIRS];
+  int blk[QG_PAIRS];
+  bool bad = false;
 #pragma unroll
   for (int e = 0; e < QG_PAIRS; ++e) {
-    const unsigned i = first + 32 * e;
-    if (i >= pairs) break;
-    const unsigned t = i / (unsigned)Hkv, h = i - t * Hkv, b = t / (unsigned)block_size;
-    int blk = block_table[b];
-    if (blk < 0 || blk >= num_blocks) { atomicCAS(err, 0, ERR_BAD_INDEX); blk = 0; }
-    const uint8_t* src = cache + 2 * side * blk + ((long long)(t - b * block_size) * Hkv + h) * Q8_D + c;
-    const float* s = scale + (long long)blk * 2 * Hkv + h;
-    k[e] = *reinterpret_cast<const uint4*>(src);
-    v[e] = *reinterpret_cast<const uint4*>(src + side);
-    sk[e] = s[0];
-    sv[e] = s[Hkv];
+    const unsigned i = first + 16 * e;
+    blk[e] = i < pairs ? block_table[i / (unsigned)Hkv / (unsigned)block_size] : 0;
+  }
+#pragma unroll
+  for (int e = 0; e < QG_PAIRS; ++e) bad = bad || blk[e] < 0 || blk[e] >= num_blocks;
+  if (bad) atomicCAS(err, 0, ERR_BAD_INDEX);
+#pragma unroll
+  for (int e = 0; e < QG_PAIRS; ++e) {
+    const unsigned i = first + 16 * e;
+    if (i < pairs) {
+      const unsigned t = i / (unsigned)Hkv, h = i - t * Hkv, b = t / (unsigned)block_size;
+      if (blk[e] < 0 || blk[e] >= num_blocks) blk[e] = 0;
+      const uint8_t* src = cache + 2 * side * blk[e] + ((long long)(t - b * block_size) * Hkv + h) * Q8_D + c;
+      const float* s = scale + (long long)blk[e] * 2 * Hkv + h;
+      k[e] = *reinterpret_cast<const uint2*>(src);
+      v[e] = *reinterpret_cast<const uint2*>(src + side);
+      sk[e] = s[0];
+      sv[e] = s[Hkv];
+    }
   }
 #pragma unroll
   for (int e = 0; e < QG_PAIRS; ++e) {
-    const unsigned i = first + 32 * e;
-    if (i >= pairs) break;
-    auto put = [&](uint4 q, float f, __nv_bfloat16* out) {
-      const unsigned w[4] = {q.x, q.y, q.z, q.w};
-      unsigned o[8];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float4 a = q8_floats<FMT>(w[j]);
-        o[2 * j] = pack_bf16x2(a.x * f, a.y * f);
-        o[2 * j + 1] = pack_bf16x2(a.z * f, a.w * f);
-      }
-      uint4* d = reinterpret_cast<uint4*>(out + (long long)i * Q8_D + c);
-      d[0] = make_uint4(o[0], o[1], o[2], o[3]);
-      d[1] = make_uint4(o[4], o[5], o[6], o[7]);
+    const unsigned i = first + 16 * e;
+    if (i >= pairs) continue;
+    auto put = [&](uint2 q, float f, __nv_bfloat16* out) {
+      const float4 a = q8_floats<FMT>(q.x), b = q8_floats<FMT>(q.y);
+      *reinterpret_cast<uint4*>(out + (long long)i * Q8_D + c) =
+          make_uint4(pack_bf16x2(a.x * f, a.y * f), pack_bf16x2(a.z * f, a.w * f), pack_bf16x2(b.x * f, b.y * f), pack_bf16x2(b.z * f, b.w * f));
     };
     put(k[e], sk[e], out_k);
     put(v[e], sv[e], out_v);
@@ -274,7 +308,9 @@ MLF_API int mlf_kv_write_q8(void* cache, float* scale, int fmt, const void* k, c
   p.err = device_status_word();
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (p.map != nullptr) MLF_CHECK_CUDA(launch_pdl(q8_map_kernel, dim3((unsigned)((T + 255) / 256)), dim3(256), 0, st, p));
-  const dim3 grid((unsigned)((T + p.group - 1) / p.group), (unsigned)((2 * Hkv + QW_WARPS - 1) / QW_WARPS));
+  // a CTA finds its blocks once for all heads that it takes: about as many of them as fit, four to an SM
+  const long long x = (T + p.group - 1) / p.group, most = (2 * Hkv + QW_WARPS - 1) / QW_WARPS, fill = 4LL * sm_count() / x > 0 ? 4LL * sm_count() / x : 1;
+  const dim3 grid((unsigned)x, (unsigned)(fill < most ? fill : most));
   const auto kernel = fmt == Q8_E4M3 ? q8_write_kernel<Q8_E4M3> : q8_write_kernel<Q8_INT8>;
   MLF_CHECK_CUDA(launch_pdl(kernel, grid, dim3(QW_WARPS * 32), 0, st, p));
   count_launch(p.map != nullptr ? 2 : 1);
@@ -290,7 +326,7 @@ MLF_API int mlf_kv_gather_q8(const void* cache, const float* scale, int fmt, con
               table_len);
   MLF_REQUIRE((reinterpret_cast<uintptr_t>(cache) & 15) == 0, "kv_gather_q8: the cache must be 16-byte aligned");
   MLF_REQUIRE((long long)len * Hkv < (1LL << 31), "kv_gather_q8: %d tokens of %d heads", len, Hkv);
-  const unsigned pairs = (unsigned)len * (unsigned)Hkv, g = (pairs + 32 * QG_PAIRS - 1) / (32 * QG_PAIRS);
+  const unsigned pairs = (unsigned)len * (unsigned)Hkv, g = (pairs + 16 * QG_PAIRS - 1) / (16 * QG_PAIRS);
   const auto kernel = fmt == Q8_E4M3 ? q8_gather_kernel<Q8_E4M3> : q8_gather_kernel<Q8_INT8>;
   MLF_CHECK_CUDA(launch_pdl(kernel, dim3(g), dim3(256), 0, reinterpret_cast<cudaStream_t>(stream), static_cast<const uint8_t*>(cache), scale,
                             block_table, pairs, Hkv, block_size, num_blocks, static_cast<__nv_bfloat16*>(out_k), static_cast<__nv_bfloat16*>(out_v),

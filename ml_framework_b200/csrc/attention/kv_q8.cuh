@@ -29,17 +29,19 @@ __device__ __forceinline__ float q8_scale_for(float amax) {
   return __uint_as_float((unsigned)(x + 127) << 23);
 }
 
-// Two numbers (already divided by their scale) rounded to 8 bits, the first one in the low byte. Magnitudes beyond the
-// largest become the largest; a NaN stays one in e4m3 and becomes 0 in int8.
-template <int FMT>
-__device__ __forceinline__ unsigned q8_pack2(float a, float b) {
-  if (FMT == Q8_E4M3) return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
-  const int x = max(-127, min(127, __float2int_rn(a))), y = max(-127, min(127, __float2int_rn(b)));
-  return (unsigned)(x & 0xff) | (unsigned)(y & 0xff) << 8;
-}
+// Numbers (already divided by their scale) rounded to 8 bits, the first one in the low byte. Magnitudes beyond the largest become the
+// largest; a NaN stays one in e4m3 and becomes 0 in int8.
 template <int FMT>
 __device__ __forceinline__ unsigned q8_pack4(float a, float b, float c, float d) {
-  return q8_pack2<FMT>(a, b) | q8_pack2<FMT>(c, d) << 16;
+  if (FMT == Q8_E4M3)
+    return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3) | (unsigned)__nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3) << 16;
+  // conversion and packing saturate above, the comparison below (-128 is no number of the format)
+  int x = __float2int_rn(a), y = __float2int_rn(b), z = __float2int_rn(c), w = __float2int_rn(d);
+  x = max(x, -127); y = max(y, -127); z = max(z, -127); w = max(w, -127);
+  unsigned hi, all;
+  asm("cvt.pack.sat.s8.s32.b32 %0, %1, %2, 0;" : "=r"(hi) : "r"(w), "r"(z));
+  asm("cvt.pack.sat.s8.s32.b32 %0, %1, %2, %3;" : "=r"(all) : "r"(y), "r"(x), "r"(hi));
+  return all;
 }
 
 // The four numbers of a word as two f16 pairs, (byte 0, byte 1) and (byte 2, byte 3): every one of both types is exact in f16.
