@@ -61,12 +61,13 @@ copy_blocks_kernel(const __grid_constant__ CopyBlocksParams p, unsigned chunk) {
 
 using namespace mlf;
 
-// bases / block_bytes: n_tensors tensors of num_blocks blocks each; pairs: n_pairs (src, dst) block numbers on the host. A block
+// bases / bytes: n_tensors tensors of num_blocks blocks each, and how large they are; pairs: n_pairs (src, dst) block numbers on the host. A block
 // is written at most once and not read where it is written, so that the order of the copies does not matter.
-MLF_API int mlf_kv_copy_blocks(void* const* bases, const long long* block_bytes, int n_tensors, const int* pairs, int n_pairs, int num_blocks,
+MLF_API int mlf_kv_copy_blocks(void* const* bases, const long long* bytes, int n_tensors, const int* pairs, int n_pairs, int num_blocks,
                                uint64_t stream) {
   MLF_REQUIRE(n_tensors >= 0 && n_pairs >= 0 && num_blocks >= 0, "kv_copy_blocks: negative counts");
   if (n_tensors == 0 || n_pairs == 0) return 0;
+  MLF_REQUIRE(num_blocks > 0, "kv_copy_blocks: no blocks");
   std::vector<unsigned char> role;
   try {
     role.assign(num_blocks, 0);
@@ -83,7 +84,7 @@ MLF_API int mlf_kv_copy_blocks(void* const* bases, const long long* block_bytes,
   for (int i = 0; i < n_pairs; ++i)
     MLF_REQUIRE(!(role[pairs[2 * i + 1]] & 1), "kv_copy_blocks: block %d is both read and written", pairs[2 * i + 1]);
   for (int t = 0; t < n_tensors; ++t)
-    MLF_REQUIRE(block_bytes[t] > 0 && block_bytes[t] < (1LL << 31), "kv_copy_blocks: blocks of %lld bytes", block_bytes[t]);
+    MLF_REQUIRE(bytes[t] > 0 && bytes[t] % num_blocks == 0 && bytes[t] / num_blocks < (1LL << 31), "kv_copy_blocks: %d blocks in %lld bytes", num_blocks, bytes[t]);
   const unsigned chunk = CB_THREADS * CB_VECS * 16;
   for (int t0 = 0; t0 < n_tensors; t0 += CB_TENSORS) {
     const int nt = n_tensors - t0 < CB_TENSORS ? n_tensors - t0 : CB_TENSORS;
@@ -91,8 +92,8 @@ MLF_API int mlf_kv_copy_blocks(void* const* bases, const long long* block_bytes,
     long long most = 0;
     for (int t = 0; t < nt; ++t) {
       p.base[t] = static_cast<char*>(bases[t0 + t]);
-      p.bytes[t] = (unsigned)block_bytes[t0 + t];
-      most = most > block_bytes[t0 + t] ? most : block_bytes[t0 + t];
+      p.bytes[t] = (unsigned)(bytes[t0 + t] / num_blocks);
+      most = most > p.bytes[t] ? most : p.bytes[t];
     }
     for (int i0 = 0; i0 < n_pairs; i0 += CB_PAIRS) {
       const int np = n_pairs - i0 < CB_PAIRS ? n_pairs - i0 : CB_PAIRS;
