@@ -35,8 +35,7 @@ namespace mlf {
 
 namespace cg = cooperative_groups;
 
-constexpr int DQ_WARPS = 4;
-constexpr int DQ_THREADS = DQ_WARPS * 32;
+constexpr int DQ_WARPS = 4;                                  // at most
 constexpr int DQ_TILE = 16;                                  // tokens
 constexpr int DQ_PAIR = 2;                                   // tiles that a warp works on at once
 constexpr int DQ_STAGES = 2;                                 // pairs in flight per warp
@@ -44,7 +43,7 @@ constexpr int DQ_TILE_BYTES = 2 * DQ_TILE * Q8_D + 128;      // keys, values, 16
 constexpr int DQ_STAGE_BYTES = DQ_PAIR * DQ_TILE_BYTES;
 constexpr int DQ_SMEM = DQ_WARPS * DQ_STAGES * DQ_STAGE_BYTES;
 constexpr int DQ_BOX_STAGE = DQ_PAIR * 2 * DQ_TILE * Q8_D;   // of the TMA form: scales stay in registers
-constexpr int DQ_BOX_SMEM = DQ_WARPS * DQ_STAGES * DQ_BOX_STAGE + 1024;
+constexpr int dq_box_smem(int warps) { return warps * DQ_STAGES * DQ_BOX_STAGE + 1024; }
 constexpr float DQ_UP = 15.f;                                // log2 of the largest weight
 constexpr int DQ_CLUSTER = 8;                                // splits that a cluster merges
 constexpr int DQ_RED = Q8_D + 2;                             // floats of a partial result: maximum, sum, output
@@ -137,13 +136,13 @@ __device__ __forceinline__ unsigned q8_append_row(const DecodeQ8Params& p, float
 }
 
 // NT: tiles of eight query heads (the group's heads, zero-padded).
-// WHOLE: blocks of a multiple of 16 tokens, so that a tile lies in one.
-template <int FMT, int NT, bool ROPE, bool WHOLE>
-__global__ void __launch_bounds__(DQ_THREADS)
+// WHOLE: blocks of a multiple of 16 tokens, so that a tile lies in one. W: warps of a CTA.
+template <int FMT, int NT, bool ROPE, bool WHOLE, int W>
+__global__ void __launch_bounds__(W * 32, NT == 1 ? 12 / W : 2)
 paged_decode_q8_kernel(const DecodeQ8Params p, const __grid_constant__ CUtensorMap tm) {
   extern __shared__ __align__(128) uint8_t dq_raw[];
   uint8_t* dq_smem = WHOLE ? dq_raw + (1024 - (smem_u32(dq_raw) & 1023)) % 1024 : dq_raw;      // swizzled boxes start on 1024 bytes
-  __shared__ __align__(8) uint64_t s_full[DQ_WARPS * DQ_STAGES];
+  __shared__ __align__(8) uint64_t s_full[W * DQ_STAGES];
   __shared__ int s_abort;
   __shared__ __align__(16) uint8_t s_new[2][Q8_D];
   __shared__ float s_new_scale[2];
@@ -155,7 +154,7 @@ paged_decode_q8_kernel(const DecodeQ8Params p, const __grid_constant__ CUtensorM
       s_abort = 0;
       tma_prefetch_desc(&tm);
     }
-    if (threadIdx.x < DQ_WARPS * DQ_STAGES) mbar_init(smem_u32(&s_full[threadIdx.x]), 1);
+    if (threadIdx.x < W * DQ_STAGES) mbar_init(smem_u32(&s_full[threadIdx.x]), 1);
     mbar_fence_init();
     __syncthreads();
   }
@@ -175,12 +174,12 @@ paged_decode_q8_kernel(const DecodeQ8Params p, const __grid_constant__ CUtensorM
   const int t_lo = min(len, sp * per), t_hi = min(len, t_lo + per);
   float* ws = p.ws ? p.ws + (((long long)b * p.Hkv + hkv) * p.splits + sp) * p.G * DQ_RED : nullptr;
   // behind the warps' partial results in shared memory: this CTA's, for the others of its cluster
-  float* mine_out = reinterpret_cast<float*>(dq_smem) + DQ_WARPS * p.G * DQ_RED;
+  float* mine_out = reinterpret_cast<float*>(dq_smem) + W * p.G * DQ_RED;
   // The splits of a sequence and KV head are the CTAs of a cluster: each merges a part of the output from all of them.
   auto merge_cluster = [&]() {
     cg::cluster_group cl = cg::this_cluster();
     cl.sync();
-    for (int i = sp * DQ_THREADS + tid; i < p.G * Q8_D; i += p.splits * DQ_THREADS) {
+    for (int i = sp * (W * 32) + tid; i < p.G * Q8_D; i += p.splits * (W * 32)) {
       const int at = i / Q8_D * DQ_RED, d = i % Q8_D;
       float m[DQ_CLUSTER], M = -INFINITY, L = 0.f, acc = 0.f;
 #pragma unroll
@@ -204,12 +203,12 @@ paged_decode_q8_kernel(const DecodeQ8Params p, const __grid_constant__ CUtensorM
   if (t_lo >= t_hi) {
     if (early) pdl_wait();
     if (ws) {
-      for (int i = tid; i < p.G * DQ_RED; i += DQ_THREADS) ws[i] = i % DQ_RED == 0 ? -INFINITY : 0.f;
+      for (int i = tid; i < p.G * DQ_RED; i += (W * 32)) ws[i] = i % DQ_RED == 0 ? -INFINITY : 0.f;
     } else if (p.splits > 1) {
-      for (int i = tid; i < p.G * DQ_RED; i += DQ_THREADS) mine_out[i] = i % DQ_RED == 0 ? -INFINITY : 0.f;
+      for (int i = tid; i < p.G * DQ_RED; i += (W * 32)) mine_out[i] = i % DQ_RED == 0 ? -INFINITY : 0.f;
       merge_cluster();
     } else {
-      for (int i = tid; i < p.G * Q8_D; i += DQ_THREADS) p.out[((long long)b * p.Hq + hkv * p.G) * Q8_D + i] = __float2bfloat16(0.f);
+      for (int i = tid; i < p.G * Q8_D; i += (W * 32)) p.out[((long long)b * p.Hq + hkv * p.G) * Q8_D + i] = __float2bfloat16(0.f);
     }
     return;
   }
@@ -217,7 +216,7 @@ paged_decode_q8_kernel(const DecodeQ8Params p, const __grid_constant__ CUtensorM
   const long long v_off = (long long)p.block_size * p.Hkv * Q8_D, blk_bytes = 2 * v_off;
   constexpr int SPAN = DQ_PAIR * DQ_TILE;
   const int pairs = (t_hi - t_lo + SPAN - 1) / SPAN;
-  const int mine = pairs > warp ? (pairs - warp + DQ_WARPS - 1) / DQ_WARPS : 0;      // pairs of tiles warp, warp + 4, ...
+  const int mine = pairs > warp ? (pairs - warp + W - 1) / W : 0;      // pairs of tiles warp, warp + 4, ...
   constexpr int STAGE = WHOLE ? DQ_BOX_STAGE : DQ_STAGE_BYTES, TILE_BYTES = STAGE / DQ_PAIR;
   uint8_t* ring_p = dq_smem + warp * DQ_STAGES * STAGE;
   const uint32_t ring = smem_u32(ring_p), full = smem_u32(&s_full[warp * DQ_STAGES]);
@@ -237,12 +236,12 @@ paged_decode_q8_kernel(const DecodeQ8Params p, const __grid_constant__ CUtensorM
   float scales[2][2];
   scales[0][0] = scales[0][1] = scales[1][0] = scales[1][1] = 1.f;
   auto issue = [&](int i) {                    // this warp's i-th pair
-    const int first = t_lo + (warp + i * DQ_WARPS) * SPAN;
+    const int first = t_lo + (warp + i * W) * SPAN;
     const uint32_t st = ring + (i % DQ_STAGES) * STAGE;
     if (WHOLE) {
       if ((i & ~15) != pages_from) {
         pages_from = i & ~15;
-        const int t = t_lo + (warp + (pages_from + (lane >> 1)) * DQ_WARPS) * SPAN + (lane & 1) * DQ_TILE;
+        const int t = t_lo + (warp + (pages_from + (lane >> 1)) * W) * SPAN + (lane & 1) * DQ_TILE;
         pages = t < t_hi ? checked(bt[block_of(t)]) : 0;
         const float* sc = p.scale + (long long)pages * 2 * p.Hkv + hkv;
         const float sk = t < t_hi ? sc[0] : 1.f, sv = t < t_hi ? sc[p.Hkv] : 1.f;
@@ -294,7 +293,7 @@ paged_decode_q8_kernel(const DecodeQ8Params p, const __grid_constant__ CUtensorM
     const int row = 2 * c + (j & 1) + 8 * (j >> 1);
     return DQ_TILE * Q8_D + (WHOLE ? row * Q8_D + ((g ^ (row & 7)) << 4) : j * 512 + lane * 16);
   };
-  auto late = [&](int i) { return has_new && t_lo + (warp + i * DQ_WARPS) * SPAN + SPAN > held_back; };
+  auto late = [&](int i) { return has_new && t_lo + (warp + i * W) * SPAN + SPAN > held_back; };
 #pragma unroll
   for (int i = 0; i < DQ_STAGES; ++i) {
     if (i < mine && !late(i)) issue(i);
@@ -408,7 +407,7 @@ paged_decode_q8_kernel(const DecodeQ8Params p, const __grid_constant__ CUtensorM
 #pragma unroll
     for (int h = 0; h < DQ_PAIR; ++h) {
       uint8_t* st = stage + h * TILE_BYTES;
-      const int t0 = t_lo + (warp + i * DQ_WARPS) * SPAN + h * DQ_TILE;
+      const int t0 = t_lo + (warp + i * W) * SPAN + h * DQ_TILE;
       float vs[2];
       if (WHOLE) {
         const bool odd = (i >> 4) & 1;
@@ -513,7 +512,7 @@ paged_decode_q8_kernel(const DecodeQ8Params p, const __grid_constant__ CUtensorM
       uint4 v[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const uint4*>(st + value_at(j));
-      const int left = t_hi - (t_lo + (warp + i * DQ_WARPS) * SPAN + h * DQ_TILE);
+      const int left = t_hi - (t_lo + (warp + i * W) * SPAN + h * DQ_TILE);
       if (WHOLE && left < DQ_TILE) {           // rows behind the sequence hold anything, and 0 times a NaN is one
 #pragma unroll
         for (int j = 0; j < 4; ++j)
@@ -560,15 +559,15 @@ paged_decode_q8_kernel(const DecodeQ8Params p, const __grid_constant__ CUtensorM
       }
     }
   __syncthreads();
-  for (int i = tid; i < p.G * Q8_D; i += DQ_THREADS) {
+  for (int i = tid; i < p.G * Q8_D; i += (W * 32)) {
     const int h = i / Q8_D, d = i % Q8_D;
     float M = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < DQ_WARPS; ++w) M = fmaxf(M, red[(w * p.G + h) * DQ_RED]);
+    for (int w = 0; w < W; ++w) M = fmaxf(M, red[(w * p.G + h) * DQ_RED]);
     const float M_use = M == -INFINITY ? 0.f : M;
     float acc = 0.f, l = 0.f;
 #pragma unroll
-    for (int w = 0; w < DQ_WARPS; ++w) {
+    for (int w = 0; w < W; ++w) {
       const float* r = red + (w * p.G + h) * DQ_RED;
       const float f = exp2f(r[0] - M_use);     // a warp without tokens has m = -inf, l = 0, o = 0
       acc += f * r[2 + d];
@@ -584,7 +583,8 @@ paged_decode_q8_kernel(const DecodeQ8Params p, const __grid_constant__ CUtensorM
   }
   if (p.splits > 1 && ws == nullptr) merge_cluster();
 }
-static_assert((DQ_WARPS + 1) * 16 * DQ_RED * 4 + 1024 <= DQ_BOX_SMEM && (DQ_WARPS + 1) * 16 * DQ_RED * 4 <= DQ_SMEM, "partial results of 16 heads fit the rings");
+static_assert((2 + 1) * 8 * DQ_RED * 4 <= 2 * DQ_STAGES * DQ_BOX_STAGE && (DQ_WARPS + 1) * 16 * DQ_RED * 4 <= DQ_WARPS * DQ_STAGES * DQ_BOX_STAGE,
+              "partial results of 8 heads (of 16: four warps) fit the rings");
 
 // out = sum_s exp2(m_s - M) o_s / sum_s exp2(m_s - M) l_s over the splits of a sequence and head. The splits' factors first, one a
 // thread, so that the loop over their outputs has nothing but loads in it, eight at a time.
@@ -639,12 +639,12 @@ using namespace mlf;
 // One query token per sequence over an 8-bit cache. Without slots: q [B, Hq, 128], row pitch ldq. With slots (the packed form): q is
 // the QKV product [B, (Hq + 2 Hkv) * 128], not yet rotated; the newest token of a sequence, the last of its seq_lens, is rotated at
 // position seq_lens - 1, written to its slot (< 0: not written) as mlf_kv_write_q8 would and attended to like the cached ones.
-// fmt: 0 e4m3, 1 int8. ws: B * Hq * splits * 130 floats (ws_elems: what is there) for splits that a second kernel merges; without it
+// max_seq_len: an upper bound of seq_lens, for the launch's shape alone. fmt: 0 e4m3, 1 int8. ws: B * Hq * splits * 130 floats (ws_elems: what is there) for splits that a second kernel merges; without it
 // up to 8 are merged by clusters of the launch, which is faster where all of them are resident at once (a 4-split launch of 24 x
 // 900 tokens of 40 heads, nine rounds: 67 us, 49 with ws). inputs_static: as for mlf_paged_decode_rope.
 MLF_API int mlf_paged_decode_q8(const void* q, long long ldq, void* cache, float* scale, int fmt, const int* block_table, const int* seq_lens,
                                 const long long* slots, void* out, float* ws, long long ws_elems, int B, int Hq, int Hkv, int block_size, int max_blocks,
-                                int num_blocks, int splits, float softmax_scale, float theta, int inputs_static, uint64_t stream) {
+                                int num_blocks, int max_seq_len, int splits, float softmax_scale, float theta, int inputs_static, uint64_t stream) {
   if (B <= 0) return 0;
   MLF_REQUIRE(fmt == Q8_E4M3 || fmt == Q8_INT8, "paged_decode_q8: format %d", fmt);
   MLF_REQUIRE(Hkv > 0 && Hq > 0 && Hq % Hkv == 0, "paged_decode_q8: bad head counts %d, %d", Hq, Hkv);
@@ -669,7 +669,7 @@ MLF_API int mlf_paged_decode_q8(const void* q, long long ldq, void* cache, float
   p.ws = second ? ws : nullptr;
   p.B = B; p.Hq = Hq; p.Hkv = Hkv; p.G = G; p.block_size = block_size; p.max_blocks = max_blocks; p.num_blocks = num_blocks;
   p.splits = splits;
-  p.unit = block_size * ((DQ_WARPS * DQ_TILE + block_size - 1) / block_size);
+  p.unit = block_size * ((64 + block_size - 1) / block_size);
   p.bs_shift = -1;
   for (int sh = 0; sh < 31; ++sh) if ((1 << sh) == block_size) p.bs_shift = sh;
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
@@ -679,30 +679,36 @@ MLF_API int mlf_paged_decode_q8(const void* q, long long ldq, void* cache, float
   p.slots = slots;
   p.theta = theta;
   p.early = inputs_static;
-#define DQ_KERNELS(FMT, NT) \
-  {{paged_decode_q8_kernel<FMT, NT, false, false>, paged_decode_q8_kernel<FMT, NT, false, true>}, \
-   {paged_decode_q8_kernel<FMT, NT, true, false>, paged_decode_q8_kernel<FMT, NT, true, true>}}
-  void (*const kernels[2][2][2][2])(DecodeQ8Params, CUtensorMap) = {{DQ_KERNELS(Q8_E4M3, 1), DQ_KERNELS(Q8_E4M3, 2)}, {DQ_KERNELS(Q8_INT8, 1), DQ_KERNELS(Q8_INT8, 2)}};
-#undef DQ_KERNELS
   const long long cache_rows = 2LL * num_blocks * block_size;
-  const int nt = G > 8 ? 1 : 0, whole = block_size % DQ_TILE == 0 && cache_rows < (1LL << 31) ? 1 : 0;
-  const int smem = whole ? DQ_BOX_SMEM : DQ_SMEM;
+  const bool whole = block_size % DQ_TILE == 0 && cache_rows < (1LL << 31);
+  // Warps of a CTA: four, of which three CTAs fit an SM (a warp's ring is 16 KB), or with eight heads at most as many as bring all CTAs into
+  // one round: four CTAs of three, six of two. Two also where there are not more than two pairs of tiles. us with 4 / 3 / 2 warps: 512 CTAs
+  // of 576 tokens 19 / 16 / 19, 800 of 576 24 / 26 / 22, 2048 of 64 21 / 17 / 15, 2048 of 1024 82 / 83 / 84, 384 of 4096 60 / 66 / 81.
+  const long long ctas = (long long)B * Hkv * splits, sms = sm_count();
+  const int warps = !whole || G > 8 || ctas <= 3 * sms ? 4 : ctas <= 4 * sms ? 3 : ctas <= 6 * sms || max_seq_len <= 64LL * splits ? 2 : 4;
+  const int smem = whole ? dq_box_smem(warps) : DQ_SMEM;
   CUtensorMap tm = {};
   if (whole) {
     const int rc = make_tmap_2d(&tm, cache, 1, (uint64_t)Hkv * Q8_D, (uint64_t)cache_rows, (uint64_t)Hkv * Q8_D, Q8_D, DQ_TILE, true);
     if (rc) return rc;
   }
-  const auto kernel = kernels[fmt][nt][rope ? 1 : 0][whole];
-  static bool attr_set[64][16] = {};
+#define DQ_ROPE(FMT, NT, WHOLE, W) {paged_decode_q8_kernel<FMT, NT, false, WHOLE, W>, paged_decode_q8_kernel<FMT, NT, true, WHOLE, W>}
+#define DQ_KERNELS(FMT) {DQ_ROPE(FMT, 1, false, 4), DQ_ROPE(FMT, 2, false, 4), DQ_ROPE(FMT, 2, true, 4), DQ_ROPE(FMT, 1, true, 4), DQ_ROPE(FMT, 1, true, 3), DQ_ROPE(FMT, 1, true, 2)}
+  void (*const kernels[2][6][2])(DecodeQ8Params, CUtensorMap) = {DQ_KERNELS(Q8_E4M3), DQ_KERNELS(Q8_INT8)};
+#undef DQ_KERNELS
+#undef DQ_ROPE
+  const int form = !whole ? (G > 8 ? 1 : 0) : G > 8 ? 2 : 7 - warps;
+  const auto kernel = kernels[fmt][form][rope ? 1 : 0];
+  static bool attr_set[64][24] = {};
   int dev = 0;
   cudaGetDevice(&dev);
-  bool& set = attr_set[dev & 63][fmt * 8 + nt * 4 + (rope ? 2 : 0) + whole];
+  bool& set = attr_set[dev & 63][(fmt * 6 + form) * 2 + (rope ? 1 : 0)];
   if (!set) {
     MLF_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     set = true;
   }
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  MLF_CHECK_CUDA(launch_pdl_cluster(kernel, dim3(B, Hkv, splits), dim3(DQ_THREADS), smem, dim3(1, 1, second ? 1 : splits), st, p, tm));
+  MLF_CHECK_CUDA(launch_pdl_cluster(kernel, dim3(B, Hkv, splits), dim3(warps * 32), smem, dim3(1, 1, second ? 1 : splits), st, p, tm));
   count_launch();
   if (second) {
     MLF_CHECK_CUDA(launch_pdl(paged_decode_q8_merge_kernel, dim3((unsigned)(B * Hq)), dim3(Q8_D), 0, st, (const float*)ws, p.out, Hq, Hkv, G, splits));

@@ -525,9 +525,9 @@ def _decode_q8(what: str, q: torch.Tensor, ldq: int, Hq: int, kv_cache, kv_scale
     # maximum, sum and output of each split; up to eight that are resident at once are merged within the launch
     within = splits <= 8 and (splits == 1 or B * Hkv * splits <= 3 * sms)
     ws = None if within else torch.empty(B * Hq * splits * 130, dtype=torch.float32, device=q.device)
-    rc = _function("mlf_paged_decode_q8", "plppipppppliiiiiiiffiu")(
+    rc = _function("mlf_paged_decode_q8", "plppipppppliiiiiiiiffiu")(
         q.data_ptr(), ldq, kv_cache.data_ptr(), kv_scale.data_ptr(), fmt, table.data_ptr(), lens.data_ptr(), _at(slots), out.data_ptr(), _at(ws),
-        0 if ws is None else ws.numel(), B, Hq, Hkv, kv_cache.shape[2], table.shape[1], kv_cache.shape[0], splits,
+        0 if ws is None else ws.numel(), B, Hq, Hkv, kv_cache.shape[2], table.shape[1], kv_cache.shape[0], max_seq_len, splits,
         scale if scale is not None else 128 ** -0.5, theta, int(inputs_static), _stream())
     _lib.check(rc, "mlf_paged_decode_q8")
     return out

@@ -210,6 +210,29 @@ def test_attention_many_splits(dtype, split, bs, Hq):
 
 
 @pytest.mark.parametrize("dtype", KINDS)
+@pytest.mark.parametrize("B,n,Hq,Hkv", [(150, 333, 8, 4), (200, 300, 12, 4), (300, 60, 16, 8), (300, 130, 24, 8), (40, 100, 16, 8)])
+def test_attention_forms_of_the_launch(dtype, B, n, Hq, Hkv):
+    """Four, three and two warps to a CTA: as many as bring the CTAs into one round, and short sequences; then with the append."""
+    g = _gen(B)
+    lens = torch.randint(1, n + 1, (B,), generator=torch.Generator().manual_seed(B)).tolist()
+    lens[0] = n
+    table, nb = _tables(lens, 16, g)
+    cache, scale = _random_cache(nb, 16, Hkv, dtype, g)
+    scale = scale * 2.0 ** -4
+    q = torch.randn(B, Hq, D, device="cuda", generator=g).to(torch.bfloat16)
+    sl = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    want, tol = _exact(q, cache, scale, table, lens, D ** -0.5)
+    _check(native.paged_decode(q, cache, table, sl, n, split_tokens=0, kv_scale=scale), want, tol)
+    qkv = torch.randn(B, (Hq + 2 * Hkv) * D, device="cuda", generator=g).to(torch.bfloat16)
+    slots = table.gather(1, ((sl.long() - 1) // 16)[:, None])[:, 0].long() * 16 + (sl.long() - 1) % 16
+    a_c, a_s, rot = cache.clone(), scale.clone(), qkv.clone()
+    native.rope_kv_write_(rot, sl.long() - 1, slots, a_c, Hq, Hkv, 5e5, kv_scale=a_s)
+    want = native.paged_decode(rot[:, :Hq * D].view(B, Hq, D), a_c, table, sl, n, split_tokens=0, kv_scale=a_s)
+    got = native.paged_decode_rope(qkv, cache, table, sl, slots, Hq, Hkv, n, 5e5, kv_scale=scale)
+    assert torch.equal(got, want) and torch.equal(_bytes(cache), _bytes(a_c)) and torch.equal(scale, a_s)
+
+
+@pytest.mark.parametrize("dtype", KINDS)
 def test_attention_wide_ranges(dtype):
     """Scales 2^-40 to 2^40 side by side, queries of very different size, one key that takes all the weight."""
     lens, bs, Hkv, G = [300, 77], 16, 2, 4
