@@ -14,7 +14,7 @@
 // A cluster of CTAs takes a row, and each lane keeps its logits in shared memory where eight CTAs can (rows of more are read again in
 // every pass, from the caches): a pass costs its arithmetic and an exchange through distributed shared memory.
 // (1) Largest logit, and mean and variance of a sample.
-// (2) Where k limits the row, or a p under which few tokens are expected: the bins of equal width that hold the k (256) largest
+// (2) Where k limits the row, or a p under which few tokens are expected: the bins of equal width that hold the k (128) largest
 // of the maxima of eight neighbours hold at least as many tokens, and hardly more. These go to a list in one CTA, where the token
 // is decided: eight logits cost one comparison in both passes.
 // (3) Where p alone keeps many tokens: the weights of all of them in bins, and the deciding bin alone in the list.
@@ -43,7 +43,7 @@ constexpr int SM_BINS = 2048;
 constexpr int SM_GROUPS = 64;                  // sums of neighbouring bins that CTAs exchange
 constexpr int SM_COARSE = 512;                 // bins of the maxima
 constexpr int SM_LIST = 2048;                  // tokens that a list takes
-constexpr int SM_FEW = 256;                    // tokens that a p alone is expected to keep, where they are listed
+constexpr int SM_FEW = 128;                    // tokens that a p alone is expected to keep, where they are listed
 constexpr int SM_CLUSTER = 8;                  // CTAs per row, at most
 constexpr int SM_ONE = 40;                     // log2 of the weight of the largest logit
 
@@ -154,6 +154,9 @@ __device__ __forceinline__ u64 sm_block_scan(u64 v, SampleSmem& s, u64* total) {
   *total = all;
   return before + inc - v;
 }
+
+// Threads for each of n <= SM_THREADS tokens of a list: a power of two up to eight.
+__device__ __forceinline__ int sm_parts(int n) { return n <= SM_THREADS / 8 ? 8 : n <= SM_THREADS / 4 ? 4 : n <= SM_THREADS / 2 ? 2 : 1; }
 
 // Ascending sort of n entries (a power of two, up to SM_LIST) in shared memory.
 __device__ __forceinline__ void sm_sort(u64* a, int n) {
@@ -685,8 +688,8 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_rows_kernel(const Sample
     };
     bool open = true;
     // p alone: a normal distribution with this mean and variance has V exp((mean - m) / T + var / 2 T^2) of the largest logit's weight, and
-    // z standard deviations above the mean 256 tokens, below which all but the upper tail beyond z - sigma / T of that weight
-    // lies. Where that is more than p leaves out, 256 tokens will not do. Only the way depends on it, not the token.
+    // z standard deviations above the mean 128 tokens, below which all but the upper tail beyond z - sigma / T of that weight
+    // lies. Where that is more than p leaves out, 128 tokens will not do. Only the way depends on it, not the token.
     bool flat = false;
     if (!need_k && p.vocab > SM_LIST) {
       const float inv_t = __fdiv_rn(1.f, temp), t = sqrtf(2.f * __logf((float)p.vocab / SM_FEW));
@@ -721,41 +724,53 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_rows_kernel(const Sample
           u64 target = target_p;
           bool enough = true;
           if (n <= SM_THREADS) {
-            // a token per thread: what comes before it is counted and summed directly
+            // a token for every one to eight threads: what comes before it is counted and summed directly
+            const int parts = sm_parts(n), t = tid / parts, part = tid % parts;
             u64 mine = ~0ull, w = 0, before = 0;
             int ahead = 0;
             if (tid < n) {
-              mine = entry(tid);
-              w = weight(sm_entry_value(mine));
-              s.pair[tid] = make_ulonglong2(mine, w);
+              const u64 e = entry(tid);
+              s.pair[tid] = make_ulonglong2(e, weight(sm_entry_value(e)));
             }
             __syncthreads();
-            if (tid < n)
-              for (int j = 0; j < n; ++j) {
+            if (t < n) {
+              mine = s.pair[t].x;
+              w = s.pair[t].y;
+              for (int j = part; j < n; j += parts) {
                 const ulonglong2 o = s.pair[j];
                 if (o.x < mine) { ++ahead; before += o.y; }
               }
+            }
+            for (int o = 1; o < parts; o <<= 1) {
+              ahead += __shfl_xor_sync(0xffffffffu, ahead, o);
+              before += __shfl_xor_sync(0xffffffffu, before, o);
+            }
             if (need_p) {
               u64 all;
-              sm_block_scan(tid < n && ahead < n_k ? w : 0ull, s, &all);
+              sm_block_scan(t < n && part == 0 && ahead < n_k ? w : 0ull, s, &all);
               if (need_k) target = sm_reach(top_p, all);
               enough = all >= target;
             }
             // kept: what begins below the target, is among the first k and not below min_p; the first token always
-            const bool in = tid < n && ahead < n_k && (ahead == 0 || ((!need_p || before < target) && sm_entry_value(mine) >= least));
+            const bool in = t < n && ahead < n_k && (ahead == 0 || ((!need_p || before < target) && sm_entry_value(mine) >= least));
             __syncthreads();
-            if (tid < n) s.pair[tid] = make_ulonglong2(mine, in ? w : 0ull);
+            if (t < n && part == 0) s.pair[t].y = in ? w : 0ull;
             __syncthreads();
-            if (in && enough) {
-              u64 all = 0;
-              before = 0;
-              for (int j = 0; j < n; ++j) {
+            u64 all = 0;
+            before = 0;
+            if (t < n)
+              for (int j = part; j < n; j += parts) {
                 const ulonglong2 o = s.pair[j];
                 all += o.y;
                 before += (unsigned)o.x < (unsigned)mine ? o.y : 0;
               }
-              const u64 t = sm_above(u, all);
-              if (before < t && before + w >= t) finish((long long)(unsigned)mine, sm_entry_value(mine), all);
+            for (int o = 1; o < parts; o <<= 1) {
+              all += __shfl_xor_sync(0xffffffffu, all, o);
+              before += __shfl_xor_sync(0xffffffffu, before, o);
+            }
+            if (in && part == 0 && enough) {
+              const u64 goal = sm_above(u, all);
+              if (before < goal && before + w >= goal) finish((long long)(unsigned)mine, sm_entry_value(mine), all);
             }
           } else {
             constexpr int PER = SM_LIST / SM_THREADS;
@@ -866,20 +881,24 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_rows_kernel(const Sample
               for (int q = 0; q < C; ++q) *cl.map_shared_rank(&s.last, q) = e;
             };
             if (n <= SM_THREADS) {
-              u64 mine = ~0ull, w = 0, before = sp.w;
+              const int parts = sm_parts(n), t = tid / parts, part = tid % parts;
+              u64 mine = ~0ull, w = 0, before = 0;
               if (tid < n) {
-                mine = entry(tid);
-                w = weight(sm_entry_value(mine));
-                s.pair[tid] = make_ulonglong2(mine, w);
+                const u64 e = entry(tid);
+                s.pair[tid] = make_ulonglong2(e, weight(sm_entry_value(e)));
               }
               __syncthreads();
-              if (tid < n) {
-                for (int j = 0; j < n; ++j) {
+              if (t < n) {
+                mine = s.pair[t].x;
+                w = s.pair[t].y;
+                for (int j = part; j < n; j += parts) {
                   const ulonglong2 o = s.pair[j];
                   if (o.x < mine) before += o.y;
                 }
-                if (before < target_p && before + w >= target_p) last_one(mine);
               }
+              for (int o = 1; o < parts; o <<= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+              before += sp.w;
+              if (t < n && part == 0 && before < target_p && before + w >= target_p) last_one(mine);
             } else {
               int pow2 = 2 * SM_THREADS;
               while (pow2 < n) pow2 <<= 1;
