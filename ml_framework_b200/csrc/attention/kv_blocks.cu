@@ -2,7 +2,8 @@
 // and the moves of a compaction (bookkeeping in serving/block_manager.cpp). dst block <- src block, for every tensor and pair.
 //
 // Bound by HBM: a copied byte is read once and written once. The tensors' addresses and the pairs, which the host knows, are
-// kernel parameters: nothing is uploaded ahead of the launch, and a captured launch keeps its own.
+// kernel parameters: nothing is uploaded ahead of the launch, and a captured launch keeps its own. 700 blocks of 64 KB in 8 layers
+// 115 us (6.4 TB/s), one in each of 32 layers 1.8.
 #include <string.h>
 
 #include <new>

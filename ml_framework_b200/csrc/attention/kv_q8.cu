@@ -9,7 +9,8 @@
 // nothing at all, point at tokens of other slots.
 //
 // Bound by HBM in long calls (a row is read in 16 bits and written in 8), by the chain of loads slots - rows (slots - map - slots -
-// rows) in short ones. WRITE_FIGURES
+// rows) in short ones. us (floor at 6.54 TB/s): 37 tokens of 8 heads 5 (0.03), 2048 10 (1.9), 8192 17 (7.7), 4096 of 40 heads 40 (19).
+// The way back, q8_gather_kernel: 3159 tokens of 8 heads 5 - 7 (3.0), 8192 8 - 10 (7.7).
 #include "../common/host.h"
 #include "../common/ptx.cuh"
 #include "../mlf_api.h"

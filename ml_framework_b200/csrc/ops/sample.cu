@@ -11,8 +11,9 @@
 // their order, so that a row gives the same token in any batch and with any number of CTAs, and a border between
 // two tokens is as sharp as the weights themselves.
 //
-// A cluster of CTAs takes a row, and each lane keeps its logits in shared memory where eight CTAs can (rows of more are read again in
-// every pass, from the caches): a pass costs its arithmetic and an exchange through distributed shared memory.
+// A cluster of CTAs takes a row, and each lane keeps its logits in shared memory where four steps of 256 a warp are enough; rows of
+// more are read again in every pass, from the caches, and their lanes' maxima of eight neighbours are kept instead. A pass costs
+// its arithmetic and an exchange through distributed shared memory.
 // (1) Largest logit, and mean and variance of a sample.
 // (2) Where k limits the row, or a p under which few tokens are expected: the bins of equal width that hold the k (128) largest
 // of the maxima of eight neighbours hold at least as many tokens, and hardly more. These go to a list in one CTA, where the token
@@ -21,6 +22,10 @@
 // (4) Where a list is too long (many equal logits), the deciding value digit by digit over the row, 11 + 11 + 10 bits of the
 // order-preserving integer of a float.
 // (5) After (3), (4) or no limit: the token from sums of 256 neighbours.
+//
+// Bound by the chain of passes and exchanges for few rows and by the instructions of the weights for many (some 40 each, 150 a
+// logit in (3)). us for 1 / 256 rows of 128256 bf16 logits (floor 0.04 / 10): largest logit 3 / 18, k = 50 with p 10 / 44, no limit
+// 10 / 87, a p that keeps few 17 / 130 - 170, one that keeps thousands 27 / 220, rows of all kinds - / 139.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <float.h>
