@@ -96,6 +96,9 @@ __device__ __forceinline__ unsigned dq_half2(float a, float b) {
   return *reinterpret_cast<const unsigned*>(&h);
 }
 
+// Without a token the sum is 0 and so is the output; a NaN among the scores is one of the output too.
+__device__ __forceinline__ __nv_bfloat16 dq_quotient(float o, float l) { return __float2bfloat16(l == 0.f ? 0.f : o / l); }
+
 // The newest token's key (side 0: rotated) or value, in 8 bits: a warp, four elements a lane. Its block's scale is settled as a
 // cache write would (a block's first row starts it anew; a larger scale rounds the held rows again), and the row is written;
 // a row without a slot has a scale of its own. Returns the four bytes and the scale that they stand in.
@@ -200,7 +203,7 @@ paged_decode_q8_kernel(const DecodeQ8Params p, const __grid_constant__ CUtensorM
           L += f * r[1];
           acc += f * r[2 + d];
         }
-      p.out[((long long)b * p.Hq + hkv * p.G) * Q8_D + i] = __float2bfloat16(L > 0.f ? acc / L : 0.f);
+      p.out[((long long)b * p.Hq + hkv * p.G) * Q8_D + i] = dq_quotient(acc, L);
     }
     cl.sync();                                 // nobody leaves while its results are read
   };
@@ -582,7 +585,7 @@ paged_decode_q8_kernel(const DecodeQ8Params p, const __grid_constant__ CUtensorM
       to[2 + d] = acc;
       if (d == 0) { to[0] = M; to[1] = l; }
     } else {
-      p.out[((long long)b * p.Hq + hkv * p.G + h) * Q8_D + d] = __float2bfloat16(l > 0.f ? acc / l : 0.f);
+      p.out[((long long)b * p.Hq + hkv * p.G + h) * Q8_D + d] = dq_quotient(acc, l);
     }
   }
   if (p.splits > 1 && ws == nullptr) merge_cluster();
@@ -632,7 +635,7 @@ paged_decode_q8_merge_kernel(const float* ws, __nv_bfloat16* out, int Hq, int Hk
     }
     for (; s < n; ++s) o += s_f[s] * at[s * sstride];
   }
-  out[(long long)blockIdx.x * Q8_D + d] = __float2bfloat16(L > 0.f ? o / L : 0.f);
+  out[(long long)blockIdx.x * Q8_D + d] = dq_quotient(o, L);
 }
 static_assert(Q8_D == 128, "four warps");
 

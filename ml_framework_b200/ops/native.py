@@ -456,7 +456,7 @@ def _heads(what: str, name: str, t: torch.Tensor, H: Optional[int] = None) -> to
 
 def _aligned_rows(t: torch.Tensor) -> torch.Tensor:
     """``t`` with rows that start on 16 bytes: itself where they do."""
-    return t if t.data_ptr() % 16 == 0 and t.stride(0) % 8 == 0 else t.contiguous()
+    return t if t.data_ptr() % 16 == 0 and t.stride(0) % 8 == 0 else t.clone(memory_format=torch.contiguous_format)
 
 
 @lru_cache(maxsize=None)
@@ -505,7 +505,7 @@ def _decode_q8(what: str, q: torch.Tensor, ldq: int, Hq: int, kv_cache, kv_scale
     """Attention of :func:`paged_decode` (``slots`` None) and :func:`paged_decode_rope` over an 8-bit cache."""
     fmt = _q8_format(what, kv_cache, kv_scale)
     B, Hkv = q.shape[0], kv_cache.shape[3]
-    if Hq % Hkv or Hq // Hkv > 16:
+    if Hkv == 0 or Hq % Hkv or not 0 < Hq // Hkv <= 16:
         raise ValueError(f"{what}: {Hq} query heads over {Hkv} KV heads (groups of 1 to 16)")
     if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != B:
         raise ValueError(f"{what}: block_table must be int32 [{B}, max_blocks], got {block_table.dtype} {tuple(block_table.shape)}")
@@ -513,7 +513,7 @@ def _decode_q8(what: str, q: torch.Tensor, ldq: int, Hq: int, kv_cache, kv_scale
     slots = _index(what, "slots", slots, torch.int64, B) if slots is not None else None
     _on_current_device(what, q, kv_cache, kv_scale, table, lens, slots)
     out = torch.empty(B, Hq, 128, dtype=q.dtype, device=q.device)
-    if B == 0 or Hq == 0:
+    if B == 0:
         return out
     if table.shape[1] == 0:
         return out.zero_()
@@ -546,14 +546,14 @@ def paged_decode(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Ten
     a second small kernel; it measured slower (57 us against 48 us at batch 64, 576 cached tokens), hence off.
 
     An 8-bit cache (float8_e4m3fn or int8) comes with ``kv_scale``, float32 [num_blocks, 2, Hkv]: a value is its number times the
-    scale of its block, side (K, V) and head. Any positive scales; groups of 1 to 16 query heads per KV head; the splits
-    are a whole number of blocks each. A sequence of length 0 gives zeros.
+    scale of its block, side (K, V) and head. Scales from 2^-60 to 2^60, not powers of two alone; groups of 1 to 16 query heads per KV
+    head; the splits are a whole number of blocks each, and ``fused_merge`` changes nothing. A sequence of length 0 gives zeros.
     """
     if kv_scale is not None or kv_cache.dtype in _Q8:
         q = _heads("paged_decode", "q", q)
         if q.data_ptr() % 4 or q.stride(0) % 2:
-            q = q.contiguous()
-        return _decode_q8("paged_decode", q, q.stride(0), q.shape[1], kv_cache, kv_scale, block_table, seq_lens, None, max_seq_len, scale, split_tokens, 0.0, False)
+            q = q.clone(memory_format=torch.contiguous_format)
+        return _decode_q8("paged_decode", q, q.stride(0), q.shape[1], kv_cache, kv_scale, block_table, seq_lens, None, int(max_seq_len), scale, split_tokens, 0.0, False)
     B, Hq, D = q.shape
     nb, two, bs, Hkv, D2 = kv_cache.shape
     assert D == 128 and D2 == 128 and two == 2 and kv_cache.is_contiguous()
@@ -590,7 +590,8 @@ def paged_decode_rope(qkv: torch.Tensor, kv_cache: torch.Tensor, block_table: to
     cached rows of earlier tokens, which may then be read ahead of the kernels before this one.
 
     With ``kv_scale`` (an 8-bit cache, see :func:`paged_decode`) the new rows are rounded to 8 bits as :func:`kv_cache_write` does
-    and attended to as they are then held; ``inputs_static`` speaks of the scales too."""
+    and attended to as they are then held; ``inputs_static`` speaks of the scales too. A slot is the place of the sequence's newest
+    token by its block table, in a block that no other sequence reads (a shared one is copied first): the block's scale may grow."""
     B = qkv.shape[0]
     if kv_scale is not None or kv_cache.dtype in _Q8:
         what = "paged_decode_rope"
@@ -600,7 +601,7 @@ def paged_decode_rope(qkv: torch.Tensor, kv_cache: torch.Tensor, block_table: to
             raise ValueError(f"{what}: rows must be 8-byte aligned and theta positive")
         if inputs_static and not (seq_lens.is_contiguous() and block_table.is_contiguous() and slots.is_contiguous()):
             raise ValueError(f"{what}: inputs_static needs contiguous block_table, seq_lens and slots")      # a copy here would write them
-        return _decode_q8(what, qkv, qkv.stride(0), Hq, kv_cache, kv_scale, block_table, seq_lens, slots, max_seq_len, scale, split_tokens, theta, inputs_static)
+        return _decode_q8(what, qkv, qkv.stride(0), Hq, kv_cache, kv_scale, block_table, seq_lens, slots, int(max_seq_len), scale, split_tokens, theta, inputs_static)
     nb, two, bs, Hc, D = kv_cache.shape
     assert D == 128 and two == 2 and Hc == Hkv and kv_cache.is_contiguous() and qkv.shape[1] == (Hq + 2 * Hkv) * D
     assert qkv.stride(1) == 1 and qkv.dtype == torch.bfloat16 and kv_cache.dtype == torch.bfloat16 and slots.dtype == torch.int64
@@ -691,7 +692,7 @@ def kv_gather(kv_cache: torch.Tensor, block_table_row: torch.Tensor, length: int
     """Contiguous (k, v) [length, Hkv, 128] of one sequence from its pages; in bf16 the values of an 8-bit cache (``kv_scale``)."""
     if kv_scale is not None or kv_cache.dtype in _Q8:
         what = "kv_gather"
-        fmt = _q8_format(what, kv_cache, kv_scale)
+        fmt, length = _q8_format(what, kv_cache, kv_scale), int(length)
         nb, _, bs, Hkv, _ = kv_cache.shape
         row = _index(what, "block_table_row", block_table_row, torch.int32, block_table_row.numel())
         if not 0 <= length <= row.numel() * bs:
@@ -747,7 +748,7 @@ def argmax_rows(logits: torch.Tensor, vocab: int) -> torch.Tensor:
 
 def sample_rows(logits: torch.Tensor, vocab: int, u: torch.Tensor, temperature: torch.Tensor, top_k: Optional[torch.Tensor] = None,
                 top_p: Optional[torch.Tensor] = None, min_p: Optional[torch.Tensor] = None, want_logprobs: bool = False):
-    """Next tokens (int64 [rows]) from the first ``vocab`` columns of ``logits`` [rows, ld], bf16 or fp32, each row with settings of its own:
+    """Next tokens (int64 [rows]) from the first ``vocab`` columns (up to 2^20) of ``logits`` [rows, ld], bf16 or fp32, each row with settings of its own:
     ``temperature`` (float32; 0 or less: the largest logit), ``top_k`` (int32; 0 or less: no limit), ``top_p`` (1 or more: no limit) and
     ``min_p`` (0 or less: no limit; float32 each). ``u``: a random number of [0, 1) per row, float32.
 
@@ -757,7 +758,7 @@ def sample_rows(logits: torch.Tensor, vocab: int, u: torch.Tensor, temperature: 
     whatever stands in the other rows. NaN counts as -inf; a row without any other logit gives token 0. With
     ``want_logprobs``: (tokens, logprobs), float32 [rows], the logarithm of the token's probability among the kept ones (0 for
     temperature 0, -inf for a row of -inf)."""
-    what = "sample_rows"
+    what, vocab = "sample_rows", int(vocab)
     if logits.dim() != 2 or logits.dtype not in (torch.bfloat16, torch.float32) or not 0 < vocab <= logits.shape[1]:
         raise ValueError(f"{what}: logits must be bfloat16 or float32 [rows, at least {vocab}], got {logits.dtype} {tuple(logits.shape)}")
     rows = logits.shape[0]

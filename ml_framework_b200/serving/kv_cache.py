@@ -115,7 +115,8 @@ class KVCacheBlockManager:
 
     def compact(self) -> int:
         """Moves the blocks in use to the lowest numbers, contents and all, so that the free ones lie behind them in one run.
-        Sequences keep their tokens and their sharing; block tables built before are void. Returns the number of blocks moved."""
+        Sequences keep their tokens and their sharing; block tables and slots handed out before are void, so it is called between
+        steps, on their stream. Returns the number of blocks moved."""
         pairs = array("i", bytes(8 * self.total_blocks))
         n = self._L.mlf_bm_compact(self._h, C.c_void_p(pairs.buffer_info()[0]))
         if n < 0:

@@ -685,6 +685,7 @@ class PrefillHandler:
 # ------------------------------------------------------------------ client
 @dataclass
 class GenerationOptions:
+    """``temperature`` above 0 draws the tokens (:class:`SamplingParameters`)."""
     stop_strings: Sequence[str] = ()
     temperature: float = 0.0
     top_k: int = 0

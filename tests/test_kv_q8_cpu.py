@@ -44,6 +44,16 @@ def test_attention_refuses(dtype):
         _decode(c, s)
 
 
+def test_no_heads_are_refused():
+    for H, Hq in ((0, 4), (2, 0), (0, 0)):
+        c, s = _cache(H=H)
+        with pytest.raises(ValueError, match="groups of 1 to 16"):
+            _decode(c, s, Hq=Hq)
+        with pytest.raises(ValueError):
+            native.paged_decode_rope(torch.zeros(3, (Hq + 2 * H) * 128, dtype=BF), c, torch.zeros(3, 2, dtype=torch.int32), torch.ones(3, dtype=torch.int32),
+                                     torch.zeros(3, dtype=torch.int64), Hq, H, 32, 1e4, kv_scale=s)
+
+
 def test_append_refuses():
     c, s = _cache()
     qkv, table, lens, slots = torch.zeros(3, 8 * 128, dtype=BF), torch.zeros(3, 2, dtype=torch.int32), torch.ones(3, dtype=torch.int32), torch.zeros(3, dtype=torch.int64)

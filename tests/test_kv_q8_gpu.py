@@ -270,6 +270,50 @@ def test_attention_ignores_what_lies_behind_a_sequence():
     assert torch.equal(native.paged_decode(q, cache, table, sl, 33, kv_scale=scale), want)
 
 
+@pytest.mark.parametrize("dtype", KINDS)
+@pytest.mark.parametrize("n,split", [(40, 0), (700, 128), (3000, 128)])
+def test_attention_keeps_nan(dtype, n, split):
+    """A NaN in a query head, or (e4m3) in a cached key or value, is one of that head's outputs, and of no other's."""
+    g = _gen(n)
+    cache, scale = _random_cache(n // 16 + 2, 16, 2, dtype, g)
+    table = torch.arange(n // 16 + 2, device="cuda", dtype=torch.int32)[None].expand(2, -1).contiguous()
+    lens = torch.tensor([n, n], device="cuda", dtype=torch.int32)
+    q = torch.randn(2, 8, D, device="cuda", generator=g).bfloat16()
+    good = native.paged_decode(q, cache, table, lens, n, split_tokens=split, kv_scale=scale)
+    q[1, 5, 17] = float("nan")
+    got = native.paged_decode(q, cache, table, lens, n, split_tokens=split, kv_scale=scale)
+    assert got[1, 5].isnan().all()
+    got[1, 5] = good[1, 5]
+    assert torch.equal(got, good)
+    if dtype == torch.float8_e4m3fn:
+        q[1, 5, 17] = 0.0
+        bad = cache.clone()
+        _bytes(bad)[1, 0, 3, 1, 9] = 0x7f                      # token 19: the key of head 1
+        got = native.paged_decode(q, bad, table, lens, n, split_tokens=split, kv_scale=scale)
+        assert got[:, 4:].isnan().all() and torch.equal(got[0, :4], good[0, :4])
+        bad = cache.clone()
+        _bytes(bad)[1, 1, 3, 0, 9] = 0x7f                      # a value of head 0
+        got = native.paged_decode(q, bad, table, lens, n, split_tokens=split, kv_scale=scale)
+        assert got[:, :4, 9].isnan().all() and not got[:, :4, :9].isnan().any() and torch.equal(got[0, 4:], good[0, 4:])
+
+
+def test_operands_at_odd_addresses():
+    """Rows that start on no 16 (queries: 4) bytes, contiguous ones too, are copied before the launch."""
+    g = _gen(77)
+    for T in (1, 5):
+        cache, scale = _random_cache(3, 16, 2, torch.int8, g)
+        flat = torch.randn(2 * T * 2 * D + 3, device="cuda", generator=g).bfloat16()
+        k, v = flat[1:1 + T * 2 * D].view(T, 2, D), flat[3 + T * 2 * D:].view(T, 2, D)
+        slots = torch.arange(20, 20 + T, device="cuda")
+        want_c, want_s = cache.clone(), scale.clone()
+        native.kv_cache_write(want_c, k.clone(), v.clone(), slots, kv_scale=want_s)
+        native.kv_cache_write(cache, k, v, slots, kv_scale=scale)
+        assert torch.equal(_bytes(cache), _bytes(want_c)) and torch.equal(scale, want_s)
+        table, lens = torch.ones(T, 1, device="cuda", dtype=torch.int32), torch.full((T,), 16, device="cuda", dtype=torch.int32)
+        want = native.paged_decode(k.clone(), cache, table, lens, 16, kv_scale=scale)
+        assert torch.equal(native.paged_decode(k, cache, table, lens, 16, kv_scale=scale), want)
+
+
 def test_attention_long_cache():
     """Cache offsets past 2^32 bytes."""
     bs, Hkv, nb = 16, 8, (1 << 32) // (2 * 16 * 8 * D) + 4
