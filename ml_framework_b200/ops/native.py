@@ -425,19 +425,20 @@ def _on_current_device(what: str, *tensors: Optional[torch.Tensor]):
             raise ValueError(f"{what}: a tensor is on {t.device}, the kernel runs on the current CUDA device")
 
 
-def _q8_format(what: str, kv_cache: torch.Tensor, kv_scale: Optional[torch.Tensor]) -> int:
-    """Format of an 8-bit cache [num_blocks, 2, block_size, Hkv, 128] with its scales [num_blocks, 2, Hkv]."""
+def _q8_cache(what: str, kv_cache: torch.Tensor, kv_scale: Optional[torch.Tensor]) -> Tuple[int, int, int, int]:
+    """Format, num_blocks, block_size and Hkv of an 8-bit cache [num_blocks, 2, block_size, Hkv, 128] with its scales [num_blocks, 2, Hkv]."""
     fmt = _Q8.get(kv_cache.dtype)
     if fmt is None:
         raise TypeError(f"{what}: scales belong to a cache of torch.float8_e4m3fn or torch.int8, not {kv_cache.dtype}")
     shape = kv_cache.shape
-    if len(shape) != 5 or shape[1] != 2 or shape[4] != 128 or not kv_cache.is_contiguous():
+    nb, two, bs, Hkv, D = shape if len(shape) == 5 else (0,) * 5
+    if two != 2 or D != 128 or not kv_cache.is_contiguous():
         raise ValueError(f"{what}: the cache must be contiguous [num_blocks, 2, block_size, kv_heads, 128], got {tuple(shape)}")
     if kv_scale is None:
         raise ValueError(f"{what}: a cache of {kv_cache.dtype} needs kv_scale")
-    if kv_scale.shape != (shape[0], 2, shape[3]) or kv_scale.dtype != torch.float32 or not kv_scale.is_contiguous():
-        raise ValueError(f"{what}: kv_scale must be contiguous float32 {(shape[0], 2, shape[3])}, got {kv_scale.dtype} {tuple(kv_scale.shape)}")
-    return fmt
+    if kv_scale.shape != (nb, 2, Hkv) or kv_scale.dtype != torch.float32 or not kv_scale.is_contiguous():
+        raise ValueError(f"{what}: kv_scale must be contiguous float32 {(nb, 2, Hkv)}, got {kv_scale.dtype} {tuple(kv_scale.shape)}")
+    return fmt, nb, bs, Hkv
 
 
 def _index(what: str, name: str, t: torch.Tensor, dtype, *shape: int) -> torch.Tensor:
@@ -448,10 +449,11 @@ def _index(what: str, name: str, t: torch.Tensor, dtype, *shape: int) -> torch.T
 
 def _heads(what: str, name: str, t: torch.Tensor, H: Optional[int] = None) -> torch.Tensor:
     """bf16 [T, H, 128] whose tokens are whole rows at any pitch."""
-    if t.dim() != 3 or t.shape[2] != 128 or (H is not None and t.shape[1] != H) or t.dtype != torch.bfloat16:
-        raise ValueError(f"{what}: {name} must be bfloat16 [tokens, {'heads' if H is None else H}, 128], got {t.dtype} {tuple(t.shape)}")
+    shape = t.shape
+    if len(shape) != 3 or shape[2] != 128 or (H is not None and shape[1] != H) or t.dtype != torch.bfloat16:
+        raise ValueError(f"{what}: {name} must be bfloat16 [tokens, {'heads' if H is None else H}, 128], got {t.dtype} {tuple(shape)}")
     _, head, one = t.stride()
-    return t if one == 1 and (head == 128 or t.shape[1] == 1) else t.contiguous()
+    return t if one == 1 and (head == 128 or shape[1] == 1) else t.contiguous()
 
 
 def _aligned_rows(t: torch.Tensor) -> torch.Tensor:
@@ -503,19 +505,19 @@ def _decode_split_q8(pairs: int, max_seq_len: int, sms: int) -> int:
 def _decode_q8(what: str, q: torch.Tensor, ldq: int, Hq: int, kv_cache, kv_scale, block_table, seq_lens, slots, max_seq_len: int, scale, split_tokens: int,
                theta: float, inputs_static: bool) -> torch.Tensor:
     """Attention of :func:`paged_decode` (``slots`` None) and :func:`paged_decode_rope` over an 8-bit cache."""
-    fmt = _q8_format(what, kv_cache, kv_scale)
-    B, Hkv = q.shape[0], kv_cache.shape[3]
+    fmt, nb, bs, Hkv = _q8_cache(what, kv_cache, kv_scale)
+    B, rows = q.shape[0], block_table.shape
     if Hkv == 0 or Hq % Hkv or not 0 < Hq // Hkv <= 16:
         raise ValueError(f"{what}: {Hq} query heads over {Hkv} KV heads (groups of 1 to 16)")
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != B:
-        raise ValueError(f"{what}: block_table must be int32 [{B}, max_blocks], got {block_table.dtype} {tuple(block_table.shape)}")
+    if block_table.dtype != torch.int32 or len(rows) != 2 or rows[0] != B:
+        raise ValueError(f"{what}: block_table must be int32 [{B}, max_blocks], got {block_table.dtype} {tuple(rows)}")
     table, lens = block_table.contiguous(), _index(what, "seq_lens", seq_lens, torch.int32, B)
     slots = _index(what, "slots", slots, torch.int64, B) if slots is not None else None
     _on_current_device(what, q, kv_cache, kv_scale, table, lens, slots)
-    out = torch.empty(B, Hq, 128, dtype=q.dtype, device=q.device)
+    out = q.new_empty((B, Hq, 128))
     if B == 0:
         return out
-    if table.shape[1] == 0:
+    if rows[1] == 0:
         return out.zero_()
     sms = _sm_count(torch._C._cuda_getDevice())
     if split_tokens <= 0:
@@ -527,7 +529,7 @@ def _decode_q8(what: str, q: torch.Tensor, ldq: int, Hq: int, kv_cache, kv_scale
     ws = None if within else torch.empty(B * Hq * splits * 130, dtype=torch.float32, device=q.device)
     rc = _function("mlf_paged_decode_q8", "plppipppppliiiiiiiiffiu")(
         q.data_ptr(), ldq, kv_cache.data_ptr(), kv_scale.data_ptr(), fmt, table.data_ptr(), lens.data_ptr(), _at(slots), out.data_ptr(), _at(ws),
-        0 if ws is None else ws.numel(), B, Hq, Hkv, kv_cache.shape[2], table.shape[1], kv_cache.shape[0], max_seq_len, splits,
+        0 if ws is None else ws.numel(), B, Hq, Hkv, bs, rows[1], nb, max_seq_len, splits,
         scale if scale is not None else 128 ** -0.5, theta, int(inputs_static), _stream())
     _lib.check(rc, "mlf_paged_decode_q8")
     return out
@@ -622,6 +624,15 @@ def paged_decode_rope(qkv: torch.Tensor, kv_cache: torch.Tensor, block_table: to
     return out
 
 
+def _write_q8(kv_cache, kv_scale, layout: Tuple[int, int, int, int], k: int, v: int, slots: torch.Tensor, T: int, ldk: int, ldv: int):
+    """T rows at the addresses ``k`` and ``v``, checked by the callers."""
+    fmt, nb, bs, Hkv = layout
+    where = kv_cache.new_empty(nb * bs, dtype=torch.int32) if T > 2048 or bs > 64 else None
+    rc = _function("mlf_kv_write_q8", "ppippppliiillu")(kv_cache.data_ptr(), kv_scale.data_ptr(), fmt, k, v, slots.data_ptr(), _at(where), T, Hkv, bs, nb,
+                                                        ldk, ldv, _stream())
+    _lib.check(rc, "mlf_kv_write_q8")
+
+
 def kv_cache_write(kv_cache: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, kv_scale: Optional[torch.Tensor] = None):
     """Scatter k, v [T, Hkv, 128] into cache slots (slot = block * block_size + offset; < 0 skips).
 
@@ -633,21 +644,15 @@ def kv_cache_write(kv_cache: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slo
     stand anywhere in the list; a slot given twice keeps one of its rows, whole. NaN stays NaN in e4m3 and becomes 0 in int8."""
     if kv_scale is not None or kv_cache.dtype in _Q8:
         what = "kv_cache_write"
-        fmt = _q8_format(what, kv_cache, kv_scale)
-        k, v = _aligned_rows(_heads(what, "k", k, kv_cache.shape[3])), _aligned_rows(_heads(what, "v", v, kv_cache.shape[3]))
+        fmt, nb, bs, Hkv = _q8_cache(what, kv_cache, kv_scale)
+        k, v = _aligned_rows(_heads(what, "k", k, Hkv)), _aligned_rows(_heads(what, "v", v, Hkv))
         T = k.shape[0]
         if v.shape[0] != T:
             raise ValueError(f"{what}: {T} keys and {v.shape[0]} values")
         slots = _index(what, "slots", slots, torch.int64, T)
         _on_current_device(what, kv_cache, kv_scale, k, v, slots)
-        if T == 0 or kv_cache.numel() == 0:
-            return
-        nb, _, bs, Hkv, _ = kv_cache.shape
-        where = torch.empty(nb * bs, dtype=torch.int32, device=k.device) if T > 2048 or bs > 64 else None
-        rc = _function("mlf_kv_write_q8", "ppippppliiillu")(
-            kv_cache.data_ptr(), kv_scale.data_ptr(), fmt, k.data_ptr(), v.data_ptr(), slots.data_ptr(), _at(where), T, Hkv, bs, nb,
-            k.stride(0), v.stride(0), _stream())
-        _lib.check(rc, "mlf_kv_write_q8")
+        if T > 0 and kv_cache.numel() > 0:
+            _write_q8(kv_cache, kv_scale, (fmt, nb, bs, Hkv), k.data_ptr(), v.data_ptr(), slots, T, k.stride(0), v.stride(0))
         return
     nb, _, bs, Hkv, D = kv_cache.shape
     T = k.shape[0]
@@ -665,9 +670,9 @@ def rope_kv_write_(qkv: torch.Tensor, pos: torch.Tensor, slots: torch.Tensor, kv
     :func:`kv_cache_write`'s, in launches of its own, and rows must be 16-byte aligned."""
     if kv_scale is not None or kv_cache.dtype in _Q8:
         what = "rope_kv_write_"
-        _q8_format(what, kv_cache, kv_scale)
+        layout = _q8_cache(what, kv_cache, kv_scale)
         T = qkv.shape[0]
-        if qkv.dim() != 2 or qkv.dtype != torch.bfloat16 or qkv.shape[1] != (Hq + 2 * Hkv) * 128 or qkv.stride(1) != 1 or kv_cache.shape[3] != Hkv:
+        if qkv.dim() != 2 or qkv.dtype != torch.bfloat16 or qkv.shape[1] != (Hq + 2 * Hkv) * 128 or qkv.stride(1) != 1 or layout[3] != Hkv:
             raise ValueError(f"{what}: qkv must be bfloat16 [T, ({Hq} + 2 * {Hkv}) * 128] beside a cache of {Hkv} heads, got {qkv.dtype} {tuple(qkv.shape)}")
         if qkv.data_ptr() % 16 or qkv.stride(0) % 8:
             raise ValueError(f"{what}: rows must be 16-byte aligned")
@@ -676,7 +681,9 @@ def rope_kv_write_(qkv: torch.Tensor, pos: torch.Tensor, slots: torch.Tensor, kv
         if T == 0:
             return qkv
         rope_qkv(qkv, pos, Hq, Hkv, theta, out=qkv)
-        kv_cache_write(kv_cache, qkv[:, Hq * 128:(Hq + Hkv) * 128].view(T, Hkv, 128), qkv[:, (Hq + Hkv) * 128:].view(T, Hkv, 128), slots, kv_scale)
+        if kv_cache.numel() > 0:
+            k = qkv.data_ptr() + Hq * 256
+            _write_q8(kv_cache, kv_scale, layout, k, k + Hkv * 256, slots, T, qkv.stride(0), qkv.stride(0))
         return qkv
     nb, _, bs, Hc, D = kv_cache.shape
     assert D == 128 and Hc == Hkv and qkv.dim() == 2 and qkv.stride(1) == 1 and qkv.shape[1] == (Hq + 2 * Hkv) * 128
@@ -692,17 +699,17 @@ def kv_gather(kv_cache: torch.Tensor, block_table_row: torch.Tensor, length: int
     """Contiguous (k, v) [length, Hkv, 128] of one sequence from its pages; in bf16 the values of an 8-bit cache (``kv_scale``)."""
     if kv_scale is not None or kv_cache.dtype in _Q8:
         what = "kv_gather"
-        fmt, length = _q8_format(what, kv_cache, kv_scale), int(length)
-        nb, _, bs, Hkv, _ = kv_cache.shape
-        row = _index(what, "block_table_row", block_table_row, torch.int32, block_table_row.numel())
-        if not 0 <= length <= row.numel() * bs:
-            raise ValueError(f"{what}: {length} tokens, {row.numel()} block-table entries of {bs}")
+        fmt, nb, bs, Hkv = _q8_cache(what, kv_cache, kv_scale)
+        length, entries = int(length), block_table_row.numel()
+        row = _index(what, "block_table_row", block_table_row, torch.int32, entries)
+        if not 0 <= length <= entries * bs:
+            raise ValueError(f"{what}: {length} tokens, {entries} block-table entries of {bs}")
         _on_current_device(what, kv_cache, kv_scale, row)
-        k = torch.empty(length, Hkv, 128, dtype=torch.bfloat16, device=kv_cache.device)
+        k = kv_cache.new_empty((length, Hkv, 128), dtype=torch.bfloat16)
         v = torch.empty_like(k)
         if length:
             rc = _function("mlf_kv_gather_q8", "ppipiiiiippu")(
-                kv_cache.data_ptr(), kv_scale.data_ptr(), fmt, row.data_ptr(), row.numel(), length, Hkv, bs, nb, k.data_ptr(), v.data_ptr(), _stream())
+                kv_cache.data_ptr(), kv_scale.data_ptr(), fmt, row.data_ptr(), entries, length, Hkv, bs, nb, k.data_ptr(), v.data_ptr(), _stream())
             _lib.check(rc, "mlf_kv_gather_q8")
         return k, v
     nb, _, bs, Hkv, D = kv_cache.shape
