@@ -45,6 +45,7 @@ constexpr int SM_STEP = 256;                   // logits that a warp takes at a 
 constexpr int SM_HELD = 4;                     // such steps that a warp can keep in shared memory
 constexpr int SM_STEPS = 32;                   // at most, per warp
 constexpr int SM_BINS = 2048;
+constexpr int SM_FINE = 4096;                   // bins of one bf16 value each: 16 binades of either sign
 constexpr int SM_GROUPS = 64;                  // sums of neighbouring bins that CTAs exchange
 constexpr int SM_COARSE = 512;                 // bins of the maxima
 constexpr int SM_LIST = 2048;                  // tokens that a list takes
@@ -75,6 +76,7 @@ struct SampleSmem {
       alignas(16) unsigned lo[SM_BINS];        // weights of the bins
       alignas(16) unsigned hi[SM_BINS];
     };
+    alignas(16) unsigned fine[SM_FINE];        // counts of bf16 values
   };
   union {
     alignas(16) unsigned cnt[SM_BINS];         // counts of the bins
@@ -163,10 +165,12 @@ __device__ __forceinline__ u64 sm_block_scan(u64 v, SampleSmem& s, u64* total) {
 // Threads for each of n <= SM_THREADS tokens of a list: a power of two up to eight.
 __device__ __forceinline__ int sm_parts(int n) { return n <= SM_THREADS / 8 ? 8 : n <= SM_THREADS / 4 ? 4 : n <= SM_THREADS / 2 ? 2 : 1; }
 
-// Ascending sort of n entries (a power of two, up to SM_LIST) in shared memory.
+// Ascending sort of n entries (a power of two from 128 to SM_LIST) in shared memory, by bitonic merges: what lies within 128 neighbours
+// in a warp's registers, the rest with a barrier each (1024 entries: 6 of 55 steps).
 __device__ __forceinline__ void sm_sort(u64* a, int n) {
-  for (int k = 2; k <= n; k <<= 1)
-    for (int j = k >> 1; j > 0; j >>= 1) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int k = 128; k <= n; k <<= 1) {
+    for (int j = k >> 1; j >= 128; j >>= 1) {
       __syncthreads();
       for (int t = threadIdx.x; t < n / 2; t += SM_THREADS) {
         const int i = 2 * t - (t & (j - 1));
@@ -174,8 +178,33 @@ __device__ __forceinline__ void sm_sort(u64* a, int n) {
         if ((x > y) == ((i & k) == 0)) { a[i] = y; a[i + j] = x; }
       }
     }
+    __syncthreads();
+    if (warp * 128 >= n) continue;             // a warp's 128, four a lane
+    u64* own = a + warp * 128 + lane * 4;
+    u64 v[4] = {own[0], own[1], own[2], own[3]};
+    for (int k2 = k == 128 ? 2 : k; k2 <= k; k2 <<= 1)
+#pragma unroll
+      for (int j = 64; j > 0; j >>= 1) {
+        if (j >= k2) continue;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int i = warp * 128 + lane * 4 + q;
+          if (j >= 4) {
+            const u64 o = __shfl_xor_sync(0xffffffffu, v[q], j / 4);
+            v[q] = ((i & j) == 0) == ((i & k2) == 0) ? min(v[q], o) : max(v[q], o);
+          } else if ((q & j) == 0) {
+            const u64 x = v[q], y = v[q | j];
+            const bool up = (i & k2) == 0;
+            v[q] = up ? min(x, y) : max(x, y);
+            v[q | j] = up ? max(x, y) : min(x, y);
+          }
+        }
+      }
+    own[0] = v[0]; own[1] = v[1]; own[2] = v[2]; own[3] = v[3];
+  }
   __syncthreads();
 }
+static_assert(SM_LIST <= SM_WARPS * 128, "a warp for every 128 entries");
 
 // Smallest integer sum that reaches p of `total`; that is above u of it.
 __device__ __forceinline__ u64 sm_reach(double p, u64 total) {
@@ -257,16 +286,25 @@ struct SampleRow {
   }
   // f(step, logits) over all steps, the next ones on their way
   template <typename F>
-  __device__ __forceinline__ void each_values(F f) const {
+  __device__ __forceinline__ void each_words(F f) const {
     unsigned w[WORDS];
     if (steps > 0) words(0, w);
 #pragma unroll 1
     for (int st = 0; st < steps; ++st) {
+      unsigned now[WORDS];
+#pragma unroll
+      for (int j = 0; j < WORDS; ++j) now[j] = w[j];
+      if (st + 1 < steps) words(st + 1, w);
+      f(st, now);
+    }
+  }
+  template <typename F>
+  __device__ __forceinline__ void each_values(F f) const {
+    each_words([&](int st, const unsigned (&w)[WORDS]) {
       float x[8];
       unpack(w, x);
-      if (st + 1 < steps) words(st + 1, w);
       f(st, x);
-    }
+    });
   }
   // the largest of a lane's eight logits; NaN only where all are
   __device__ __forceinline__ static float maximum(const unsigned (&w)[WORDS]) {
@@ -435,6 +473,8 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_rows_kernel(const Sample
   if (tid < 32) s.exp2[tid] = c_exp2[tid];
   if (tid == 0) s.n_local = 0;
   for (int i = tid; i < SM_COARSE; i += SM_THREADS) s.cnt[i] = 0;
+  if (sizeof(T) == 2)
+    for (int i = tid; i < SM_FINE / 4; i += SM_THREADS) reinterpret_cast<uint4*>(s.fine)[i] = make_uint4(0u, 0u, 0u, 0u);
   pdl_wait();
   const int r = blockIdx.x / C;
   SampleRow<T, HELD> row;
@@ -489,9 +529,9 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_rows_kernel(const Sample
     }
   }
   if (lane == 0) {
-    s.list[warp] = top;
-    s.list[SM_WARPS + warp] = (u64)__float_as_uint(sum) << 32 | __float_as_uint(square);
-    s.list[2 * SM_WARPS + warp] = (u64)n_sum;
+    s.group[warp] = top;
+    s.group[SM_WARPS + warp] = (u64)__float_as_uint(sum) << 32 | __float_as_uint(square);
+    s.group[2 * SM_WARPS + warp] = (u64)n_sum;
   }
   __syncthreads();
   cl.barrier_wait();
@@ -500,10 +540,10 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_rows_kernel(const Sample
     float f = 0.f, g = 0.f;
 #pragma unroll
     for (int i = 0; i < SM_WARPS; ++i) {
-      t = max(t, s.list[i]);
-      f += __uint_as_float((unsigned)(s.list[SM_WARPS + i] >> 32));
-      g += __uint_as_float((unsigned)s.list[SM_WARPS + i]);
-      n += s.list[2 * SM_WARPS + i];
+      t = max(t, s.group[i]);
+      f += __uint_as_float((unsigned)(s.group[SM_WARPS + i] >> 32));
+      g += __uint_as_float((unsigned)s.group[SM_WARPS + i]);
+      n += s.group[2 * SM_WARPS + i];
     }
     u64* to = cl.map_shared_rank(&s.slot[0][0][0], tid);
     to[rank] = t;
@@ -692,17 +732,113 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_rows_kernel(const Sample
       return s.list[q * room + i];
     };
     bool open = true;
+    u64 n_class = 0, n_take = 0;                            // tokens with the deciding logit, and how many of them are kept
     // p alone: a normal distribution with this mean and variance has V exp((mean - m) / T + var / 2 T^2) of the largest logit's weight, and
     // z standard deviations above the mean 128 tokens, below which all but the upper tail beyond z - sigma / T of that weight
     // lies. Where that is more than p leaves out, 128 tokens will not do. Only the way depends on it, not the token.
     bool flat = false;
-    if (!need_k && p.vocab > SM_LIST) {
+    if (sizeof(T) == 4 && !need_k && p.vocab > SM_LIST) {
       const float inv_t = __fdiv_rn(1.f, temp), t = sqrtf(2.f * __logf((float)p.vocab / SM_FEW));
       const float z = t - (2.30753f + 0.27061f * t) / (1.f + t * (0.99229f + 0.04481f * t));      // Hastings' approximation of the normal quantile
       const float bulk = __expf(__logf((float)p.vocab) + ((mean - m) + 0.5f * var * inv_t) * inv_t);
       flat = bulk * normcdff(z - sqrtf(fmaxf(var, 0.f)) * inv_t) > (1.f - top_p) * (bulk + 2.f);
     }
-    if (!flat) {
+    if (sizeof(T) == 2 && !need_k) {
+      // ---- (3) for bf16
+      const float low = mean - 4.f * sqrtf(fmaxf(var, 0.f));
+      const int e_top = max(max((int)(__float_as_uint(m) >> 23 & 255u), (int)(__float_as_uint(low) >> 23 & 255u)), 16);
+      const int most = e_top << 7 | 127;                    // magnitudes (15 bits) from here down: SM_FINE / 2 of them, no subnormal one
+      u64 w_small = 0, w_low = 0;                           // weights of what is nearer to 0 than the bins, and of what lies below them
+      row.each_words([&](int st, const unsigned (&w)[SampleRow<T, HELD>::WORDS]) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const unsigned b = j & 1 ? w[j / 2] >> 16 : w[j / 2] & 0xffffu;
+          const int mag = (int)(b & 0x7fffu), d = most - mag;
+          if ((unsigned)d < SM_FINE / 2 && mag <= 0x7f80) {
+            atomicAdd(&s.fine[b & 0x8000u ? SM_FINE - 1 - d : d], 1u);
+          } else if (mag <= 0x7f80) {
+            const u64 v = weight(__uint_as_float(b << 16));
+            if (d < 0) w_low += v;
+            else w_small += v;
+          }
+        }
+      });
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        w_small += __shfl_xor_sync(0xffffffffu, w_small, o);
+        w_low += __shfl_xor_sync(0xffffffffu, w_low, o);
+      }
+      if (lane == 0) {
+        s.group[warp] = w_small;
+        s.group[SM_WARPS + warp] = w_low;
+      }
+      __syncthreads();
+      if (tid < C) {
+        w_small = w_low = 0;
+#pragma unroll
+        for (int i = 0; i < SM_WARPS; ++i) {
+          w_small += s.group[i];
+          w_low += s.group[SM_WARPS + i];
+        }
+        u64* to = cl.map_shared_rank(&s.slot[ex][0][0], tid);
+        to[rank] = w_small;
+        to[SM_CLUSTER + rank] = w_low;
+      }
+      cl.sync();
+      w_small = w_low = 0;
+      for (int i = 0; i < C; ++i) {
+        w_small += s.slot[ex][0][i];
+        w_low += s.slot[ex][1][i];
+      }
+      ++ex;
+      // every CTA takes its share of the bins from all, `per` of them a thread in the order of the logits; what is near 0 stands before the
+      // first negative one
+      constexpr int MOST = SM_FINE / SM_THREADS;
+      const int per = MOST / C, base = (rank * SM_THREADS + tid) * per;
+      unsigned n[MOST];
+#pragma unroll
+      for (int i = 0; i < MOST; ++i) n[i] = cl.map_shared_rank(s.fine, i / per)[base + i % per];
+#pragma unroll
+      for (int o = MOST / 2; o > 0; o >>= 1)
+        if (per <= o)
+#pragma unroll
+          for (int i = 0; i < o; ++i) { n[i] += n[i + o]; n[i + o] = 0; }
+      auto value_of = [&](int bin) {
+        return __uint_as_float(bin < SM_FINE / 2 ? (unsigned)(most - bin) << 16 : 0x80000000u | (unsigned)(most - (SM_FINE - 1 - bin)) << 16);
+      };
+      u64 w[MOST], mine = base == SM_FINE / 2 ? w_small : 0ull, here;
+#pragma unroll
+      for (int j = 0; j < MOST; ++j) {
+        w[j] = n[j] > 0 ? weight(value_of(base + j)) : 0ull;
+        mine += n[j] * w[j];
+      }
+      u64 before = sm_block_scan(mine, s, &here) + (base == SM_FINE / 2 ? w_small : 0ull);
+      u64 (*const found)[SM_CLUSTER] = s.slot[ex + 1];      // of the deciding bin: logit, tokens, how many of them are kept
+      if (tid == 0) found[1][0] = 0;
+      const ulonglong2 sums = exchange_sum(here);
+      before += sums.y;
+      const u64 target = reach(sums.x + w_low);
+      ++ex;
+#pragma unroll
+      for (int j = 0; j < MOST; ++j) {
+        const u64 a = n[j] * w[j];
+        if (a > 0 && before < target && before + a >= target)
+          for (int q = 0; q < C; ++q) {
+            u64* to = cl.map_shared_rank(&found[0][0], q);
+            to[0] = __float_as_uint(value_of(base + j));
+            to[SM_CLUSTER] = n[j];
+            to[2 * SM_CLUSTER] = (target - before + w[j] - 1) / w[j];
+          }
+        before += a;
+      }
+      cl.sync();
+      n_class = found[1][0];
+      if (n_class > 0) {                                    // else near 0, or below the bins: (4)
+        last_x = __uint_as_float((unsigned)found[0][0]);
+        n_take = found[2][0];
+        open = false;
+      }
+    } else if (!flat) {
       // ---- (2)
       bins(SM_COARSE, m - mean);
       u64 w_here = 0;
@@ -812,7 +948,7 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_rows_kernel(const Sample
             if (enough) {
               const int nk = (int)n_kept;
               u64* by_index = s.list + SM_LIST;             // the same by index
-              int pow2k = 2;
+              int pow2k = 128;
               while (pow2k < nk) pow2k <<= 1;
               for (int i = tid; i < pow2k; i += SM_THREADS) {
                 const u64 x = s.list[i];
@@ -845,8 +981,8 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_rows_kernel(const Sample
         if (!open) return;
       }
     }
-    if (!need_k && open) {
-      // ---- (3) down to where a third of what p leaves out is expected below; where that misses the deciding value, as far below
+    if (sizeof(T) == 4 && !need_k && open) {
+      // ---- (3) for fp32: down to where a third of what p leaves out is expected below; where that misses the deciding value, as far below
       // the mean as half of what the largest logit is above it
       const float inv_t = __fdiv_rn(1.f, temp);
       const float deep = m - (mean + var * inv_t + sqrtf(fmaxf(var, 0.f)) * normcdfinvf(fmaxf(1.f - top_p, 1e-6f) * 0.33f));
@@ -972,7 +1108,7 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_rows_kernel(const Sample
         cl.sync();                             // the others have read the counts, whose place the sums take
         return prefix;
       };
-      u64 n_class, n_above, w_above, n_take = 0, w_total = w_all;
+      u64 n_above, w_above, w_total = w_all;
       unsigned key = 0;
       if (need_k) {
         key = decide(false, (u64)top_k, &n_class, &n_above, &w_above);
@@ -991,14 +1127,14 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_rows_kernel(const Sample
         n_class = c;
       }
       last_x = sm_value(key);
-      if (n_take < n_class) {                  // some of the tokens with this logit: those of the lowest indices
-        locate(last_x, [&](float x, int) { return x == last_x ? 1ull : 0ull; }, [&](u64) { return n_take; },
-               [&](int i, float, u64) {
-                 for (int q = 0; q < C; ++q) *cl.map_shared_rank(&s.last, q) = (u64)i;
-               });
-        cl.sync();
-        last_i = (int)s.last;
-      }
+    }
+    if (n_take < n_class) {                    // some of the tokens with this logit: those of the lowest indices
+      locate(last_x, [&](float x, int) { return x == last_x ? 1ull : 0ull; }, [&](u64) { return n_take; },
+             [&](int i, float, u64) {
+               for (int q = 0; q < C; ++q) *cl.map_shared_rank(&s.last, q) = (u64)i;
+             });
+      cl.sync();
+      last_i = (int)s.last;
     }
   }
   if (least > last_x) {
