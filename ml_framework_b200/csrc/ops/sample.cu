@@ -3,8 +3,9 @@
 // With m the largest logit, T the temperature and w_i = exp((x_i - m) / T), in the order of x (the larger first, of equal ones the
 // lower index): the first k tokens are kept; of these the shortest prefix whose weights reach top_p of theirs; of these the
 // tokens with w_i >= min_p; the first one in any case. The token is the first one, by index, at which the running sum of the kept
-// weights is above u times their total. T = 0: the largest logit, of equal ones the lowest index. NaN counts as -inf, a subnormal
-// logit as 0.
+// weights is above u times their total. T < 2^-90: the largest logit, of equal ones the lowest index. T > 2^90
+// counts as 2^90 (beyond either, the differences of logits that matter, or the second float of log2(e) / T, are no normal fp32 numbers).
+// NaN counts as -inf, a subnormal logit as 0.
 //
 // Weights are integers, w_i rounded to 2^-40, from an exponential that is good to about 2^-30: x - m and the product with
 // log2(e) / T are carried in two floats, 2^(j/32) comes from a table and the rest from a polynomial. Sums of integers do not depend on
@@ -15,17 +16,21 @@
 // more are read again in every pass, from the caches, and their lanes' maxima of eight neighbours are kept instead. A pass costs
 // its arithmetic and an exchange through distributed shared memory.
 // (1) Largest logit, and mean and variance of a sample.
-// (2) Where k limits the row, or a p under which few tokens are expected: the bins of equal width that hold the k (128) largest
-// of the maxima of eight neighbours hold at least as many tokens, and hardly more. These go to a list in one CTA, where the token
-// is decided: eight logits cost one comparison in both passes.
-// (3) Where p alone keeps many tokens: the weights of all of them in bins, and the deciding bin alone in the list.
-// (4) Where a list is too long (many equal logits), the deciding value digit by digit over the row, 11 + 11 + 10 bits of the
-// order-preserving integer of a float.
+// (2) Where k limits the row, or (fp32 logits) a p under which few tokens are expected: the bins of equal width that hold the k (128)
+// largest of the maxima of eight neighbours hold at least as many tokens, and hardly more. These go to a list in one CTA, where the
+// token is decided: eight logits cost one comparison in both passes.
+// (3) Where p alone limits it: bf16 logits are counted by their value, 16 binades of either sign, and a value's tokens have the same
+// weight, so that 4096 weights give the total and the deciding value. fp32 logits under a p that keeps many: the weights of all
+// of them in bins, and the deciding bin alone in the list.
+// (4) Where a list is too long (many equal logits), or a bf16 row decided next to 0, the deciding value digit by digit over the row,
+// 11 + 11 + 10 bits of the order-preserving integer of a float.
 // (5) After (3), (4) or no limit: the token from sums of 256 neighbours.
 //
-// Bound by the chain of passes and exchanges for few rows and by the instructions of the weights for many (some 40 each, 150 a
-// logit in (3)). us for 1 / 256 rows of 128256 bf16 logits (floor 0.04 / 10): largest logit 3 / 18, k = 50 with p 10 / 44, no limit
-// 10 / 87, a p that keeps few 17 / 130 - 170, one that keeps thousands 27 / 220, rows of all kinds - / 139.
+// Bound by the chain of passes and exchanges for few rows and by the instructions of the weights (some 40 each), the atomics of the
+// counts (some 16 clocks for 32 logits) and, with fp32 logits in (3), both for many. us for 1 / 256 rows of 128256 bf16 logits (floor
+// 0.04 / 10): largest logit 3 / 18, k = 50 with p 10 / 44, k = 1000 32 / 138, no limit 10 / 88, a p that keeps few 14 / 88, one that keeps
+// thousands 20 / 130 - 150, rows of all kinds - / 100; of fp32 logits (floor 0.08 / 20) a p
+// that keeps few 19 / 185, thousands 28 / 240.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <float.h>
@@ -486,9 +491,9 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_rows_kernel(const Sample
   row.held = s.held + tid;
   row.maxima = reinterpret_cast<float*>(s.held) + tid;
   row.hold();
-  const float temp = p.temperature[r], top_p = p.top_p ? p.top_p[r] : 1.f, min_p = p.min_p ? p.min_p[r] : 0.f, u = p.u[r];
+  const float given = p.temperature[r], temp = given > 0x1p90f ? 0x1p90f : given, top_p = p.top_p ? p.top_p[r] : 1.f, min_p = p.min_p ? p.min_p[r] : 0.f, u = p.u[r];
   const int top_k = p.top_k ? p.top_k[r] : 0;
-  const bool greedy = !(temp > 0.f) || min_p > 1.f;          // the first token of the order alone
+  const bool greedy = !(temp >= 0x1p-90f) || min_p > 1.f;          // the first token of the order alone
 
   // ---- (1) the largest logit, with its first index where that is the answer; mean and variance of the first step
   float best = -INFINITY, sum = 0.f, square = 0.f;
@@ -570,7 +575,7 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_rows_kernel(const Sample
   mean = __fdiv_rn(mean, n_mean);
   var = __fdiv_rn(var, n_mean) - mean * mean;
   SampleWeight<sizeof(T) == 2> weight;
-  const double scale = fmin(32. * 1.4426950408889634074 / (double)temp, 1e30);     // beyond: the same weights, and 0 times it is 0
+  const double scale = 32. * 1.4426950408889634074 / (double)temp;
   weight.m = fminf(m, FLT_MAX);
   weight.ch = (float)scale;
   weight.cl = (float)(scale - (double)weight.ch);
@@ -1152,9 +1157,9 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_rows_kernel(const Sample
 using namespace mlf;
 
 // CTAs per row: as many as a warp's steps need, none with less than 4096 logits; beyond that, more of them shorten the rows whose p keeps
-// most of a flat distribution, which take seven times as long as one with a small k, and cost every row their exchanges.
-// us at 128256 bf16 logits with 1 / 2 / 4 / 8 CTAs: 256 rows of k = 50 35 / 45 / 60 / 90, without limits 87 / 85 / 96 / 125, of all kinds
-// 215 / 139 / 132 / 153; 33 rows of 50257 fp32 logits, k = 50 23 / 20 / 16 / 21, of all kinds 75 / 50 / 40 / 32 (two CTAs fit an SM, but
+// most of a flat distribution, which take four times as long as one with a small k, and cost every row their exchanges.
+// us at 128256 bf16 logits with 1 / 2 / 4 / 8 CTAs: 256 rows of k = 50 34 / 43 / 59 / 85, without limits 89 / 88 / 97 / 113, of all kinds
+// 144 / 101 / 108 / 129; 33 rows of 50257 fp32 logits, k = 50 22 / 20 / 17 / 22, of all kinds 73 / 49 / 39 / 31 (two CTAs fit an SM, but
 // clusters of eight only 32 times). So four CTAs for every SM, and clusters of eight where all run at once.
 static int sample_cluster(long long rows, int vocab) {
   int c = 1;

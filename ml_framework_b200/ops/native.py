@@ -756,7 +756,7 @@ def argmax_rows(logits: torch.Tensor, vocab: int) -> torch.Tensor:
 def sample_rows(logits: torch.Tensor, vocab: int, u: torch.Tensor, temperature: torch.Tensor, top_k: Optional[torch.Tensor] = None,
                 top_p: Optional[torch.Tensor] = None, min_p: Optional[torch.Tensor] = None, want_logprobs: bool = False):
     """Next tokens (int64 [rows]) from the first ``vocab`` columns (up to 2^20) of ``logits`` [rows, ld], bf16 or fp32, each row with settings of its own:
-    ``temperature`` (float32; 0 or less: the largest logit), ``top_k`` (int32; 0 or less: no limit), ``top_p`` (1 or more: no limit) and
+    ``temperature`` (float32; below 2^-90: the largest logit; at most 2^90), ``top_k`` (int32; 0 or less: no limit), ``top_p`` (1 or more: no limit) and
     ``min_p`` (0 or less: no limit; float32 each). ``u``: a random number of [0, 1) per row, float32.
 
     With w_i = exp((x_i - max x) / temperature), in the order of x (of equal ones the lower index first): the first top_k tokens
@@ -764,7 +764,7 @@ def sample_rows(logits: torch.Tensor, vocab: int, u: torch.Tensor, temperature: 
     case. The token is the first one, by index, at which the running sum of the kept weights exceeds u times their total. A row gives the same token
     whatever stands in the other rows. NaN counts as -inf; a row without any other logit gives token 0. With
     ``want_logprobs``: (tokens, logprobs), float32 [rows], the logarithm of the token's probability among the kept ones (0 for
-    temperature 0, -inf for a row of -inf)."""
+    the largest logit alone, -inf for a row of -inf)."""
     what, vocab = "sample_rows", int(vocab)
     if logits.dim() != 2 or logits.dtype not in (torch.bfloat16, torch.float32) or not 0 < vocab <= logits.shape[1]:
         raise ValueError(f"{what}: logits must be bfloat16 or float32 [rows, at least {vocab}], got {logits.dtype} {tuple(logits.shape)}")

@@ -151,8 +151,8 @@ def sample_ref(logits: torch.Tensor, vocab: int, u: torch.Tensor, temperature: t
     x = logits[:, :vocab].double()
     x = torch.where(torch.isnan(x), torch.full_like(x, float("-inf")), x)
     rows, dev = x.shape[0], x.device
-    t = temperature.double()[:, None]
-    greedy = ~(t > 0)
+    t = temperature.double()[:, None].clamp(max=2.0 ** 90)
+    greedy = ~(t >= 2.0 ** -90)
     top = x.amax(1, keepdim=True)
     first = (x == top).to(torch.int8).argmax(1)                     # of equal ones the lowest index
     w = torch.where(x == top, 1.0, torch.exp((x - top) / torch.where(greedy, 1.0, t)))

@@ -105,6 +105,46 @@ def test_where_candidates_lie(dtype, vocab, shape):
     _same(x.to(dtype), vocab, u, t, k, p, m)
 
 
+@pytest.mark.parametrize("vocab", [9001, 70001, 140001])
+@pytest.mark.parametrize("shape", ["near zero", "far below", "negative", "small", "huge", "with nan and inf"])
+def test_p_decides_anywhere(vocab, shape):
+    """A p alone over bf16 logits that lie near 0 beside large ones, far below the first ones of the row, below 0, among the smallest normal
+    numbers, among the largest, and beside NaN and infinities; temperatures that make most of them count."""
+    rows = 8
+    g = _gen(vocab + len(shape))
+    x = torch.randn(rows, vocab, device="cuda", generator=g)
+    heat = 1.0
+    if shape == "near zero":
+        x = x * 2.0 ** -16
+        x[:, 11] = 8.0
+        heat = 4.0
+    elif shape == "far below":
+        x[:, vocab // 9:] -= 1000.0
+        heat = 2000.0
+    elif shape == "negative":
+        x = -20.0 - 3 * x.abs()
+        heat = 3.0
+    elif shape == "small":
+        x = x * 2.0 ** -126
+        heat = 2.0 ** -126
+    elif shape == "huge":
+        x = x * 2.0 ** 125
+        heat = 2.0 ** 126
+    else:
+        x[:, ::7] = float("nan")
+        x[:, 1::7] = -x[:, 1::7].abs()
+        x[:, 2::7] = float("-inf")
+        x[::2, 3] = float("inf")
+    x = x.to(torch.bfloat16)
+    if shape == "small":
+        x = torch.where(x.float().abs() < 2.0 ** -126, 0.0, x.float()).to(torch.bfloat16)      # a subnormal logit counts as 0
+    u = torch.rand(rows, device="cuda", generator=g)
+    t = heat * torch.tensor([1.0, 0.5, 1.5, 1.0, 0.7, 1.0, 2.0, 0.3], device="cuda")
+    p = torch.tensor([0.1, 0.3, 0.5, 0.7, 0.9, 0.99, 0.9999, 0.6], device="cuda")
+    _same(x, vocab, u, t, None, p)
+    _same(x, vocab, u, t, None, p, torch.full((rows,), 0.05, device="cuda"))
+
+
 def test_ends_of_u_and_odd_numbers():
     x = torch.tensor([[1.0, 3.0, 2.0, 3.0, float("nan"), float("-inf")]] * 6, device="cuda")
     x[3, 1] = float("inf")
