@@ -6,6 +6,7 @@ value."""
 import pytest
 import torch
 
+from ml_framework_b200 import _lib
 from ml_framework_b200.ops import native, reference
 
 pytestmark = pytest.mark.gpu
@@ -103,6 +104,22 @@ def test_where_candidates_lie(dtype, vocab, shape):
     p = torch.tensor([0.9, 0.95, 0.99, 0.9, 1.0, 0.9, 0.5, 0.9, 1.0, 0.9999], device="cuda")
     m = torch.tensor([0, 0, 0, 0, 0.01, 0, 0, 0, 0, 0.001], device="cuda")
     _same(x.to(dtype), vocab, u, t, k, p, m)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_largest_vocabulary(dtype):
+    """2^20 tokens, and one more, which is refused."""
+    n = 1 << 20
+    g = _gen(20)
+    x = (3 * torch.randn(3, n + 8, device="cuda", generator=g)).to(dtype)
+    u = torch.rand(3, device="cuda", generator=g)
+    t = torch.tensor([0.7, 1.0, 1.3], device="cuda")
+    p = torch.tensor([0.9, 1.0, 0.95], device="cuda")
+    k = torch.tensor([0, 0, 700], dtype=torch.int32, device="cuda")
+    _same(x, n, u, t, k, p)
+    _same(x, n - 5, u, t, None, p)
+    with pytest.raises(_lib.MlfError, match="vocabulary"):
+        native.sample_rows(x, n + 1, u, t)
 
 
 @pytest.mark.parametrize("vocab", [9001, 70001, 140001])
