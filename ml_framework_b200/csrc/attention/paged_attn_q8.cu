@@ -26,7 +26,8 @@
 //
 // Few sequences are split over CTAs, which merge through distributed shared memory where they all run at once. Other figures (us,
 // floor): 1 x 700 5.3 (0.2: the chain length - table - tile - softmax and the merge), 13 x 2500 18 (9.3), 64 x 576 16 (8.9: one round of
-// CTAs, half of it their first loads), 24 x 900 of 40 heads 36 (26: 2.2 rounds).
+// CTAs, half of it their first loads), 24 x 900 of 40 heads 34 (26: 1.6 rounds), 600 x 900
+// 185 (169).
 #include <cooperative_groups.h>
 
 #include "../common/host.h"
@@ -154,7 +155,9 @@ paged_decode_q8_kernel(const DecodeQ8Params p, const __grid_constant__ CUtensorM
   __shared__ __align__(16) uint8_t s_new[2][Q8_D];
   __shared__ float s_new_scale[2];
   __shared__ float2 s_cs[ROPE ? Q8_D / 2 : 1];
-  const int b = blockIdx.x, hkv = blockIdx.y, sp = blockIdx.z;
+  // the heads of a sequence run side by side: their 128 bytes of a token are neighbours in memory (4800 CTAs of 900 tokens 246 us with the
+  // sequences side by side, 177 so)
+  const int b = blockIdx.x / p.Hkv, hkv = blockIdx.x - b * p.Hkv, sp = blockIdx.z;
   pdl_trigger();
   if (WHOLE) {
     if (threadIdx.x == 0) {
@@ -659,7 +662,7 @@ MLF_API int mlf_paged_decode_q8(const void* q, long long ldq, void* cache, float
   MLF_REQUIRE(G <= 16, "paged_decode_q8: group size %d not supported (1 to 16)", G);
   MLF_REQUIRE(block_size > 0 && max_blocks > 0 && num_blocks > 0 && splits > 0, "paged_decode_q8: bad sizes");
   MLF_REQUIRE((long long)max_blocks * block_size < (1LL << 31) - (1 << 20), "paged_decode_q8: block table of %d x %d tokens", max_blocks, block_size);
-  MLF_REQUIRE(Hkv <= 65535 && splits <= 65535, "paged_decode_q8: grid");
+  MLF_REQUIRE((long long)B * Hq < (1LL << 31) && splits <= 65535, "paged_decode_q8: grid");
   MLF_REQUIRE((splits <= DQ_CLUSTER && ws == nullptr) || (ws != nullptr && ws_elems >= (long long)B * Hq * splits * DQ_RED), "paged_decode_q8: workspace too small for %d splits", splits);
   MLF_REQUIRE((reinterpret_cast<uintptr_t>(cache) & 15) == 0, "paged_decode_q8: the cache must be 16-byte aligned");
   const bool rope = slots != nullptr;
@@ -688,11 +691,18 @@ MLF_API int mlf_paged_decode_q8(const void* q, long long ldq, void* cache, float
   p.early = inputs_static;
   const long long cache_rows = 2LL * num_blocks * block_size;
   const bool whole = block_size % DQ_TILE == 0 && cache_rows < (1LL << 31);
-  // Warps of a CTA: four, of which three CTAs fit an SM (a warp's ring is 16 KB), or with eight heads at most as many as bring all CTAs into
-  // one round: four CTAs of three, six of two. Two also where there are not more than two pairs of tiles. us with 4 / 3 / 2 warps: 512 CTAs
-  // of 576 tokens 19 / 16 / 19, 800 of 576 24 / 26 / 22, 2048 of 64 21 / 17 / 15, 2048 of 1024 82 / 83 / 84, 384 of 4096 60 / 66 / 81.
+  // Warps of a CTA (a warp's ring is 16 KB): three CTAs of four fit an SM, four of three, six of two. With up to eight heads the form whose
+  // rounds have the fewest places; of equal ones, and for short sequences in more than a round, the one with the fewest warps. us
+  // with 4 / 3 / 2 warps (places an SM in brackets): 480 CTAs of 900 tokens 31 / 24 / 31 (6, 4, 6), 720 37 / 43 / 34 (6, 8, 6), 960 47 /
+  // 46 / 54 (9, 8, 12), 1280 55 / 63 / 62 (9, 12, 12), 1600 69 / 68 / 66 (12, 12, 12), 2000 83 / 87 / 90 (15, 16, 18); 1280 of 300 30 / 30
+  // / 28, 2000 of 300 46 / 41 / 39, 4800 of 300 92 / 80 / 74.
   const long long ctas = (long long)B * Hkv * splits, sms = sm_count();
-  const int warps = !whole || G > 8 || ctas <= 3 * sms ? 4 : ctas <= 4 * sms ? 3 : ctas <= 6 * sms || max_seq_len <= 64LL * splits ? 2 : 4;
+  auto places = [&](int per_sm) { return (ctas + sms * per_sm - 1) / (sms * per_sm) * per_sm; };
+  int warps = 4;
+  if (whole && G <= 8) {
+    if (places(4) <= places(3)) warps = 3;
+    if (places(6) <= places(7 - warps) || (ctas > 6 * sms && max_seq_len <= 400LL * splits)) warps = 2;
+  }
   const int smem = whole ? dq_box_smem(warps) : DQ_SMEM;
   CUtensorMap tm = {};
   if (whole) {
@@ -715,7 +725,7 @@ MLF_API int mlf_paged_decode_q8(const void* q, long long ldq, void* cache, float
     set = true;
   }
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  MLF_CHECK_CUDA(launch_pdl_cluster(kernel, dim3(B, Hkv, splits), dim3(warps * 32), smem, dim3(1, 1, second ? 1 : splits), st, p, tm));
+  MLF_CHECK_CUDA(launch_pdl_cluster(kernel, dim3((unsigned)(B * Hkv), 1, splits), dim3(warps * 32), smem, dim3(1, 1, second ? 1 : splits), st, p, tm));
   count_launch();
   if (second) {
     MLF_CHECK_CUDA(launch_pdl(paged_decode_q8_merge_kernel, dim3((unsigned)(B * Hq)), dim3(Q8_D), 0, st, (const float*)ws, p.out, Hq, Hkv, G, splits));

@@ -491,15 +491,15 @@ def _decode_split(pairs: int, max_seq_len: int, sms: int) -> int:
 
 
 @lru_cache(maxsize=4096)
-def _decode_split_q8(pairs: int, max_seq_len: int, sms: int) -> int:
-    """Tokens per split of the 8-bit decode kernel for ``pairs`` (sequence, KV head) pairs on ``sms`` SMs: one round of three CTAs on
-    each, of which every one has 128 tokens at least, 256 where that makes more than eight splits, and a 96th of the
-    longest sequence; none up to 384 tokens, where the merge costs more than it saves. us with 8 KV heads: 1 x 200 none 4.8
-    (2: 6.1); 1 x 700 6 splits 5.4 (1: 8.4, 3: 6.6); 1 x 4000 16 7.7 (8: 8.3, 32: 9.7); 8 x 4000 6 17 (2: 24, 16: 23);
-    13 x 2500 4 18 (1: 27, 5: 25); 16 x 4096 3 27 (1: 39, 4: 37); 48 x 4096 none 58 (2: 63); 4 x 60001 13 86 (16: 108); one KV head,
-    1 x 60000 64 16 (32: 20, 435: 25)."""
-    most = 1 if max_seq_len <= 384 else max(min(8, -(-max_seq_len // 128)), min(96, max_seq_len // 256))
-    return -(-max_seq_len // max(1, min(3 * sms // pairs, most)))
+def _decode_splits_q8(pairs: int, max_seq_len: int, sms: int) -> int:
+    """Splits of the 8-bit decode kernel for ``pairs`` (sequence, KV head) pairs on ``sms`` SMs: one round of three CTAs on
+    each, of which every one has 128 tokens at least, 256 (all that its warps fetch at once) where that makes more than eight splits,
+    and 96 splits at most; none up to 384 tokens, where the merge costs more than it saves. us with 8 KV heads: 1 x 200 none 4.7
+    (2: 5.5); 1 x 700 6 splits 5.3 (1: 8.6, 3: 6.5); 1 x 4000 16 8.6 (8: 9.0, 11: 10.4, 32: 10.1); 8 x 4000 6 18 (2: 31, 4: 21, 16: 24);
+    13 x 2500 4 18 (1: 34, 3: 21, 5: 21); 16 x 4096 3 29 (1: 54, 2: 35, 4: 31); 48 x 4096 none 70 (2: 73); 4 x 60001 13 87 (8: 107,
+    16: 85); one KV head, 1 x 60000 96 20 (32: 22, 64: 19, 200: 23)."""
+    most = 1 if max_seq_len <= 384 else max(min(8, -(-max_seq_len // 128)), min(96, -(-max_seq_len // 256)))
+    return max(1, min(3 * sms // pairs, most))
 
 
 def _decode_q8(what: str, q: torch.Tensor, ldq: int, Hq: int, kv_cache, kv_scale, block_table, seq_lens, slots, max_seq_len: int, scale, split_tokens: int,
@@ -521,9 +521,10 @@ def _decode_q8(what: str, q: torch.Tensor, ldq: int, Hq: int, kv_cache, kv_scale
         return out.zero_()
     sms = _sm_count(torch._C._cuda_getDevice())
     if split_tokens <= 0:
-        split_tokens = _decode_split_q8(B * Hkv, max_seq_len, sms)
-    st = (max(split_tokens, 128) + 127) // 128 * 128
-    splits = max(1, (max_seq_len + st - 1) // st)
+        splits = _decode_splits_q8(B * Hkv, max_seq_len, sms)
+    else:
+        st = (max(split_tokens, 128) + 127) // 128 * 128
+        splits = max(1, (max_seq_len + st - 1) // st)
     # maximum, sum and output of each split; up to eight that are resident at once are merged within the launch
     within = splits <= 8 and (splits == 1 or B * Hkv * splits <= 3 * sms)
     ws = None if within else torch.empty(B * Hq * splits * 130, dtype=torch.float32, device=q.device)
