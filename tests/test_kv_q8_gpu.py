@@ -210,9 +210,10 @@ def test_attention_many_splits(dtype, split, bs, Hq):
 
 
 @pytest.mark.parametrize("dtype", KINDS)
-@pytest.mark.parametrize("B,n,Hq,Hkv", [(150, 333, 8, 4), (200, 300, 12, 4), (300, 60, 16, 8), (300, 130, 24, 8), (40, 100, 16, 8)])
+@pytest.mark.parametrize("B,n,Hq,Hkv", [(150, 333, 8, 4), (200, 300, 12, 4), (300, 60, 16, 8), (300, 130, 24, 8), (40, 100, 16, 8), (65, 450, 16, 8),
+                                        (130, 450, 8, 8), (160, 450, 16, 8), (300, 450, 4, 4)])
 def test_attention_forms_of_the_launch(dtype, B, n, Hq, Hkv):
-    """Four, three and two warps to a CTA: as many as bring the CTAs into one round, and short sequences; then with the append."""
+    """Four, three and two warps to a CTA: by the places that the rounds of CTAs take, and short sequences; then with the append."""
     g = _gen(B)
     lens = torch.randint(1, n + 1, (B,), generator=torch.Generator().manual_seed(B)).tolist()
     lens[0] = n
