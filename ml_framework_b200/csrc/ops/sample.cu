@@ -27,10 +27,10 @@
 // (5) After (3), (4) or no limit: the token from sums of 256 neighbours.
 //
 // Bound by the chain of passes and exchanges for few rows and by the instructions of the weights (some 40 each), the atomics of the
-// counts (some 16 clocks for 32 logits) and, with fp32 logits in (3), both for many. us for 1 / 256 rows of 128256 bf16 logits (floor
-// 0.04 / 10): largest logit 3 / 18, k = 50 with p 10 / 44, k = 1000 32 / 138, no limit 10 / 88, a p that keeps few 14 / 88, one that keeps
-// thousands 20 / 130 - 150, rows of all kinds - / 100; of fp32 logits (floor 0.08 / 20) a p
-// that keeps few 19 / 185, thousands 28 / 240.
+// counts (some 16 clocks for 32 logits) and, with fp32 logits in (3), both for many; rows that take longest start first where not all
+// run at once. us for 1 / 256 rows of 128256 bf16 logits (floor 0.04 / 10): largest logit 3 / 20, k = 50 with p 10 / 45, k = 1000
+// 32 / 138, no limit 10 / 89, a p that keeps few 14 / 94, one that keeps thousands 20 / 138 - 156, rows of all kinds - / 80; of fp32 logits
+// (floor 0.08 / 20) a p that keeps few 19 / 187, thousands 28 / 240.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <float.h>
@@ -56,12 +56,13 @@ constexpr int SM_COARSE = 512;                 // bins of the maxima
 constexpr int SM_LIST = 2048;                  // tokens that a list takes
 constexpr int SM_FEW = 128;                    // tokens that a p alone is expected to keep, where they are listed
 constexpr int SM_CLUSTER = 8;                  // CTAs per row, at most
+constexpr int SM_ORDER = 1024;                 // rows that a launch can put in order
 constexpr int SM_ONE = 40;                     // log2 of the weight of the largest logit
 
 struct SampleParams {
   const void* logits;
   long long ld;
-  int rows, vocab, steps, vec;
+  int rows, vocab, steps, vec, longest_first;
   const float *u, *temperature, *top_p, *min_p;
   const int* top_k;
   long long* tokens;
@@ -92,9 +93,9 @@ struct SampleSmem {
   u64 last;
   u64 warp[SM_WARPS];
   u64 res[5];
-  u64 group[SM_GROUPS * SM_CLUSTER];
+  alignas(16) u64 group[SM_GROUPS * SM_CLUSTER];
   unsigned exp2[32];
-  int n_local;
+  int n_local, row;
   alignas(16) uint4 held[1];                   // SM_HELD steps of logits, or the maxima of all steps, as far as the launch goes
 };
 
@@ -466,6 +467,61 @@ __device__ __forceinline__ void sm_add(SampleSmem& s, int b, u64 w) {
   if (up) atomicAdd(&s.hi[b], up);
 }
 
+// The q-th row where those that take longest come first: a p alone (0), no limit (1), a k or min_p alone (2), the largest logit (3).
+// Up to SM_ORDER rows; every CTA looks at all of them. 256 rows of 128256 logits: of all kinds 100 us in their order, 80 so; of one
+// kind 2 - 7 us more.
+__device__ __forceinline__ int sm_longest_first(const SampleParams& p, SampleSmem& s, int q) {
+  constexpr int PER = SM_ORDER / SM_THREADS, EACH = 4 * PER * SM_WARPS / 32;
+  int* counts = reinterpret_cast<int*>(s.group);            // [class][run of 512 rows][warp]
+  static_assert(4 * PER * SM_WARPS * 4 <= sizeof(s.group) && EACH % 4 == 0, "a few counts a lane");
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  int kind[PER], before[PER];
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    const int r = j * SM_THREADS + tid, at = min(r, p.rows - 1);
+    const float temp = p.temperature[at], top_p = p.top_p ? p.top_p[at] : 1.f, min_p = p.min_p ? p.min_p[at] : 0.f;
+    const int k = p.top_k ? p.top_k[at] : 0;
+    kind[j] = r >= p.rows ? 4 : !(temp >= 0x1p-90f) ? 3 : k > 0 && k < p.vocab ? 2 : top_p < 1.f ? 0 : min_p > 0.f ? 2 : 1;
+    before[j] = 0;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const unsigned all = __ballot_sync(0xffffffffu, kind[j] == c);
+      if (lane == 0) counts[(c * PER + j) * SM_WARPS + warp] = __popc(all);
+      if (kind[j] == c) before[j] = __popc(all & ((1u << lane) - 1u));
+    }
+  }
+  __syncthreads();
+  // every warp sums them up for itself
+  int n[EACH], sum = 0;
+#pragma unroll
+  for (int i = 0; i < EACH; i += 4) {
+    const int4 v = reinterpret_cast<const int4*>(counts)[(lane * EACH + i) / 4];
+    n[i] = v.x; n[i + 1] = v.y; n[i + 2] = v.z; n[i + 3] = v.w;
+  }
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) { const int c = n[i]; n[i] = sum; sum += c; }
+  int first = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int t = __shfl_up_sync(0xffffffffu, first, o);
+    if (lane >= o) first += t;
+  }
+  first -= sum;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    const int i = (min(kind[j], 3) * PER + j) * SM_WARPS + warp;
+    int place = before[j] + __shfl_sync(0xffffffffu, first, i / EACH);
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+      const int t = __shfl_sync(0xffffffffu, n[e], i / EACH);
+      place += e == i % EACH ? t : 0;
+    }
+    if (kind[j] < 4 && place == q) s.row = j * SM_THREADS + tid;
+  }
+  __syncthreads();
+  return s.row;
+}
+
 template <typename T, bool HELD>
 __global__ void __launch_bounds__(SM_THREADS, 2) sample_rows_kernel(const SampleParams p) {
   extern __shared__ __align__(16) uint8_t sm_raw[];
@@ -481,7 +537,7 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_rows_kernel(const Sample
   if (sizeof(T) == 2)
     for (int i = tid; i < SM_FINE / 4; i += SM_THREADS) reinterpret_cast<uint4*>(s.fine)[i] = make_uint4(0u, 0u, 0u, 0u);
   pdl_wait();
-  const int r = blockIdx.x / C;
+  const int r = p.longest_first ? sm_longest_first(p, s, blockIdx.x / C) : blockIdx.x / C;
   SampleRow<T, HELD> row;
   row.row = reinterpret_cast<const T*>(p.logits) + (long long)r * p.ld;
   row.vocab = p.vocab;
@@ -1158,8 +1214,8 @@ using namespace mlf;
 
 // CTAs per row: as many as a warp's steps need, none with less than 4096 logits; beyond that, more of them shorten the rows whose p keeps
 // most of a flat distribution, which take four times as long as one with a small k, and cost every row their exchanges.
-// us at 128256 bf16 logits with 1 / 2 / 4 / 8 CTAs: 256 rows of k = 50 34 / 43 / 59 / 85, without limits 89 / 88 / 97 / 113, of all kinds
-// 144 / 101 / 108 / 129; 33 rows of 50257 fp32 logits, k = 50 22 / 20 / 17 / 22, of all kinds 73 / 49 / 39 / 31 (two CTAs fit an SM, but
+// us at 128256 bf16 logits with 1 / 2 / 4 CTAs: 256 rows of k = 50 34 / 44 / 64, without limits 88 / 89 / 102, of all kinds 147 / 80 / 95;
+// with 1 / 2 / 4 / 8, 33 rows of 50257 fp32 logits, k = 50 22 / 20 / 17 / 22, of all kinds 73 / 49 / 39 / 31 (two CTAs fit an SM, but
 // clusters of eight only 32 times). So four CTAs for every SM, and clusters of eight where all run at once.
 static int sample_cluster(long long rows, int vocab) {
   int c = 1;
@@ -1182,6 +1238,7 @@ MLF_API int mlf_sample_rows(const void* logits, int is_fp32, long long rows, lon
   p.logits = logits; p.ld = ld; p.rows = (int)rows; p.vocab = vocab;
   p.steps = (vocab + C * SM_WARPS * SM_STEP - 1) / (C * SM_WARPS * SM_STEP);
   p.vec = (ld * (is_fp32 ? 4 : 2)) % 16 == 0 && (reinterpret_cast<uintptr_t>(logits) & 15) == 0;
+  p.longest_first = rows * C > 2 * sm_count() && rows <= SM_ORDER;
   p.u = u; p.temperature = temperature; p.top_k = top_k; p.top_p = top_p; p.min_p = min_p;
   p.tokens = tokens; p.logprobs = logprobs;
   const bool held = p.steps <= SM_HELD;

@@ -208,6 +208,24 @@ def test_a_row_does_not_depend_on_the_others():
         assert a.item() == every[i].item() and b.item() == lp[i].item()
 
 
+@pytest.mark.parametrize("rows", [200, 300, 513, 1000, 1024, 1025])
+def test_every_row_of_a_large_batch(rows):
+    """More rows than run at once, of all kinds in any order, without settings too: each gets its own token."""
+    vocab = 9000
+    g = _gen(rows)
+    x = (3 * torch.randn(rows, vocab, device="cuda", generator=g)).to(torch.bfloat16)
+    u = torch.rand(rows, device="cuda", generator=g)
+    t, k, p, m = _settings(rows, g, "kpm")
+    kind = torch.randint(0, 6, (rows,), device="cuda", generator=g)
+    t[kind == 0] = 0.0
+    k[(kind == 1) | (kind >= 4)] = 0
+    p[(kind == 2) | (kind == 5)] = 1.0
+    m[kind != 3] = 0.0
+    _same(x, vocab, u, t, k, p, m)
+    _same(x, vocab, u, t)
+    _same(x, vocab, u, t, None, p)
+
+
 def test_frequencies():
     """200 K draws of a known distribution: counts within six standard deviations."""
     n = 200_000
