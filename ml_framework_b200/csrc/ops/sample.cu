@@ -15,7 +15,8 @@
 // A cluster of CTAs takes a row, and each lane keeps its logits in shared memory where four steps of 256 a warp are enough; rows of
 // more are read again in every pass, from the caches, and their lanes' maxima of eight neighbours are kept instead. A pass costs
 // its arithmetic and an exchange through distributed shared memory.
-// (1) Largest logit, and mean and variance of a sample.
+// (1) Largest logit, and mean and variance of a sample; logits further below the largest than 40 T, masked ones above all, are not in it
+// and none beyond 29 T, which weigh nothing, is a candidate.
 // (2) Where k limits the row, or (fp32 logits) a p under which few tokens are expected: the bins of equal width that hold the k (128)
 // largest of the maxima of eight neighbours hold at least as many tokens, and hardly more. These go to a list in one CTA, where the
 // token is decided: eight logits cost one comparison in both passes.
@@ -551,7 +552,9 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_rows_kernel(const Sample
   const int top_k = p.top_k ? p.top_k[r] : 0;
   const bool greedy = !(temp >= 0x1p-90f) || min_p > 1.f;          // the first token of the order alone
 
-  // ---- (1) the largest logit, with its first index where that is the answer; mean and variance of the first step
+  // ---- (1) the largest logit, with its first index where that is the answer; mean and variance of the first step's logits, as far as the
+  // largest (of the warp, then of the CTA, then of all) does not make them masked ones
+  const float masked = 40.f * temp;
   float best = -INFINITY, sum = 0.f, square = 0.f;
   int best_st = 0, n_sum = 0;
   row.first_pass([&](int st, float v) {
@@ -578,9 +581,10 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_rows_kernel(const Sample
     if (row.steps > 0) {
       float x[8];
       row.values(0, x);
+      const float from = fmaxf(sm_value((unsigned)(top >> 32)) - masked, -0x1p60f);
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        if (x[j] > -INFINITY) { sum += x[j]; square += x[j] * x[j]; ++n_sum; }
+        if (x[j] > from) { sum += x[j]; square += x[j] * x[j]; ++n_sum; }
     }
     n_sum = __reduce_add_sync(0xffffffffu, n_sum);
 #pragma unroll
@@ -596,30 +600,43 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_rows_kernel(const Sample
   }
   __syncthreads();
   cl.barrier_wait();
-  if (tid < C) {                               // thread i tells CTA i
-    u64 t = 0, n = 0;
-    float f = 0.f, g = 0.f;
+  // largest logit (and index) of up to 32 parts, a part a lane; sums over the parts that are not masked beside it. The sums in lane 0.
+  auto combine = [&](u64& t, float& f, float& g, unsigned& n, int parts) {
+    const unsigned hi = (unsigned)(t >> 32), most = __reduce_max_sync(0xffffffffu, hi);
+    t = (u64)most << 32 | __reduce_max_sync(0xffffffffu, hi == most ? (unsigned)t : 0u);
+    if (greedy) return;
+    const bool in = sm_value(hi) >= sm_value(most) - masked;          // an empty lane: NaN
+    n = __reduce_add_sync(0xffffffffu, in ? n : 0u);
+    f = in ? f : 0.f;
+    g = in ? g : 0.f;
 #pragma unroll
-    for (int i = 0; i < SM_WARPS; ++i) {
-      t = max(t, s.group[i]);
-      f += __uint_as_float((unsigned)(s.group[SM_WARPS + i] >> 32));
-      g += __uint_as_float((unsigned)s.group[SM_WARPS + i]);
-      n += s.group[2 * SM_WARPS + i];
+    for (int o = SM_WARPS / 2; o > 0; o >>= 1)
+      if (o < parts) {
+        f += __shfl_xor_sync(0xffffffffu, f, o);
+        g += __shfl_xor_sync(0xffffffffu, g, o);
+      }
+  };
+  u64 fg = 0;
+  if (warp == 0) {
+    top = lane < SM_WARPS ? s.group[lane] : 0ull;
+    fg = lane < SM_WARPS ? s.group[SM_WARPS + lane] : 0ull;
+    unsigned n = lane < SM_WARPS ? (unsigned)s.group[2 * SM_WARPS + lane] : 0u;
+    sum = __uint_as_float((unsigned)(fg >> 32));
+    square = __uint_as_float((unsigned)fg);
+    combine(top, sum, square, n, SM_WARPS);
+    if (lane < C) {                            // lane i tells CTA i: all lanes below 16 have the sums
+      u64* to = cl.map_shared_rank(&s.slot[0][0][0], lane);
+      to[rank] = top;
+      to[SM_CLUSTER + rank] = (u64)__float_as_uint(sum) << 32 | __float_as_uint(square);
+      to[2 * SM_CLUSTER + rank] = n;
     }
-    u64* to = cl.map_shared_rank(&s.slot[0][0][0], tid);
-    to[rank] = t;
-    to[SM_CLUSTER + rank] = (u64)__float_as_uint(f) << 32 | __float_as_uint(g);
-    to[2 * SM_CLUSTER + rank] = n;
   }
   cl.sync();
-  float mean = 0.f, var = 0.f, n_mean = 0.f;
-  top = 0;
-  for (int i = 0; i < C; ++i) {
-    top = max(top, s.slot[0][0][i]);
-    mean += __uint_as_float((unsigned)(s.slot[0][1][i] >> 32));
-    var += __uint_as_float((unsigned)s.slot[0][1][i]);
-    n_mean += (float)(unsigned)s.slot[0][2][i];
-  }
+  top = lane < C ? s.slot[0][0][lane] : 0ull;
+  fg = lane < C ? s.slot[0][1][lane] : 0ull;
+  unsigned n_all = lane < C ? (unsigned)s.slot[0][2][lane] : 0u;
+  float mean = __uint_as_float((unsigned)(fg >> 32)), var = __uint_as_float((unsigned)fg);
+  combine(top, mean, var, n_all, SM_CLUSTER);
   const float m = sm_value((unsigned)(top >> 32));
   if (m == -INFINITY || greedy) {
     if (rank == 0 && tid == 0) {
@@ -628,8 +645,13 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_rows_kernel(const Sample
     }
     return;
   }
-  mean = __fdiv_rn(mean, n_mean);
-  var = __fdiv_rn(var, n_mean) - mean * mean;
+  mean = __shfl_sync(0xffffffffu, mean, 0);
+  var = __shfl_sync(0xffffffffu, var, 0);
+  const float n_mean = (float)n_all;
+  // what lies further below the largest logit weighs 2^-41 of it at most, nothing: it is in no list and in no bin's range
+  const float nothing = fmaxf(fminf(m, FLT_MAX) - 29.f * temp, -FLT_MAX);
+  mean = n_mean > 0.f ? fmaxf(__fdiv_rn(mean, n_mean), nothing) : nothing;
+  var = n_mean > 0.f ? fmaxf(__fdiv_rn(var, n_mean) - mean * mean, 0.f) : 0.f;
   SampleWeight<sizeof(T) == 2> weight;
   const double scale = 32. * 1.4426950408889634074 / (double)temp;
   weight.m = fminf(m, FLT_MAX);
@@ -765,7 +787,7 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_rows_kernel(const Sample
         const int i = row.index(st);
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-          if (x[j] > -INFINITY && wanted(x[j], false)) {
+          if (x[j] >= nothing && wanted(x[j], false)) {
             const int at = atomicAdd(&s.n_local, 1);
             if (at < room) to[at] = sm_entry(x[j], i + j);
           }
@@ -802,11 +824,11 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_rows_kernel(const Sample
       const float inv_t = __fdiv_rn(1.f, temp), t = sqrtf(2.f * __logf((float)p.vocab / SM_FEW));
       const float z = t - (2.30753f + 0.27061f * t) / (1.f + t * (0.99229f + 0.04481f * t));      // Hastings' approximation of the normal quantile
       const float bulk = __expf(__logf((float)p.vocab) + ((mean - m) + 0.5f * var * inv_t) * inv_t);
-      flat = bulk * normcdff(z - sqrtf(fmaxf(var, 0.f)) * inv_t) > (1.f - top_p) * (bulk + 2.f);
+      flat = bulk * normcdff(z - sqrtf(var) * inv_t) > (1.f - top_p) * (bulk + 2.f);
     }
     if (sizeof(T) == 2 && !need_k) {
       // ---- (3) for bf16
-      const float low = mean - 4.f * sqrtf(fmaxf(var, 0.f));
+      const float low = fmaxf(mean - 4.f * sqrtf(var), nothing);
       const int e_top = max(max((int)(__float_as_uint(m) >> 23 & 255u), (int)(__float_as_uint(low) >> 23 & 255u)), 16);
       const int most = e_top << 7 | 127;                    // magnitudes (15 bits) from here down: SM_FINE / 2 of them, no subnormal one
       u64 w_small = 0, w_low = 0;                           // weights of what is nearer to 0 than the bins, and of what lies below them
@@ -817,7 +839,7 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_rows_kernel(const Sample
           const int mag = (int)(b & 0x7fffu), d = most - mag;
           if ((unsigned)d < SM_FINE / 2 && mag <= 0x7f80) {
             atomicAdd(&s.fine[b & 0x8000u ? SM_FINE - 1 - d : d], 1u);
-          } else if (mag <= 0x7f80) {
+          } else if (__uint_as_float(b << 16) >= nothing) { // no NaN either
             const u64 v = weight(__uint_as_float(b << 16));
             if (d < 0) w_low += v;
             else w_small += v;
@@ -906,7 +928,7 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_rows_kernel(const Sample
       row.each([&](int st) {
         const float v = row.maximum(st);
         const int b = bin_of(v);
-        if (v > -INFINITY && b < SM_COARSE - 1) atomicAdd(&s.cnt[b], 1u);
+        if (v >= nothing && b < SM_COARSE - 1) atomicAdd(&s.cnt[b], 1u);
         if (!need_k) {
           float x[8];
           row.values(st, x);
@@ -919,7 +941,7 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_rows_kernel(const Sample
       const SampleSplit sp = sm_find_coarse(cl, s, C, need_k ? (u64)top_k : (u64)SM_FEW);
       const int upto = sp.bin < SM_COARSE ? (int)sp.bin : SM_COARSE - 1;           // fewer in the bins: everything
       room = min(SM_LIST, 2 * SM_LIST / C);
-      const int n = gather([&](float x, bool) { return x > -INFINITY && bin_of(x) <= upto; });
+      const int n = gather([&](float x, bool) { return x >= nothing && bin_of(x) <= upto; });
       if (n > 0) {
         if (rank == 0) {
           const int n_k = need_k ? min(top_k, n) : n;
@@ -1046,7 +1068,7 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_rows_kernel(const Sample
       // ---- (3) for fp32: down to where a third of what p leaves out is expected below; where that misses the deciding value, as far below
       // the mean as half of what the largest logit is above it
       const float inv_t = __fdiv_rn(1.f, temp);
-      const float deep = m - (mean + var * inv_t + sqrtf(fmaxf(var, 0.f)) * normcdfinvf(fmaxf(1.f - top_p, 1e-6f) * 0.33f));
+      const float deep = m - (mean + var * inv_t + sqrtf(var) * normcdfinvf(fmaxf(1.f - top_p, 1e-6f) * 0.33f));
       SampleSplit sp;
       unsigned in_bin;
       bool known = !flat;                      // the sum of all weights

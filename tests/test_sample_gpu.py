@@ -208,6 +208,29 @@ def test_a_row_does_not_depend_on_the_others():
         assert a.item() == every[i].item() and b.item() == lp[i].item()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("vocab", [9000, 130001])
+@pytest.mark.parametrize("mask", ["lowest", -1e4, -1e9, float("-inf")])
+@pytest.mark.parametrize("left", [1, 5, 600, 5000])
+def test_masked_by_a_large_number(dtype, vocab, mask, left):
+    """Few tokens left beside the type's lowest value, -1e4, -1e9 or -inf, at places that no sample of the row needs to meet."""
+    rows = 12
+    g = _gen(left)
+    x = torch.full((rows, vocab), torch.finfo(dtype).min if mask == "lowest" else mask, device="cuda")
+    at = torch.rand(rows, vocab, device="cuda", generator=g).topk(left, 1)[1]
+    if left == 600:
+        at = torch.arange(vocab - left, vocab, device="cuda").expand(rows, -1)
+    x.scatter_(1, at, 3 * torch.randn(rows, left, device="cuda", generator=g))
+    x = x.to(dtype)
+    u = torch.rand(rows, device="cuda", generator=g)
+    t = torch.tensor([1.0, 0.0, 0.5, 1.0, 0.7, 1.3], device="cuda").repeat(2)
+    k = torch.tensor([0, 0, 50, 0, 3000, 700], dtype=torch.int32, device="cuda").repeat(2)
+    p = torch.tensor([0.9, 0.9, 0.9, 1.0, 0.95, 1.0], device="cuda").repeat(2)
+    m = torch.tensor([0.0] * 6 + [0.05] * 6, device="cuda")
+    _same(x, vocab, u, t, k, p, m)
+    _same(x, vocab, u, t, None, p)
+
+
 @pytest.mark.parametrize("rows", [200, 300, 513, 1000, 1024, 1025])
 def test_every_row_of_a_large_batch(rows):
     """More rows than run at once, of all kinds in any order, without settings too: each gets its own token."""
