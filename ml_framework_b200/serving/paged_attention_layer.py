@@ -97,7 +97,7 @@ class PagedAttentionLayer(nn.Module):
         table, lens = kv.build_tables(list(seq_ids), max_blocks, dev)
         if phase == AttentionPhase.DECODE:
             if nat:
-                a = native.paged_decode(q, cache, table, lens, int(max(st + 1 for st in starts)), kv_scale=scale)
+                a = native.paged_decode(q, cache, table, lens, int(max(st + 1 for st in starts)), split_tokens=512 if scale is None else 0, kv_scale=scale)
             else:
                 a = reference.paged_attention_ref(q.float(), reference.kv_values_ref(cache, scale), table, lens).to(x.dtype)
         else:
