@@ -29,8 +29,8 @@ struct Q8WriteParams {
   const __nv_bfloat16 *k, *v;
   const long long* slots;
   int* map;                                   // [num_blocks * block_size]; null: every CTA looks through the slots
-  long long T, ldk, ldv;
-  int Hkv, block_size, bs_shift, num_blocks, group;       // bs_shift: log2(block_size) or -1
+  long long T;
+  int ldk, ldv, Hkv, block_size, bs_shift, num_blocks, group;       // bs_shift: log2(block_size) or -1
   int* err;
 };
 
@@ -95,20 +95,27 @@ __device__ __forceinline__ void q8_write_rows(const Q8WriteParams& p, int blk, i
   const int lane = threadIdx.x & 31, half = lane >> 4, col = (lane & 15) * 8;
   const long long first = (long long)blk * p.block_size, pitch = (long long)p.Hkv * Q8_D;
   const __nv_bfloat16* src = (side ? p.v : p.k) + (long long)h * Q8_D + col;
-  const long long ld = side ? p.ldv : p.ldk;
+  const int ld = side ? p.ldv : p.ldk;
   uint8_t* dst = p.cache + (((long long)blk * 2 + side) * p.block_size * p.Hkv + h) * Q8_D + col + half * pitch;
   float* scale = p.scale + ((long long)blk * 2 + side) * p.Hkv + h;
   const int chunks = (p.block_size + 15) / 16;
   uint4 x[8];
   int tok = -1;                               // lanes 0..15: the token of row chunk * 16 + lane
+  bool whole = false;                         // every row of the chunk is written: no row decides anything by itself
   auto load = [&](int c) {
     const int row = c * 16 + lane;
     tok = -1;
     if (lane < 16 && row < p.block_size) tok = p.map == nullptr || c == 0 ? known[row] : q8_token_at(p, first + row);
+    whole = __all_sync(0xffffffffu, lane >= 16 || tok >= 0);
+    if (whole) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = *reinterpret_cast<const uint4*>(src + (long long)__shfl_sync(0xffffffffu, tok, 2 * i + half) * ld);
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int t = __shfl_sync(0xffffffffu, tok, 2 * i + half);
-      x[i] = t >= 0 ? *reinterpret_cast<const uint4*>(src + t * ld) : make_uint4(0u, 0u, 0u, 0u);
+      x[i] = t >= 0 ? *reinterpret_cast<const uint4*>(src + (long long)t * ld) : make_uint4(0u, 0u, 0u, 0u);
     }
   };
   const float held_scale = *scale;
@@ -137,6 +144,14 @@ __device__ __forceinline__ void q8_write_rows(const Q8WriteParams& p, int blk, i
   for (int c = 0; c < chunks; ++c) {
     if (chunks > 1) load(c);
     uint8_t* to = dst + c * 16 * pitch;
+    if (whole && (FMT == Q8_E4M3 || plain)) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        *reinterpret_cast<uint2*>(to) = q8_pack8<FMT>(x[i], inv, true);
+        to += 2 * pitch;
+      }
+      continue;
+    }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int t = __shfl_sync(0xffffffffu, tok, 2 * i + half);
@@ -290,6 +305,7 @@ MLF_API int mlf_kv_write_q8(void* cache, float* scale, int fmt, const void* k, c
   if (T <= 0) return 0;
   MLF_REQUIRE(fmt == Q8_E4M3 || fmt == Q8_INT8, "kv_write_q8: format %d", fmt);
   MLF_REQUIRE(Hkv > 0 && block_size > 0 && num_blocks > 0 && T < (1LL << 31), "kv_write_q8: bad sizes");
+  MLF_REQUIRE(ldk >= 0 && ldv >= 0 && ldk < (1LL << 31) && ldv < (1LL << 31), "kv_write_q8: rows %lld and %lld elements apart", ldk, ldv);
   MLF_REQUIRE(ldk % 8 == 0 && ldv % 8 == 0 && ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(cache)) & 15) == 0,
               "kv_write_q8: rows and cache must be 16-byte aligned");
   Q8WriteParams p;
@@ -303,7 +319,7 @@ MLF_API int mlf_kv_write_q8(void* cache, float* scale, int fmt, const void* k, c
   const bool few = T <= QW_FEW && block_size <= QW_ROWS;
   MLF_REQUIRE(few || map != nullptr, "kv_write_q8: %lld tokens into blocks of %d need a map", T, block_size);
   p.map = few ? nullptr : map;
-  p.T = T; p.ldk = ldk; p.ldv = ldv;
+  p.T = T; p.ldk = (int)ldk; p.ldv = (int)ldv;
   p.Hkv = Hkv; p.block_size = block_size; p.num_blocks = num_blocks;
   p.group = T > 256 ? QW_GROUP : 1;           // few tokens: often one to a block, and too few CTAs otherwise
   p.err = device_status_word();
