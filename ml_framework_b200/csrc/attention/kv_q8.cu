@@ -9,7 +9,8 @@
 // nothing at all, point at tokens of other slots.
 //
 // Bound by HBM in long calls (a row is read in 16 bits and written in 8), by the chain of loads slots - rows (slots - map - slots -
-// rows) in short ones. us (floor at 6.54 TB/s): 37 tokens of 8 heads 5 (0.03), 2048 10 (1.9), 8192 17 (7.7), 4096 of 40 heads 40 (19).
+// rows) in short ones. us (floor at 6.54 TB/s): 37 tokens of 8 heads 5 (0.03), 2048 10 (1.9), 8192 18 (7.7), 32768 50 (31), 4096 of 40
+// heads 34 (19).
 // The way back, q8_gather_kernel: 3159 tokens of 8 heads 5 - 7 (3.0), 8192 8 - 10 (7.7).
 #include "../common/host.h"
 #include "../common/ptx.cuh"
@@ -172,21 +173,23 @@ __global__ void __launch_bounds__(QW_WARPS * 32, 4) q8_write_kernel(const Q8Writ
   pdl_wait();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const long long from = (long long)blockIdx.x * p.group, end = (long long)p.num_blocks * p.block_size;
-  if (p.map == nullptr) {
-    // the blocks of the group, each once; then every token of the call that goes to one of them
-    if (warp == 0) {
-      const long long slot = lane < p.group && from + lane < p.T ? p.slots[from + lane] : -1;
-      if (slot >= end) atomicCAS(p.err, 0, ERR_BAD_INDEX);
-      const int blk = slot >= 0 && slot < end ? q8_block(p, slot) : -1;
-      const unsigned same = __match_any_sync(0xffffffffu, blk);        // every lane takes part
-      const bool once = blk >= 0 && __ffs(same) - 1 == lane;
-      const unsigned all = __ballot_sync(0xffffffffu, once);
-      if (once) s_blk[__popc(all & ((1u << lane) - 1u))] = blk;
-      if (lane == 0) s_blocks = __popc(all);
-    }
+  // the blocks of the group, each once
+  if (warp == 0) {
+    const long long slot = lane < p.group && from + lane < p.T ? p.slots[from + lane] : -1;
+    if (slot >= end) atomicCAS(p.err, 0, ERR_BAD_INDEX);
+    const int blk = slot >= 0 && slot < end ? q8_block(p, slot) : -1;
+    const unsigned same = __match_any_sync(0xffffffffu, blk);          // every lane takes part
+    const bool once = blk >= 0 && __ffs(same) - 1 == lane;
+    const unsigned all = __ballot_sync(0xffffffffu, once);
+    if (once) s_blk[__popc(all & ((1u << lane) - 1u))] = blk;
+    if (lane == 0) s_blocks = __popc(all);
+  }
+  if (p.map == nullptr)
     for (int i = tid; i < QW_GROUP * QW_ROWS; i += QW_WARPS * 32) (&s_tok[0][0])[i] = 0x7fffffff;
-    __syncthreads();
-    const int n = s_blocks;
+  __syncthreads();
+  const int n = s_blocks;
+  if (p.map == nullptr) {
+    // every token of the call that goes to one of them
     constexpr int EACH = QW_FEW / (QW_WARPS * 32);
     long long slots[EACH];
 #pragma unroll
@@ -202,40 +205,25 @@ __global__ void __launch_bounds__(QW_WARPS * 32, 4) q8_write_kernel(const Q8Writ
         if (s_blk[i] == blk) atomicMin(&s_tok[i][slots[j] - (long long)blk * p.block_size], tid + j * QW_WARPS * 32);
     }
     __syncthreads();
-    for (int i = warp; i < n; i += QW_WARPS) {
-      int first = -1;
-      for (int r0 = 0; r0 < p.block_size; r0 += 32) {
-        const int r = r0 + lane, t = r < p.block_size ? s_tok[i][r] : 0x7fffffff;
-        const unsigned there = __ballot_sync(0xffffffffu, t != 0x7fffffff);
-        if (first < 0 && there != 0) first = __shfl_sync(0xffffffffu, t, __ffs(there) - 1);
-        __syncwarp();
-        if (r < p.block_size && t == 0x7fffffff) s_tok[i][r] = -1;
-      }
-      if (lane == 0 && (first < from || first >= from + p.group)) s_blk[i] = -1;                   // another CTA's
+  }
+  // the tokens of a block's rows (with a map, of the first 16), and the first one of them, whose CTA writes the block
+  for (int i = warp; i < n; i += QW_WARPS) {
+    int first = -1;
+    for (int r0 = 0; r0 < p.block_size && (first < 0 || p.map == nullptr); r0 += 32) {
+      const int r = r0 + lane;
+      int t = -1;
+      if (r < p.block_size) t = p.map == nullptr ? s_tok[i][r] : q8_token_at(p, (long long)s_blk[i] * p.block_size + r);
+      if (t == 0x7fffffff) t = -1;
+      const unsigned there = __ballot_sync(0xffffffffu, t >= 0);
+      if (first < 0 && there != 0) first = __shfl_sync(0xffffffffu, t, __ffs(there) - 1);
+      if (r < p.block_size && (p.map == nullptr || r < 16)) s_tok[i][r] = t;
     }
-  } else {
-    if (tid == 0) s_blocks = p.group;
-    for (int i = warp; i < p.group; i += QW_WARPS) {
-      const long long t = from + i, slot = t < p.T ? p.slots[t] : -1;
-      int blk = -1;
-      if (slot >= 0 && slot < end) {
-        blk = q8_block(p, slot);
-        const long long first = (long long)blk * p.block_size;
-        const int off = (int)(slot - first);
-        bool mine = p.map[slot] == (int)t;
-        for (int r0 = 0; r0 <= off && mine; r0 += 32) {
-          const int r = r0 + lane, at = r < p.block_size ? q8_token_at(p, first + r) : -1;
-          if (r < 16) s_tok[i][r] = at;
-          if (__any_sync(0xffffffffu, at >= 0 && r < off)) mine = false;
-        }
-        if (!mine) blk = -1;
-      }
-      if (lane == 0) s_blk[i] = blk;
-    }
+    __syncwarp();
+    if (lane == 0 && (first < from || first >= from + p.group)) s_blk[i] = -1;                         // another CTA's
   }
   __syncthreads();
-  const int units = 2 * p.Hkv, blocks = s_blocks;
-  for (int i = 0; i < blocks; ++i) {
+  const int units = 2 * p.Hkv;
+  for (int i = 0; i < n; ++i) {
     if (s_blk[i] < 0) continue;
     for (int u = blockIdx.y * QW_WARPS + warp; u < units; u += gridDim.y * QW_WARPS) q8_write_rows<FMT>(p, s_blk[i], u >> 1, u & 1, s_tok[i]);
   }
