@@ -9,8 +9,8 @@
 // nothing at all, point at tokens of other slots.
 //
 // Bound by HBM in long calls (a row is read in 16 bits and written in 8), by the chain of loads slots - rows (slots - map - slots -
-// rows) in short ones. us (floor at 6.54 TB/s): 37 tokens of 8 heads 5 (0.03), 2048 10 (1.9), 8192 18 (7.7), 32768 50 (31), 4096 of 40
-// heads 34 (19).
+// rows) in short ones. us (floor at 6.54 TB/s): 37 tokens of 8 heads 4 (0.03), 1111 6 (1.0), 2048 9 (1.9), 8192 17 (7.7), 32768 50 (31),
+// 4096 of 40 heads 33 (19).
 // The way back, q8_gather_kernel: 3159 tokens of 8 heads 5 - 7 (3.0), 8192 8 - 10 (7.7).
 #include "../common/host.h"
 #include "../common/ptx.cuh"
@@ -91,7 +91,7 @@ __device__ __noinline__ void q8_shrink8(uint2* at, float ratio) {
 }
 
 // A block's rows of one head and side. known: the tokens of its rows (-1: not written by this call), the first 16 of them with a map.
-template <int FMT>
+template <int FMT, bool MAP>
 __device__ __forceinline__ void q8_write_rows(const Q8WriteParams& p, int blk, int h, int side, const int* known) {
   const int lane = threadIdx.x & 31, half = lane >> 4, col = (lane & 15) * 8;
   const long long first = (long long)blk * p.block_size, pitch = (long long)p.Hkv * Q8_D;
@@ -106,7 +106,7 @@ __device__ __forceinline__ void q8_write_rows(const Q8WriteParams& p, int blk, i
   auto load = [&](int c) {
     const int row = c * 16 + lane;
     tok = -1;
-    if (lane < 16 && row < p.block_size) tok = p.map == nullptr || c == 0 ? known[row] : q8_token_at(p, first + row);
+    if (lane < 16 && row < p.block_size) tok = !MAP || c == 0 ? known[row] : q8_token_at(p, first + row);
     whole = __all_sync(0xffffffffu, lane >= 16 || tok >= 0);
     if (whole) {
 #pragma unroll
@@ -164,10 +164,12 @@ __device__ __forceinline__ void q8_write_rows(const Q8WriteParams& p, int blk, i
   if (lane == 0) *scale = now;
 }
 
+// Three CTAs on an SM without a map, four with one: registers against loads in flight (us with three / four: 37 tokens of 8 heads 4.1 / 5.1,
+// 1111 6.2 / 7.8, 8192 19.6 / 17.4, 4096 of 40 heads 39 / 33).
 // A CTA looks at the blocks of `group` tokens and writes those whose first row, of the rows that the call writes there, one of these
 // tokens is; the heads and sides are split over blockIdx.y.
-template <int FMT>
-__global__ void __launch_bounds__(QW_WARPS * 32, 4) q8_write_kernel(const Q8WriteParams p) {
+template <int FMT, bool MAP>
+__global__ void __launch_bounds__(QW_WARPS * 32, MAP ? 4 : 3) q8_write_kernel(const Q8WriteParams p) {
   __shared__ int s_blk[QW_GROUP], s_tok[QW_GROUP][QW_ROWS], s_blocks;
   pdl_trigger();
   pdl_wait();
@@ -184,11 +186,11 @@ __global__ void __launch_bounds__(QW_WARPS * 32, 4) q8_write_kernel(const Q8Writ
     if (once) s_blk[__popc(all & ((1u << lane) - 1u))] = blk;
     if (lane == 0) s_blocks = __popc(all);
   }
-  if (p.map == nullptr)
+  if (!MAP)
     for (int i = tid; i < QW_GROUP * QW_ROWS; i += QW_WARPS * 32) (&s_tok[0][0])[i] = 0x7fffffff;
   __syncthreads();
   const int n = s_blocks;
-  if (p.map == nullptr) {
+  if (!MAP) {
     // every token of the call that goes to one of them
     constexpr int EACH = QW_FEW / (QW_WARPS * 32);
     long long slots[EACH];
@@ -209,14 +211,14 @@ __global__ void __launch_bounds__(QW_WARPS * 32, 4) q8_write_kernel(const Q8Writ
   // the tokens of a block's rows (with a map, of the first 16), and the first one of them, whose CTA writes the block
   for (int i = warp; i < n; i += QW_WARPS) {
     int first = -1;
-    for (int r0 = 0; r0 < p.block_size && (first < 0 || p.map == nullptr); r0 += 32) {
+    for (int r0 = 0; r0 < p.block_size && (first < 0 || !MAP); r0 += 32) {
       const int r = r0 + lane;
       int t = -1;
-      if (r < p.block_size) t = p.map == nullptr ? s_tok[i][r] : q8_token_at(p, (long long)s_blk[i] * p.block_size + r);
+      if (r < p.block_size) t = !MAP ? s_tok[i][r] : q8_token_at(p, (long long)s_blk[i] * p.block_size + r);
       if (t == 0x7fffffff) t = -1;
       const unsigned there = __ballot_sync(0xffffffffu, t >= 0);
       if (first < 0 && there != 0) first = __shfl_sync(0xffffffffu, t, __ffs(there) - 1);
-      if (r < p.block_size && (p.map == nullptr || r < 16)) s_tok[i][r] = t;
+      if (r < p.block_size && (!MAP || r < 16)) s_tok[i][r] = t;
     }
     __syncwarp();
     if (lane == 0 && (first < from || first >= from + p.group)) s_blk[i] = -1;                         // another CTA's
@@ -225,7 +227,7 @@ __global__ void __launch_bounds__(QW_WARPS * 32, 4) q8_write_kernel(const Q8Writ
   const int units = 2 * p.Hkv;
   for (int i = 0; i < n; ++i) {
     if (s_blk[i] < 0) continue;
-    for (int u = blockIdx.y * QW_WARPS + warp; u < units; u += gridDim.y * QW_WARPS) q8_write_rows<FMT>(p, s_blk[i], u >> 1, u & 1, s_tok[i]);
+    for (int u = blockIdx.y * QW_WARPS + warp; u < units; u += gridDim.y * QW_WARPS) q8_write_rows<FMT, MAP>(p, s_blk[i], u >> 1, u & 1, s_tok[i]);
   }
 }
 static_assert(QW_GROUP <= 32, "a lane for every token of a group");
@@ -316,7 +318,8 @@ MLF_API int mlf_kv_write_q8(void* cache, float* scale, int fmt, const void* k, c
   // a CTA finds its blocks once for all heads that it takes: about as many of them as fit, four to an SM
   const long long x = (T + p.group - 1) / p.group, most = (2 * Hkv + QW_WARPS - 1) / QW_WARPS, fill = 4LL * sm_count() / x > 0 ? 4LL * sm_count() / x : 1;
   const dim3 grid((unsigned)x, (unsigned)(fill < most ? fill : most));
-  const auto kernel = fmt == Q8_E4M3 ? q8_write_kernel<Q8_E4M3> : q8_write_kernel<Q8_INT8>;
+  const auto kernel = fmt == Q8_E4M3 ? (few ? q8_write_kernel<Q8_E4M3, false> : q8_write_kernel<Q8_E4M3, true>)
+                                     : (few ? q8_write_kernel<Q8_INT8, false> : q8_write_kernel<Q8_INT8, true>);
   MLF_CHECK_CUDA(launch_pdl(kernel, grid, dim3(QW_WARPS * 32), 0, st, p));
   count_launch(p.map != nullptr ? 2 : 1);
   return 0;
