@@ -248,7 +248,7 @@ paged_decode_q8_kernel(const DecodeQ8Params p, const __grid_constant__ CUtensorM
   auto issue = [&](int i) {                    // this warp's i-th pair
     const int first = t_lo + (warp + i * W) * SPAN;
     const uint32_t st = ring + (i % DQ_STAGES) * STAGE;
-    if (WHOLE) {
+    if constexpr (WHOLE) {
       if ((i & ~15) != pages_from) {
         pages_from = i & ~15;
         const int t = t_lo + (warp + (pages_from + (lane >> 1)) * W) * SPAN + (lane & 1) * DQ_TILE;
@@ -271,27 +271,27 @@ paged_decode_q8_kernel(const DecodeQ8Params p, const __grid_constant__ CUtensorM
           tma_load_2d(st + h * TILE_BYTES + DQ_TILE * Q8_D, &tm, hkv * Q8_D, row + p.block_size, bar);
         }
       }
-      return;
-    }
+    } else {
 #pragma unroll
-    for (int h = 0; h < DQ_PAIR; ++h) {
-      const uint32_t to = st + h * TILE_BYTES;
-      const int t = first + h * DQ_TILE + (lane & 15), tt = t < t_hi ? t : t_lo;
-      const int blk = block_of(tt), at = t < t_hi ? t - blk * p.block_size : -1;
-      const int page = checked(bt[blk]);
-      dq_copy4(to + 2 * DQ_TILE * Q8_D + lane * 4, p.scale + ((long long)page * 2 + (lane >> 4)) * p.Hkv + hkv, at >= 0 ? 4 : 0);
+      for (int h = 0; h < DQ_PAIR; ++h) {
+        const uint32_t to = st + h * TILE_BYTES;
+        const int t = first + h * DQ_TILE + (lane & 15), tt = t < t_hi ? t : t_lo;
+        const int blk = block_of(tt), at = t < t_hi ? t - blk * p.block_size : -1;
+        const int page = checked(bt[blk]);
+        dq_copy4(to + 2 * DQ_TILE * Q8_D + lane * 4, p.scale + ((long long)page * 2 + (lane >> 4)) * p.Hkv + hkv, at >= 0 ? 4 : 0);
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {            // rows g and g + 8 of the keys, 16-byte columns 2c and 2c + 1
-        const int pg = __shfl_sync(0xffffffffu, page, g + 8 * j), r = __shfl_sync(0xffffffffu, at, g + 8 * j);
-        const uint8_t* src = p.cache + pg * blk_bytes + max(r, 0) * row_bytes + hkv * Q8_D + c * 32;
-        dq_copy16(to + (j * 2) * 512 + lane * 16, src, r >= 0 ? 16 : 0);
-        dq_copy16(to + (j * 2 + 1) * 512 + lane * 16, src + 16, r >= 0 ? 16 : 0);
-      }
+        for (int j = 0; j < 2; ++j) {            // rows g and g + 8 of the keys, 16-byte columns 2c and 2c + 1
+          const int pg = __shfl_sync(0xffffffffu, page, g + 8 * j), r = __shfl_sync(0xffffffffu, at, g + 8 * j);
+          const uint8_t* src = p.cache + pg * blk_bytes + max(r, 0) * row_bytes + hkv * Q8_D + c * 32;
+          dq_copy16(to + (j * 2) * 512 + lane * 16, src, r >= 0 ? 16 : 0);
+          dq_copy16(to + (j * 2 + 1) * 512 + lane * 16, src + 16, r >= 0 ? 16 : 0);
+        }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {            // rows 2c, 2c + 1, 2c + 8, 2c + 9 of the values, column g
-        const int tr = 2 * c + (j & 1) + 8 * (j >> 1);
-        const int pg = __shfl_sync(0xffffffffu, page, tr), r = __shfl_sync(0xffffffffu, at, tr);
-        dq_copy16(to + DQ_TILE * Q8_D + j * 512 + lane * 16, p.cache + pg * blk_bytes + v_off + max(r, 0) * row_bytes + hkv * Q8_D + g * 16, r >= 0 ? 16 : 0);
+        for (int j = 0; j < 4; ++j) {            // rows 2c, 2c + 1, 2c + 8, 2c + 9 of the values, column g
+          const int tr = 2 * c + (j & 1) + 8 * (j >> 1);
+          const int pg = __shfl_sync(0xffffffffu, page, tr), r = __shfl_sync(0xffffffffu, at, tr);
+          dq_copy16(to + DQ_TILE * Q8_D + j * 512 + lane * 16, p.cache + pg * blk_bytes + v_off + max(r, 0) * row_bytes + hkv * Q8_D + g * 16, r >= 0 ? 16 : 0);
+        }
       }
     }
   };

@@ -413,16 +413,17 @@ def _at(t: Optional[torch.Tensor]) -> Optional[int]:
     return t.data_ptr() if t is not None else None
 
 
-def _stream() -> int:
-    return _lib.stream_handle()
+def _stream(device_index: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(device_index)
 
 
-def _on_current_device(what: str, *tensors: Optional[torch.Tensor]):
-    """Launches go to the current device's stream: tensors of another device, or of the host, are refused."""
+def _on_current_device(what: str, *tensors: Optional[torch.Tensor]) -> int:
+    """Launches go to the current device's stream: tensors of another device, or of the host, are refused. The device's index."""
     here = torch._C._cuda_getDevice() if torch.cuda.is_initialized() else 0
     for t in tensors:
         if t is not None and t.get_device() != here:
             raise ValueError(f"{what}: a tensor is on {t.device}, the kernel runs on the current CUDA device")
+    return here
 
 
 def _q8_cache(what: str, kv_cache: torch.Tensor, kv_scale: Optional[torch.Tensor]) -> Tuple[int, int, int, int]:
@@ -513,13 +514,13 @@ def _decode_q8(what: str, q: torch.Tensor, ldq: int, Hq: int, kv_cache, kv_scale
         raise ValueError(f"{what}: block_table must be int32 [{B}, max_blocks], got {block_table.dtype} {tuple(rows)}")
     table, lens = block_table.contiguous(), _index(what, "seq_lens", seq_lens, torch.int32, B)
     slots = _index(what, "slots", slots, torch.int64, B) if slots is not None else None
-    _on_current_device(what, q, kv_cache, kv_scale, table, lens, slots)
+    dev = _on_current_device(what, q, kv_cache, kv_scale, table, lens, slots)
     out = q.new_empty((B, Hq, 128))
     if B == 0:
         return out
     if rows[1] == 0:
         return out.zero_()
-    sms = _sm_count(torch._C._cuda_getDevice())
+    sms = _sm_count(dev)
     if split_tokens <= 0:
         splits = _decode_splits_q8(B * Hkv, max_seq_len, sms)
     else:
@@ -531,7 +532,7 @@ def _decode_q8(what: str, q: torch.Tensor, ldq: int, Hq: int, kv_cache, kv_scale
     rc = _function("mlf_paged_decode_q8", "plppipppppliiiiiiiiffiu")(
         q.data_ptr(), ldq, kv_cache.data_ptr(), kv_scale.data_ptr(), fmt, table.data_ptr(), lens.data_ptr(), _at(slots), out.data_ptr(), _at(ws),
         0 if ws is None else ws.numel(), B, Hq, Hkv, bs, rows[1], nb, max_seq_len, splits,
-        scale if scale is not None else 128 ** -0.5, theta, int(inputs_static), _stream())
+        scale if scale is not None else 128 ** -0.5, theta, int(inputs_static), _stream(dev))
     _lib.check(rc, "mlf_paged_decode_q8")
     return out
 
@@ -625,12 +626,12 @@ def paged_decode_rope(qkv: torch.Tensor, kv_cache: torch.Tensor, block_table: to
     return out
 
 
-def _write_q8(kv_cache, kv_scale, layout: Tuple[int, int, int, int], k: int, v: int, slots: torch.Tensor, T: int, ldk: int, ldv: int):
+def _write_q8(dev: int, kv_cache, kv_scale, layout: Tuple[int, int, int, int], k: int, v: int, slots: torch.Tensor, T: int, ldk: int, ldv: int):
     """T rows at the addresses ``k`` and ``v``, checked by the callers."""
     fmt, nb, bs, Hkv = layout
     where = kv_cache.new_empty(nb * bs, dtype=torch.int32) if T > 2048 or bs > 64 else None
     rc = _function("mlf_kv_write_q8", "ppippppliiillu")(kv_cache.data_ptr(), kv_scale.data_ptr(), fmt, k, v, slots.data_ptr(), _at(where), T, Hkv, bs, nb,
-                                                        ldk, ldv, _stream())
+                                                        ldk, ldv, _stream(dev))
     _lib.check(rc, "mlf_kv_write_q8")
 
 
@@ -651,9 +652,9 @@ def kv_cache_write(kv_cache: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slo
         if v.shape[0] != T:
             raise ValueError(f"{what}: {T} keys and {v.shape[0]} values")
         slots = _index(what, "slots", slots, torch.int64, T)
-        _on_current_device(what, kv_cache, kv_scale, k, v, slots)
+        dev = _on_current_device(what, kv_cache, kv_scale, k, v, slots)
         if T > 0 and kv_cache.numel() > 0:
-            _write_q8(kv_cache, kv_scale, (fmt, nb, bs, Hkv), k.data_ptr(), v.data_ptr(), slots, T, k.stride(0), v.stride(0))
+            _write_q8(dev, kv_cache, kv_scale, (fmt, nb, bs, Hkv), k.data_ptr(), v.data_ptr(), slots, T, k.stride(0), v.stride(0))
         return
     nb, _, bs, Hkv, D = kv_cache.shape
     T = k.shape[0]
@@ -678,13 +679,13 @@ def rope_kv_write_(qkv: torch.Tensor, pos: torch.Tensor, slots: torch.Tensor, kv
         if qkv.data_ptr() % 16 or qkv.stride(0) % 8:
             raise ValueError(f"{what}: rows must be 16-byte aligned")
         pos, slots = _index(what, "pos", pos, torch.int64, T), _index(what, "slots", slots, torch.int64, T)
-        _on_current_device(what, qkv, pos, slots, kv_cache, kv_scale)
+        dev = _on_current_device(what, qkv, pos, slots, kv_cache, kv_scale)
         if T == 0:
             return qkv
         rope_qkv(qkv, pos, Hq, Hkv, theta, out=qkv)
         if kv_cache.numel() > 0:
             k = qkv.data_ptr() + Hq * 256
-            _write_q8(kv_cache, kv_scale, layout, k, k + Hkv * 256, slots, T, qkv.stride(0), qkv.stride(0))
+            _write_q8(dev, kv_cache, kv_scale, layout, k, k + Hkv * 256, slots, T, qkv.stride(0), qkv.stride(0))
         return qkv
     nb, _, bs, Hc, D = kv_cache.shape
     assert D == 128 and Hc == Hkv and qkv.dim() == 2 and qkv.stride(1) == 1 and qkv.shape[1] == (Hq + 2 * Hkv) * 128
@@ -705,12 +706,12 @@ def kv_gather(kv_cache: torch.Tensor, block_table_row: torch.Tensor, length: int
         row = _index(what, "block_table_row", block_table_row, torch.int32, entries)
         if not 0 <= length <= entries * bs:
             raise ValueError(f"{what}: {length} tokens, {entries} block-table entries of {bs}")
-        _on_current_device(what, kv_cache, kv_scale, row)
+        dev = _on_current_device(what, kv_cache, kv_scale, row)
         k = kv_cache.new_empty((length, Hkv, 128), dtype=torch.bfloat16)
         v = torch.empty_like(k)
         if length:
             rc = _function("mlf_kv_gather_q8", "ppipiiiiippu")(
-                kv_cache.data_ptr(), kv_scale.data_ptr(), fmt, row.data_ptr(), entries, length, Hkv, bs, nb, k.data_ptr(), v.data_ptr(), _stream())
+                kv_cache.data_ptr(), kv_scale.data_ptr(), fmt, row.data_ptr(), entries, length, Hkv, bs, nb, k.data_ptr(), v.data_ptr(), _stream(dev))
             _lib.check(rc, "mlf_kv_gather_q8")
         return k, v
     nb, _, bs, Hkv, D = kv_cache.shape
@@ -738,10 +739,11 @@ def kv_copy_blocks_(tensors: Sequence[torch.Tensor], pairs: Sequence[Tuple[int, 
     nb = tensors[0].size(0) if tensors[0].dim() else 0
     if 0 in sizes or not all(map(T.is_contiguous, tensors)) or any(len(s) == 0 or s[0] != nb for s in set(map(attrgetter("shape"), tensors))):
         raise ValueError(f"kv_copy_blocks_: tensors must be contiguous with the same number of blocks, got {[tuple(t.shape) for t in tensors]}")
-    if set(map(T.get_device, tensors)) != {torch._C._cuda_getDevice() if torch.cuda.is_initialized() else 0}:
+    dev = _on_current_device("kv_copy_blocks_", tensors[0])
+    if set(map(T.get_device, tensors)) != {dev}:
         _on_current_device("kv_copy_blocks_", *tensors)
     bases = array("Q", map(T.data_ptr, tensors))
-    rc = _function("mlf_kv_copy_blocks", "ppipiiu")(bases.buffer_info()[0], sizes.buffer_info()[0], len(tensors), flat.buffer_info()[0], len(pairs), nb, _stream())
+    rc = _function("mlf_kv_copy_blocks", "ppipiiu")(bases.buffer_info()[0], sizes.buffer_info()[0], len(tensors), flat.buffer_info()[0], len(pairs), nb, _stream(dev))
     _lib.check(rc, "mlf_kv_copy_blocks")
 
 
@@ -776,11 +778,11 @@ def sample_rows(logits: torch.Tensor, vocab: int, u: torch.Tensor, temperature: 
     top_k = _index(what, "top_k", top_k, torch.int32, rows) if top_k is not None else None
     top_p = _index(what, "top_p", top_p, torch.float32, rows) if top_p is not None else None
     min_p = _index(what, "min_p", min_p, torch.float32, rows) if min_p is not None else None
-    _on_current_device(what, logits, u, temperature, top_k, top_p, min_p)
+    dev = _on_current_device(what, logits, u, temperature, top_k, top_p, min_p)
     tokens = torch.empty(rows, dtype=torch.int64, device=logits.device)
     logprobs = torch.empty(rows, dtype=torch.float32, device=logits.device) if want_logprobs else None
     rc = _function("mlf_sample_rows", "pillipppppppu")(
         logits.data_ptr(), int(logits.dtype == torch.float32), rows, logits.stride(0), vocab, u.data_ptr(), temperature.data_ptr(), _at(top_k),
-        _at(top_p), _at(min_p), tokens.data_ptr(), _at(logprobs), _stream())
+        _at(top_p), _at(min_p), tokens.data_ptr(), _at(logprobs), _stream(dev))
     _lib.check(rc, "mlf_sample_rows")
     return (tokens, logprobs) if want_logprobs else tokens
