@@ -151,9 +151,10 @@ def test_argument_types_follow_the_entries():
 
 
 def test_splits_fill_one_round_at_most():
-    for pairs in (1, 2, 8, 31, 32, 104, 128, 200, 222, 223, 444, 512, 10000):
+    for pairs in (1, 2, 8, 31, 32, 104, 128, 200, 222, 223, 296, 297, 444, 512, 10000):
         for n in (0, 1, 128, 384, 385, 700, 1024, 2500, 4000, 60001, 1 << 20):
             splits = native._decode_splits_q8(pairs, n, 148)
-            assert 1 <= splits <= 96 and (splits == 1 or (splits * pairs <= 444 and n > 384 and -(-n // splits) >= 87))
+            assert 1 <= splits <= 96 and (splits == 1 or (splits * pairs <= (592 if splits == 2 and n >= 1500 else 444) and n > 384 and -(-n // splits) >= 87))
             assert splits == 1 or n // 128 >= splits - 1
+    assert native._decode_splits_q8(256, 4096, 148) == 2 and native._decode_splits_q8(256, 1000, 148) == 1
     assert native._decode_splits_q8(8, 4000, 148) == 16 and native._decode_splits_q8(512, 4000, 148) == 1

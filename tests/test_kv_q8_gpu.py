@@ -211,7 +211,7 @@ def test_attention_many_splits(dtype, split, bs, Hq):
 
 @pytest.mark.parametrize("dtype", KINDS)
 @pytest.mark.parametrize("B,n,Hq,Hkv", [(150, 333, 8, 4), (200, 300, 12, 4), (300, 60, 16, 8), (300, 130, 24, 8), (40, 100, 16, 8), (65, 450, 16, 8),
-                                        (130, 450, 8, 8), (160, 450, 16, 8), (300, 450, 4, 4)])
+                                        (130, 450, 8, 8), (160, 450, 16, 8), (300, 450, 4, 4), (30, 1600, 16, 8)])
 def test_attention_forms_of_the_launch(dtype, B, n, Hq, Hkv):
     """Four, three and two warps to a CTA: by the places that the rounds of CTAs take, and short sequences; then with the append."""
     g = _gen(B)
