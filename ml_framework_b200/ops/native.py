@@ -492,19 +492,20 @@ def _decode_split(pairs: int, max_seq_len: int, sms: int) -> int:
 
 
 @lru_cache(maxsize=4096)
-def _decode_splits_q8(pairs: int, max_seq_len: int, sms: int) -> int:
-    """Splits of the 8-bit decode kernel for ``pairs`` (sequence, KV head) pairs on ``sms`` SMs: one round of three CTAs on
-    each, of which every one has 128 tokens at least, 256 (all that its warps fetch at once) where that makes more than eight splits,
+def _decode_splits_q8(pairs: int, max_seq_len: int, sms: int, per_sm: int = 3, smaller: bool = True) -> int:
+    """Splits of the 8-bit decode kernel for ``pairs`` (sequence, KV head) pairs on ``sms`` SMs: one round of three CTAs
+    (``per_sm``: two for more than eight heads a group) on each, of which every one has 128 tokens at least, 256 (all that its warps fetch at once) where that makes more than eight splits,
     and 96 splits at most; none up to 384 tokens, where the merge costs more than it saves. Two of 1500 tokens or more also where
-    that makes one round of four smaller CTAs out of one of three that is two thirds full at most. us with 8 KV heads: 1 x 200 none 4.7
+    that makes one round of four ``smaller`` CTAs out of one of three that is two thirds full at most. us with 8 KV heads: 1 x 200 none 4.7
     (2: 5.5); 1 x 700 6 splits 5.3 (1: 8.6, 3: 6.5); 1 x 4000 16 8.6 (8: 9.0, 11: 10.4, 32: 10.1); 8 x 4000 6 18 (2: 31, 4: 21, 16: 24);
     13 x 2500 4 18 (1: 34, 3: 21, 5: 21); 16 x 4096 3 29 (1: 54, 2: 35, 4: 31); 48 x 4096 none 70 (2: 73); 4 x 60001 13 87 (8: 107,
     16: 86); 29 x 1500 2 25 (1: 27), 32 x 4096 2 51 (1: 60), 32 x 16384 2 177 (1: 217), 32 x 1000 none 20 (2: 20), 36 x 4096 2 58 (1: 61);
-    one KV head, 1 x 60000 96 20 (32: 22, 64: 19, 200: 23)."""
+    one KV head, 1 x 60000 96 20 (32: 22, 64: 19, 200: 23). Groups of 16: 13 x 2500 of 4 heads 5 18 (4: 20, 6: 33, 8: 30), 32 x 4096 2 40 (1: 56,
+    3: 57), 64 x 2000 none 34 (2: 47)."""
     most = 1 if max_seq_len <= 384 else max(min(8, -(-max_seq_len // 128)), min(96, -(-max_seq_len // 256)))
-    if 3 * sms < 2 * pairs <= 4 * sms and max_seq_len >= 1500:
+    if smaller and 3 * sms < 2 * pairs <= 4 * sms and max_seq_len >= 1500:
         return 2
-    return max(1, min(3 * sms // pairs, most))
+    return max(1, min(per_sm * sms // pairs, most))
 
 
 def _decode_q8(what: str, q: torch.Tensor, ldq: int, Hq: int, kv_cache, kv_scale, block_table, seq_lens, slots, max_seq_len: int, scale, split_tokens: int,
@@ -524,14 +525,14 @@ def _decode_q8(what: str, q: torch.Tensor, ldq: int, Hq: int, kv_cache, kv_scale
         return out
     if rows[1] == 0:
         return out.zero_()
-    sms = _sm_count(dev)
+    sms, per_sm = _sm_count(dev), 3 if Hq // Hkv <= 8 else 2
     if split_tokens <= 0:
-        splits = _decode_splits_q8(B * Hkv, max_seq_len, sms)
+        splits = _decode_splits_q8(B * Hkv, max_seq_len, sms, per_sm, per_sm == 3 and bs % 16 == 0)
     else:
         st = (max(split_tokens, 128) + 127) // 128 * 128
         splits = max(1, (max_seq_len + st - 1) // st)
     # maximum, sum and output of each split; up to eight that are resident at once are merged within the launch
-    within = splits <= 8 and (splits == 1 or B * Hkv * splits <= 3 * sms)
+    within = splits <= 8 and (splits == 1 or B * Hkv * splits <= per_sm * sms)
     ws = None if within else torch.empty(B * Hq * splits * 130, dtype=torch.float32, device=q.device)
     rc = _function("mlf_paged_decode_q8", "plppipppppliiiiiiiiffiu")(
         q.data_ptr(), ldq, kv_cache.data_ptr(), kv_scale.data_ptr(), fmt, table.data_ptr(), lens.data_ptr(), _at(slots), out.data_ptr(), _at(ws),

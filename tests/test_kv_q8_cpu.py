@@ -156,5 +156,6 @@ def test_splits_fill_one_round_at_most():
             splits = native._decode_splits_q8(pairs, n, 148)
             assert 1 <= splits <= 96 and (splits == 1 or (splits * pairs <= (592 if splits == 2 and n >= 1500 else 444) and n > 384 and -(-n // splits) >= 87))
             assert splits == 1 or n // 128 >= splits - 1
+            assert native._decode_splits_q8(pairs, n, 148, 2, False) * pairs <= max(pairs, 296)
     assert native._decode_splits_q8(256, 4096, 148) == 2 and native._decode_splits_q8(256, 1000, 148) == 1
     assert native._decode_splits_q8(8, 4000, 148) == 16 and native._decode_splits_q8(512, 4000, 148) == 1
