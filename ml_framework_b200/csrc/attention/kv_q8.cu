@@ -11,7 +11,7 @@
 // Bound by HBM in long calls (a row is read in 16 bits and written in 8), by the chain of loads slots - rows (slots - map - slots -
 // rows) in short ones. us (floor at 6.54 TB/s): 37 tokens of 8 heads 4 (0.03), 1111 6 (1.0), 2048 9 (1.9), 8192 17 (7.7), 32768 50 (31),
 // 4096 of 40 heads 33 (19).
-// The way back, q8_gather_kernel: 3159 tokens of 8 heads 8.5 (3.0), 8192 13 (7.7), 32768 41 (31).
+// The way back, q8_gather_kernel: 3159 tokens of 8 heads 5.5 (3.0), 8192 10 (7.7), 32768 34 (31).
 #include "../common/host.h"
 #include "../common/ptx.cuh"
 #include "../mlf_api.h"
@@ -233,34 +233,36 @@ __global__ void __launch_bounds__(QW_WARPS * 32, MAP ? 4 : 3) q8_write_kernel(co
 static_assert(QW_GROUP <= 32, "a lane for every token of a group");
 
 // out_k / out_v [len, Hkv, 128] bf16 <- pages of one sequence; sixteen threads a token and head, eight numbers of its key and of its
-// value each (16 bytes out: with sixteen numbers a thread, every store left half of its sectors to the next one), of four such
-// pairs at a time.
-constexpr int QG_PAIRS = 4;
-template <int FMT>
+// value each (16 bytes out: with sixteen numbers a thread, every store left half of its sectors to the next one), of PAIRS such
+// pairs at a time: one, or two from 64 K on (us with 1 / 2 / 4 a thread, with divisions for the shifts: 37 tokens of 8 heads 1.7 / 2.1 / 3.2, 3159 5.7 / 6.7 / 8.5, 8192
+// 11.3 / 11.1 / 13.4, 32768 39 / 36 / 41).
+template <int FMT, int PAIRS>
 __global__ void __launch_bounds__(256)
-q8_gather_kernel(const uint8_t* cache, const float* scale, const int* block_table, unsigned pairs, int Hkv, int block_size, int num_blocks,
-                 __nv_bfloat16* out_k, __nv_bfloat16* out_v, int* err) {   // tokens <= table entries * block_size (checked by the launcher)
+q8_gather_kernel(const uint8_t* cache, const float* scale, const int* block_table, unsigned pairs, int Hkv, int block_size, int hkv_shift, int bs_shift,
+                 int num_blocks, __nv_bfloat16* out_k, __nv_bfloat16* out_v, int* err) {   // tokens <= table entries * block_size (checked by the launcher)
   pdl_trigger();
   pdl_wait();
   const long long side = (long long)block_size * Hkv * Q8_D;
-  const unsigned first = blockIdx.x * (16 * QG_PAIRS) + (threadIdx.x >> 4), c = (threadIdx.x & 15) * 8;
-  uint2 k[QG_PAIRS], v[QG_PAIRS];
-  float sk[QG_PAIRS], sv[QG_PAIRS];
-  int blk[QG_PAIRS];
+  const unsigned first = blockIdx.x * (16 * PAIRS) + (threadIdx.x >> 4), c = (threadIdx.x & 15) * 8;
+  auto token_of = [&](unsigned i) { return hkv_shift >= 0 ? i >> hkv_shift : i / (unsigned)Hkv; };
+  auto entry_of = [&](unsigned t) { return bs_shift >= 0 ? t >> bs_shift : t / (unsigned)block_size; };
+  uint2 k[PAIRS], v[PAIRS];
+  float sk[PAIRS], sv[PAIRS];
+  int blk[PAIRS];
   bool bad = false;
 #pragma unroll
-  for (int e = 0; e < QG_PAIRS; ++e) {
+  for (int e = 0; e < PAIRS; ++e) {
     const unsigned i = first + 16 * e;
-    blk[e] = i < pairs ? block_table[i / (unsigned)Hkv / (unsigned)block_size] : 0;
+    blk[e] = i < pairs ? block_table[entry_of(token_of(i))] : 0;
   }
 #pragma unroll
-  for (int e = 0; e < QG_PAIRS; ++e) bad = bad || blk[e] < 0 || blk[e] >= num_blocks;
+  for (int e = 0; e < PAIRS; ++e) bad = bad || blk[e] < 0 || blk[e] >= num_blocks;
   if (bad) atomicCAS(err, 0, ERR_BAD_INDEX);
 #pragma unroll
-  for (int e = 0; e < QG_PAIRS; ++e) {
+  for (int e = 0; e < PAIRS; ++e) {
     const unsigned i = first + 16 * e;
     if (i < pairs) {
-      const unsigned t = i / (unsigned)Hkv, h = i - t * Hkv, b = t / (unsigned)block_size;
+      const unsigned t = token_of(i), h = i - t * Hkv, b = entry_of(t);
       if (blk[e] < 0 || blk[e] >= num_blocks) blk[e] = 0;
       const uint8_t* src = cache + 2 * side * blk[e] + ((long long)(t - b * block_size) * Hkv + h) * Q8_D + c;
       const float* s = scale + (long long)blk[e] * 2 * Hkv + h;
@@ -271,7 +273,7 @@ q8_gather_kernel(const uint8_t* cache, const float* scale, const int* block_tabl
     }
   }
 #pragma unroll
-  for (int e = 0; e < QG_PAIRS; ++e) {
+  for (int e = 0; e < PAIRS; ++e) {
     const unsigned i = first + 16 * e;
     if (i >= pairs) continue;
     auto put = [&](uint2 q, float f, __nv_bfloat16* out) {
@@ -282,6 +284,13 @@ q8_gather_kernel(const uint8_t* cache, const float* scale, const int* block_tabl
     put(k[e], sk[e], out_k);
     put(v[e], sv[e], out_v);
   }
+}
+
+// log2 of a power of two, else -1
+static int shift_of(int n) {
+  for (int sh = 0; sh < 31; ++sh)
+    if ((1 << sh) == n) return sh;
+  return -1;
 }
 
 }  // namespace mlf
@@ -304,8 +313,7 @@ MLF_API int mlf_kv_write_q8(void* cache, float* scale, int fmt, const void* k, c
   p.k = static_cast<const __nv_bfloat16*>(k);
   p.v = static_cast<const __nv_bfloat16*>(v);
   p.slots = slots;
-  p.bs_shift = -1;
-  for (int sh = 0; sh < 31; ++sh) if ((1 << sh) == block_size) p.bs_shift = sh;
+  p.bs_shift = shift_of(block_size);
   const bool few = T <= QW_FEW && block_size <= QW_ROWS;
   MLF_REQUIRE(few || map != nullptr, "kv_write_q8: %lld tokens into blocks of %d need a map", T, block_size);
   p.map = few ? nullptr : map;
@@ -334,11 +342,12 @@ MLF_API int mlf_kv_gather_q8(const void* cache, const float* scale, int fmt, con
               table_len);
   MLF_REQUIRE((reinterpret_cast<uintptr_t>(cache) & 15) == 0, "kv_gather_q8: the cache must be 16-byte aligned");
   MLF_REQUIRE((long long)len * Hkv < (1LL << 31), "kv_gather_q8: %d tokens of %d heads", len, Hkv);
-  const unsigned pairs = (unsigned)len * (unsigned)Hkv, g = (pairs + 16 * QG_PAIRS - 1) / (16 * QG_PAIRS);
-  const auto kernel = fmt == Q8_E4M3 ? q8_gather_kernel<Q8_E4M3> : q8_gather_kernel<Q8_INT8>;
+  const unsigned pairs = (unsigned)len * (unsigned)Hkv, each = pairs >= 65536 ? 2 : 1, g = (pairs + 16 * each - 1) / (16 * each);
+  const auto kernel = fmt == Q8_E4M3 ? (each == 1 ? q8_gather_kernel<Q8_E4M3, 1> : q8_gather_kernel<Q8_E4M3, 2>)
+                                     : (each == 1 ? q8_gather_kernel<Q8_INT8, 1> : q8_gather_kernel<Q8_INT8, 2>);
   MLF_CHECK_CUDA(launch_pdl(kernel, dim3(g), dim3(256), 0, reinterpret_cast<cudaStream_t>(stream), static_cast<const uint8_t*>(cache), scale,
-                            block_table, pairs, Hkv, block_size, num_blocks, static_cast<__nv_bfloat16*>(out_k), static_cast<__nv_bfloat16*>(out_v),
-                            device_status_word()));
+                            block_table, pairs, Hkv, block_size, shift_of(Hkv), shift_of(block_size), num_blocks, static_cast<__nv_bfloat16*>(out_k),
+                            static_cast<__nv_bfloat16*>(out_v), device_status_word()));
   count_launch();
   return 0;
 }
