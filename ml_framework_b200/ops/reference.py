@@ -76,11 +76,12 @@ def attention_ref(q, k, v, *, causal=True, scale=None, start_pos: int = 0):
     return o, lse
 
 
-def paged_attention_ref(q, kv_cache, block_table, seq_lens, *, scale=None):
+def paged_attention_ref(q, kv_cache, block_table, seq_lens, *, scale=None, kv_scale=None):
     """Decode attention through a block table.
 
     q [B, Hq, D]; kv_cache [num_blocks, 2, block_size, Hkv, D]; block_table [B, max_blocks]
     (int32); seq_lens [B] = number of cached tokens including the current one. Returns [B, Hq, D].
+    kv_scale [num_blocks, 2, Hkv]: the scales of an 8-bit cache. A sequence's own blocks are all that is converted.
     """
     B, Hq, D = q.shape
     bs = kv_cache.shape[2]
@@ -89,8 +90,9 @@ def paged_attention_ref(q, kv_cache, block_table, seq_lens, *, scale=None):
         n = int(seq_lens[b])
         nb = (n + bs - 1) // bs
         blocks = block_table[b, :nb].long()
-        k = kv_cache[blocks, 0].reshape(nb * bs, -1, D)[:n]
-        v = kv_cache[blocks, 1].reshape(nb * bs, -1, D)[:n]
+        pages = kv_values_ref(kv_cache[blocks], kv_scale[blocks] if kv_scale is not None else None)
+        k = pages[:, 0].reshape(nb * bs, -1, D)[:n]
+        v = pages[:, 1].reshape(nb * bs, -1, D)[:n]
         o, _ = attention_ref(q[b][None, None], k[None], v[None], causal=False, scale=scale)
         outs.append(o[0, 0])
     return torch.stack(outs)

@@ -481,10 +481,7 @@ class PagedLlamaExecutor:
         def attend(li, q, k, v):
             if self.cfg.torch_ops:
                 return self._attend_torch_decode(li, q, table, lens, max_len)
-            cache, kv_scale = self.kv.caches[li], self.kv.scales[li]
-            if kv_scale is not None:
-                cache = reference.kv_values_ref(cache, kv_scale)
-            return reference.paged_attention_ref(q, cache, table.cpu(), lens.cpu().tolist()).to(q.dtype)
+            return reference.paged_attention_ref(q, self.kv.caches[li], table.cpu(), lens.cpu().tolist(), kv_scale=self.kv.scales[li]).to(q.dtype)
 
         def attend_packed(li, qkv):
             return native.paged_decode_rope(qkv, self.kv.caches[li], table, lens, slots, self.hq, self.hkv, max_len, self.mc.rope_theta,

@@ -99,7 +99,7 @@ class PagedAttentionLayer(nn.Module):
             if nat:
                 a = native.paged_decode(q, cache, table, lens, int(max(st + 1 for st in starts)), split_tokens=512 if scale is None else 0, kv_scale=scale)
             else:
-                a = reference.paged_attention_ref(q.float(), reference.kv_values_ref(cache, scale), table, lens).to(x.dtype)
+                a = reference.paged_attention_ref(q.float(), cache, table, lens, kv_scale=scale).to(x.dtype)
         else:
             outs, off = [], 0
             for i, (n, st) in enumerate(zip(n_tokens, starts)):
