@@ -734,7 +734,7 @@ def kv_copy_blocks_(tensors: Sequence[torch.Tensor], pairs: Sequence[Tuple[int, 
     at most and none is both read and written, so that no order of the copies matters; anything else is refused."""
     tensors = list(tensors)
     flat = array("i", chain.from_iterable(pairs))
-    if len(flat) != 2 * len(pairs):
+    if not set(map(len, pairs)) <= {2}:
         raise ValueError("kv_copy_blocks_: pairs must be (source, destination) block numbers")
     if not tensors or not flat:
         return
