@@ -21,6 +21,7 @@ import collections
 import enum
 import heapq
 import itertools
+import operator
 import random
 import threading
 import time
@@ -59,6 +60,12 @@ class RequestState(enum.Enum):
 _ids = itertools.count(1)
 
 
+def _number(name: str, v) -> float:
+    if isinstance(v, (str, bytes)):
+        raise TypeError(f"{name} must be a number, got {v!r}")
+    return float(v)
+
+
 @dataclass
 class SamplingParameters:
     """How a request's tokens are drawn (``native.sample_rows`` has the definition). ``temperature`` 0: the likeliest token.
@@ -70,6 +77,10 @@ class SamplingParameters:
     seed: Optional[int] = None
 
     def __post_init__(self):
+        # plain numbers from here on: another type would end the step of every request in the batch
+        self.temperature, self.top_p, self.min_p = (_number(n, getattr(self, n)) for n in ("temperature", "top_p", "min_p"))
+        self.top_k = operator.index(self.top_k)
+        self.seed = operator.index(self.seed) if self.seed is not None else None
         if not 0.0 <= self.temperature < float("inf"):
             raise ValueError(f"temperature must be finite and not negative, got {self.temperature}")
         if self.top_k < 0 or self.top_k >= 1 << 31 or not 0.0 <= self.top_p <= 1.0 or not 0.0 <= self.min_p <= 1.0:
