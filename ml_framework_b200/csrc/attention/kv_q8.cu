@@ -91,8 +91,9 @@ __device__ __noinline__ void q8_shrink8(uint2* at, float ratio) {
 }
 
 // A block's rows of one head and side. known: the tokens of its rows (-1: not written by this call), the first 16 of them with a map.
+// True where the block keeps a scale that is no power of two: nothing is written, its rows are left to q8_write_divided.
 template <int FMT, bool MAP>
-__device__ __forceinline__ void q8_write_rows(const Q8WriteParams& p, int blk, int h, int side, const int* known) {
+__device__ __forceinline__ bool q8_write_rows(const Q8WriteParams& p, int blk, int h, int side, const int* known) {
   const int lane = threadIdx.x & 31, half = lane >> 4, col = (lane & 15) * 8;
   const long long first = (long long)blk * p.block_size, pitch = (long long)p.Hkv * Q8_D;
   const __nv_bfloat16* src = (side ? p.v : p.k) + (long long)h * Q8_D + col;
@@ -140,6 +141,7 @@ __device__ __forceinline__ void q8_write_rows(const Q8WriteParams& p, int blk, i
   const float amax = __uint_as_float(__reduce_max_sync(0xffffffffu, max(__float_as_uint(__low2float(numbers)), __float_as_uint(__high2float(numbers)))));
   const float fit = q8_scale_for<FMT>(amax), before = anew ? 0.f : held_scale;
   const float now = fmaxf(before, fit);
+  if (!q8_power_of_two(now)) return true;
   const float inv = __frcp_rn(now), ratio = before * inv;     // exact for powers of two
   const bool shrink = !anew && before < now, plain = with_nan <= 0x7f800000u && amax * inv <= 127.f;
   for (int c = 0; c < chunks; ++c) {
@@ -162,6 +164,23 @@ __device__ __forceinline__ void q8_write_rows(const Q8WriteParams& p, int blk, i
     }
   }
   if (lane == 0) *scale = now;
+  return false;
+}
+// A row at a time and read again, behind the other units: the way that calls take holds no registers for it.
+template <int FMT, bool MAP>
+__device__ __forceinline__ void q8_write_divided(const Q8WriteParams& p, int blk, int h, int side, const int* known, float scale) {
+  const int half = (threadIdx.x & 31) >> 4, col = (threadIdx.x & 15) * 8;
+  const __nv_bfloat16* src = (side ? p.v : p.k) + (long long)h * Q8_D + col;
+  uint8_t* dst = p.cache + (((long long)blk * 2 + side) * p.block_size * p.Hkv + h) * Q8_D + col;
+#pragma unroll 1
+  for (int row = half; row < p.block_size; row += 2) {
+    const int t = !MAP || row < 16 ? known[row] : q8_token_at(p, (long long)blk * p.block_size + row);
+    if (t < 0) continue;
+    const uint4 x = *reinterpret_cast<const uint4*>(src + (long long)t * (side ? p.ldv : p.ldk));
+    const float2 a = unpack_bf16x2(x.x), b = unpack_bf16x2(x.y), e = unpack_bf16x2(x.z), f = unpack_bf16x2(x.w);
+    *reinterpret_cast<uint2*>(dst + (long long)row * p.Hkv * Q8_D) =
+        make_uint2(q8_divide4<FMT>(a.x, a.y, b.x, b.y, scale), q8_divide4<FMT>(e.x, e.y, f.x, f.y, scale));
+  }
 }
 
 // Three CTAs on an SM without a map, four with one: registers against loads in flight (us with three / four: 37 tokens of 8 heads 4.1 / 5.1,
@@ -225,9 +244,19 @@ __global__ void __launch_bounds__(QW_WARPS * 32, MAP ? 4 : 3) q8_write_kernel(co
   }
   __syncthreads();
   const int units = 2 * p.Hkv;
+  bool left = false;
   for (int i = 0; i < n; ++i) {
     if (s_blk[i] < 0) continue;
-    for (int u = blockIdx.y * QW_WARPS + warp; u < units; u += gridDim.y * QW_WARPS) q8_write_rows<FMT, MAP>(p, s_blk[i], u >> 1, u & 1, s_tok[i]);
+    for (int u = blockIdx.y * QW_WARPS + warp; u < units; u += gridDim.y * QW_WARPS) left |= q8_write_rows<FMT, MAP>(p, s_blk[i], u >> 1, u & 1, s_tok[i]);
+  }
+  if (!left) return;
+  __syncwarp();                                // the scales that grew are lane 0's to write
+  for (int i = 0; i < s_blocks; ++i) {
+    if (s_blk[i] < 0) continue;
+    for (int u = blockIdx.y * QW_WARPS + (threadIdx.x >> 5); u < 2 * p.Hkv; u += gridDim.y * QW_WARPS) {
+      const float scale = p.scale[((long long)s_blk[i] * 2 + (u & 1)) * p.Hkv + (u >> 1)];
+      if (!q8_power_of_two(scale)) q8_write_divided<FMT, MAP>(p, s_blk[i], u >> 1, u & 1, s_tok[i], scale);
+    }
   }
 }
 static_assert(QW_GROUP <= 32, "a lane for every token of a group");

@@ -4,7 +4,7 @@
 // Scales that the kernels write are powers of two, 2^-40 .. 2^40: the smallest under which the block's largest magnitude fits
 // (448 for e4m3, 127 for int8). Dividing by one is exact, so that a number is rounded once, and a block whose scale grows
 // while rows are appended to it is rounded to the coarser step without a second error of the division. A reader takes any
-// positive scale.
+// positive scale, and a block that came with one keeps it until rows need a larger one.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -42,6 +42,14 @@ __device__ __forceinline__ unsigned q8_pack4(float a, float b, float c, float d)
   asm("cvt.pack.sat.s8.s32.b32 %0, %1, %2, 0;" : "=r"(hi) : "r"(w), "r"(z));
   asm("cvt.pack.sat.s8.s32.b32 %0, %1, %2, %3;" : "=r"(all) : "r"(y), "r"(x), "r"(hi));
   return all;
+}
+
+// Numbers in 8 bits under a scale that came with the block and is no power of two: times its inverse, which is rounded, a number half way
+// between two steps came to the wrong one of them, and to different ones in an append and in a write.
+__device__ __forceinline__ bool q8_power_of_two(float scale) { return (__float_as_uint(scale) & 0x7fffffu) == 0; }
+template <int FMT>
+__device__ __forceinline__ unsigned q8_divide4(float a, float b, float c, float d, float scale) {
+  return q8_pack4<FMT>(__fdiv_rn(a, scale), __fdiv_rn(b, scale), __fdiv_rn(c, scale), __fdiv_rn(d, scale));
 }
 
 // The four numbers of a word as two f16 pairs, (byte 0, byte 1) and (byte 2, byte 3): every one of both types is exact in f16.

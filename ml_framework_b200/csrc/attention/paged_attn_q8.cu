@@ -138,7 +138,7 @@ __device__ __forceinline__ unsigned q8_append_row(const DecodeQ8Params& p, float
     }
   }
   const float inv = __frcp_rn(now);
-  const unsigned w = q8_pack4<FMT>(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+  const unsigned w = q8_power_of_two(now) ? q8_pack4<FMT>(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv) : q8_divide4<FMT>(x[0], x[1], x[2], x[3], now);
   if (dst != nullptr) *reinterpret_cast<unsigned*>(dst) = w;
   return w;
 }
