@@ -115,9 +115,11 @@ __device__ __forceinline__ float sm_entry_value(u64 e) { return sm_value(~(unsig
 template <bool BF16>
 struct SampleWeight {
   float m, ch, cl;                             // 32 log2(e) / T in two floats
+  float above;                                 // fp32: only logits above this weigh anything: -inf, beside infinite ones the largest finite number
   const unsigned* table;                       // 2^(j / 32) in units of 2^-31, one of the 32 banks each: any lanes read at once
   __device__ __forceinline__ u64 operator()(float x) const {     // NaN and -inf: 0
-    x = fminf(x, FLT_MAX);
+    // bf16: the callers pass no NaN, and the largest number is too far below FLT_MAX to weigh anything beside it
+    x = BF16 || x > above ? fminf(x, FLT_MAX) : -INFINITY;
     const float s = __fsub_rn(x, m), t = __fadd_rn(s, m);
     const float r = BF16 ? __fsub_rn(x, t) : __fadd_rn(__fsub_rn(x, __fsub_rn(s, __fsub_rn(s, x))), -__fadd_rn(m, __fsub_rn(s, x)));
     const float p = fmaxf(__fmul_rn(s, ch), -2000.f);                               // 32nds of the exponent; 2^-62 is none
@@ -655,6 +657,7 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_rows_kernel(const Sample
   SampleWeight<sizeof(T) == 2> weight;
   const double scale = 32. * 1.4426950408889634074 / (double)temp;
   weight.m = fminf(m, FLT_MAX);
+  weight.above = m == INFINITY ? FLT_MAX : -INFINITY;
   weight.ch = (float)scale;
   weight.cl = (float)(scale - (double)weight.ch);
   weight.table = s.exp2;
