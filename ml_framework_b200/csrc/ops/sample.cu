@@ -110,8 +110,9 @@ __device__ __forceinline__ u64 sm_entry(float x, int i) { return (u64)(~sm_key(x
 __device__ __forceinline__ float sm_entry_value(u64 e) { return sm_value(~(unsigned)(e >> 32)); }
 
 // x - m as the sum of two floats. Logits that were rounded to bf16 (8 bits): exact in one where the two are within 2^16 of each other,
-// the second is their difference's rounding where m is the larger, and where x is it is lost (2^-24 of x, which is then that
-// far below m). Others: always exact.
+// the second is their difference's rounding where m is the larger. Where x is, the rounding would be lost, 2^-24 of x: a
+// largest logit so near 0 that a logit with a weight can be 2^16 times as large is left out, m = 0, and every weight is exp(largest / T)
+// times as large. Others: always exact.
 template <bool BF16>
 struct SampleWeight {
   float m, ch, cl;                             // 32 log2(e) / T in two floats
@@ -656,7 +657,8 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_rows_kernel(const Sample
   var = n_mean > 0.f ? fmaxf(__fdiv_rn(var, n_mean) - mean * mean, 0.f) : 0.f;
   SampleWeight<sizeof(T) == 2> weight;
   const double scale = 32. * 1.4426950408889634074 / (double)temp;
-  weight.m = fminf(m, FLT_MAX);
+  // bf16: above 2^-11 T nothing down to 29 T below it is 2^16 times as large
+  weight.m = sizeof(T) == 2 && fabsf(m) < 0x1p-11f * temp ? 0.f : fminf(m, FLT_MAX);
   weight.above = m == INFINITY ? FLT_MAX : -INFINITY;
   weight.ch = (float)scale;
   weight.cl = (float)(scale - (double)weight.ch);
@@ -664,7 +666,7 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_rows_kernel(const Sample
   auto finish = [&](long long token, float x, u64 total) {  // one thread of the row
     p.tokens[r] = token;
     if (p.logprobs) {
-      const double lw = x == m ? 0. : ((double)x - (double)m) / (double)temp;
+      const double lw = ((double)fminf(x, FLT_MAX) - (double)weight.m) / (double)temp;
       p.logprobs[r] = (float)(lw - log((double)total * (1. / (double)(1ull << SM_ONE))));
     }
   };
