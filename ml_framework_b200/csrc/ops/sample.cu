@@ -7,10 +7,11 @@
 // counts as 2^90 (beyond either, the differences of logits that matter, or the second float of log2(e) / T, are no normal fp32 numbers).
 // NaN counts as -inf, a subnormal logit as 0.
 //
-// Weights are integers, w_i rounded to 2^-40, from an exponential that is good to about 2^-30: x - m and the product with
+// Weights are integers, w_i rounded to 2^-40, from an exponential that is good to about 2^-30, 2^-28 at worst: x - m and the product with
 // log2(e) / T are carried in two floats, 2^(j/32) comes from a table and the rest from a polynomial. Sums of integers do not depend on
-// their order, so that a row gives the same token in any batch and with any number of CTAs, and a border between
-// two tokens is as sharp as the weights themselves.
+// their order, so that a row gives the same token in any batch and with any number of CTAs. What is lost is the rounding
+// of each weight, alike for equal ones: a border between two tokens lies within 2^-28 + vocab 2^-41 of the total from where the
+// definition has it (2^20 logits 28 T below one large one sum to 2^-20 where the definition has 0.76 of that).
 //
 // A cluster of CTAs takes a row, and each lane keeps its logits in shared memory where four steps of 256 a warp are enough; rows of
 // more are read again in every pass, from the caches, and their lanes' maxima of eight neighbours are kept instead. A pass costs

@@ -770,7 +770,8 @@ def sample_rows(logits: torch.Tensor, vocab: int, u: torch.Tensor, temperature: 
     With w_i = exp((x_i - max x) / temperature), in the order of x (of equal ones the lower index first): the first top_k tokens
     are kept; of these the shortest prefix whose weights reach top_p of theirs; of these those with w_i >= min_p; the first one in any
     case. The token is the first one, by index, at which the running sum of the kept weights exceeds u times their total. A row gives the same token
-    whatever stands in the other rows. NaN counts as -inf; a row without any other logit gives token 0. With
+    whatever stands in the other rows. Weights are multiples of 2^-40 of the largest: a border between two tokens lies within 2^-28 +
+    vocab * 2^-41 of the total from its place, and what weighs less than 2^-41 is never drawn. NaN counts as -inf; a row without any other logit gives token 0. With
     ``want_logprobs``: (tokens, logprobs), float32 [rows], the logarithm of the token's probability among the kept ones (0 for
     the largest logit alone, -inf for a row of -inf)."""
     what, vocab = "sample_rows", int(vocab)
