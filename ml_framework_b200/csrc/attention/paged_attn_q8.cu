@@ -62,7 +62,8 @@ struct DecodeQ8Params {
   const int* seq_lens;            // [B]
   __nv_bfloat16* out;             // [B, Hq, 128]
   float* ws;                      // [B, Hkv, splits, G, 130] (m, l, o[128]): splits that a second kernel merges
-  int B, Hq, Hkv, G, block_size, bs_shift, max_blocks, num_blocks, splits, unit;   // bs_shift: log2(block_size) or -1; unit: tokens that a split is a multiple of
+  int B, Hq, Hkv, G, block_size, bs_shift, max_blocks, num_blocks, splits;   // bs_shift: log2(block_size) or -1
+  unsigned unit;                  // tokens that a split is a multiple of
   float scale_log2;
   int* err;
   // packed form: unrotated heads of packed QKV rows; the newest token goes to slots[b]
@@ -180,8 +181,9 @@ paged_decode_q8_kernel(const DecodeQ8Params p, const __grid_constant__ CUtensorM
     len = len < 0 ? 0 : (int)cap;
   }
   // a split is a whole number of blocks, so that a block whose scale grows with its newest row is read by one CTA alone
-  const int per = ((len + p.splits - 1) / p.splits + p.unit - 1) / p.unit * p.unit;
-  const int t_lo = min(len, sp * per), t_hi = min(len, t_lo + per);
+  // (a unit is below 2^31, and a split behind the last token may begin beyond 2^32)
+  const unsigned per = ((unsigned)(len + p.splits - 1) / (unsigned)p.splits + p.unit - 1) / p.unit * p.unit;
+  const int t_lo = (int)min((unsigned long long)len, (unsigned long long)sp * per), t_hi = (int)min((unsigned)len, (unsigned)t_lo + per);
   float* ws = p.ws ? p.ws + (((long long)b * p.Hkv + hkv) * p.splits + sp) * p.G * DQ_RED : nullptr;
   // behind the warps' partial results in shared memory: this CTA's, for the others of its cluster
   float* mine_out = reinterpret_cast<float*>(dq_smem) + W * p.G * DQ_RED;
