@@ -549,6 +549,11 @@ paged_decode_q8_kernel(const DecodeQ8Params p, const __grid_constant__ CUtensorM
   }
   if (!WHOLE) dq_wait<0>();
   __syncthreads();                             // the rings are free
+  if (WHOLE && s_abort) {                      // a wait ran out: boxes still under way get time to land first
+    const long long t0 = clock64();
+    while (clock64() - t0 < 2000000LL) __nanosleep(1000);
+    __syncthreads();
+  }
   // ---- merge the four warps: red[warp][head][m, l, o[128]]
   float* red = reinterpret_cast<float*>(dq_smem);
 #pragma unroll
