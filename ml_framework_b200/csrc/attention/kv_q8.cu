@@ -9,8 +9,8 @@
 // nothing at all, point at tokens of other slots.
 //
 // Bound by HBM in long calls (a row is read in 16 bits and written in 8), by the chain of loads slots - rows (slots - map - slots -
-// rows) in short ones. us (floor at 6.54 TB/s): 37 tokens of 8 heads 4 (0.03), 1111 6 (1.0), 2048 9 (1.9), 8192 17 (7.7), 32768 50 (31),
-// 4096 of 40 heads 33 (19).
+// rows) in short ones. us with rows, cache and scales in HBM (floor at 6.54 TB/s): 37 tokens of 8 heads 4.6 (0.03), 1111 7 (1.0), 2048 9 (1.9), behind
+// 1111 others 11, 8192 17 (7.7), 32768 49 (31), 4096 of 40 heads 32 (19).
 // The way back, q8_gather_kernel: 3159 tokens of 8 heads 5.5 (3.0), 8192 10 (7.7), 32768 34 (31).
 #include "../common/host.h"
 #include "../common/ptx.cuh"

@@ -32,7 +32,7 @@
 // counts (some 16 clocks for 32 logits) and, with fp32 logits in (3), both for many; rows that take longest start first where not all
 // run at once. us for 1 / 256 rows of 128256 bf16 logits (floor 0.04 / 10): largest logit 3 / 20, k = 50 with p 10 / 45, k = 1000
 // 32 / 138, no limit 10 / 89, a p that keeps few 14 / 94, one that keeps thousands 20 / 138 - 156, rows of all kinds - / 80; of fp32 logits
-// (floor 0.08 / 20) a p that keeps few 19 / 187, thousands 28 / 240.
+// (floor 0.08 / 20) a p that keeps few 19 / 192, thousands 30 / 248.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <float.h>
